@@ -328,6 +328,80 @@ int w4a4_rope_qk_bf16(void* q, int64_t ldq, int32_t heads_q, void* k, int64_t ld
 int w4a4_layer_norm_bf16(const void* x, void* y, int64_t rows, int32_t h, const void* w, const void* b,
                          float eps, void* stream);
 
+/* ---- 8-bit serving operators ----
+ * No counterpart in the reference, which keeps the neighbours of its W4A4
+ * path in bf16.  Activations and weights as int8 codes with an fp32 scale for
+ * each token and output channel, and a key/value cache in int8 with an fp32
+ * scale for each block of 16 tokens and head; a value is code x scale.  Sums,
+ * norms and softmax statistics are fp32 (products of codes int32); results
+ * are rounded once.  Element types are W4A4_F32, W4A4_F16 or W4A4_BF16. */
+#define W4A4_F32 0
+#define W4A4_F16 1
+#define W4A4_BF16 2
+
+/* Residual addition + RMSNorm + 8-bit codes: per row
+ *   s = x + gate * delta (delta NULL: s = x; gate NULL: 1), total = s rounded
+ *   y = s rsqrt(mean(s^2) + eps) gain + shift (shift NULL: 0)
+ *   scale = amax|y| / 127, codes = rint(y / scale)
+ * x, delta and gate of type `dtype`, gain and shift fp32; gate, gain and shift
+ * rows of h for each observation of rows_per_batch rows, `*_stride` elements
+ * apart (0: one row for all).  total (NULL: not stored) is [rows, h]
+ * contiguous; codes have row stride ldc.  Any h > 0 and alignment; rows that
+ * begin at multiples of 16 bytes (codes: 8) with h % 8 == 0 run vectorised. */
+int w4a4_rms_norm_quant8(const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* gate,
+                         int64_t gate_stride, const float* gain, int64_t gain_stride, const float* shift,
+                         int64_t shift_stride, float eps, int32_t dtype, int64_t rows, int32_t rows_per_batch,
+                         int32_t h, void* total, int8_t* codes, int64_t ldc, float* scale, void* stream);
+
+/* 8-bit codes of rows of x, or with `up` of gelu_tanh(x) * up: scale =
+ * amax / 127, codes = rint(value / scale). */
+int w4a4_quant8(const void* x, int64_t ldx, const void* up, int64_t ldu, int32_t dtype, int64_t rows, int32_t h,
+                int8_t* codes, int64_t ldc, float* scale, void* stream);
+
+/* out[r, :] = codes[r, :] * scale[r] ([rows, h] contiguous, of type dtype). */
+int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t dtype, int64_t rows, int32_t h,
+                  void* out, void* stream);
+
+/* y[m, n] = (sum_k a[m, k] w[n, k]) sa[m] sw[n] + bias[n]: a int8 [m, k] and w
+ * int8 [n, k], rows at multiples of 16 bytes (k itself arbitrary, below
+ * 131072); y [m, n] contiguous and bias (or NULL) of type dtype. */
+int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
+               const void* bias, int32_t dtype, int64_t m, int32_t n, int32_t k, void* y, void* stream);
+
+/* The 8-bit cache: codes int8 [batch, capacity, heads, width] for keys and
+ * values (cache_stride: elements of batch, token, head; multiples of 16),
+ * scales fp32 [batch, heads, capacity / 16] contiguous; width 64, 128, 192 or
+ * 256, capacity a multiple of 16.
+ *
+ * Writes the valid tokens (valid uint8 [batch, tokens], NULL: all) of k and v
+ * ([batch, tokens, heads, width], strides of batch, token, head) without gaps
+ * to the slots from start[b] on, and lengths[b] = start[b] + their number.  A
+ * block that keeps earlier tokens keeps its scale unless the new ones need a
+ * larger one, to which the earlier codes are then rounded again.  Tokens past
+ * the capacity are dropped, a start outside [0, capacity] writes nothing;
+ * both set bit 7 of the device error word. */
+int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, const int64_t* cache_stride,
+                    int32_t capacity, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                    int32_t dtype, const uint8_t* valid, int64_t valid_stride, const int32_t* start, int32_t* lengths,
+                    int32_t batch, int32_t tokens, int32_t heads, int32_t width, void* stream);
+
+/* The keys and values the cache stands for, [batch, capacity, heads, width]
+ * contiguous of type dtype, zero from lengths[b] on. */
+int w4a4_kv8_values(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                    const int64_t* cache_stride, int32_t capacity, const int32_t* lengths, int32_t dtype, int32_t batch,
+                    int32_t heads, int32_t width, void* k_out, void* v_out, void* stream);
+
+/* Attention of q [batch, tokens, q_heads, width] (strides of batch, token,
+ * head) over the cache's first lengths[b] tokens: softmax(scale q k^T) v, each
+ * group of q_heads / heads query heads sharing a key/value head.  causal: query
+ * t sees the keys below lengths[b] - tokens + t + 1 (the queries are the
+ * cache's last tokens).  A query that sees no key gives zeros.  out like q,
+ * contiguous. */
+int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_codes, const int8_t* v_codes,
+                    const float* k_scale, const float* v_scale, const int64_t* cache_stride, int32_t capacity,
+                    const int32_t* lengths, int32_t dtype, int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads,
+                    int32_t width, int32_t causal, float scale, void* out, void* stream);
+
 /* Library ABI version (major * 100 + minor). */
 int w4a4_version(void);
 

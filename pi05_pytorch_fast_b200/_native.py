@@ -26,6 +26,9 @@ CODES_GEMM = 2
 LAYOUT_ROW_MAJOR = 0
 LAYOUT_FRAGMENT_MAJOR = 1
 LAYOUT_INT8 = 2
+F32, F16, BF16 = 0, 1, 2
+KV8_BLOCK = 16
+ERR_CACHE_FULL = 1 << 7
 ROTATE_BY_K = -1
 GEMM_SINGLE_CTA = 0
 GEMM_CTA_PAIR = 1
@@ -55,6 +58,13 @@ EXPORTED_SYMBOLS = (
     "w4a4_ada_rms_norm_bf16",
     "w4a4_rope_qk_bf16",
     "w4a4_layer_norm_bf16",
+    "w4a4_rms_norm_quant8",
+    "w4a4_quant8",
+    "w4a4_dequant8",
+    "w4a4_gemm8",
+    "w4a4_kv8_append",
+    "w4a4_kv8_values",
+    "w4a4_attention8",
     "w4a4_last_error",
     "w4a4_device_error",
     "w4a4_set_wait_limit_ns",
@@ -114,6 +124,17 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.w4a4_ada_rms_norm_bf16.argtypes = [vp, vp, c_i64, c_i32, c_i32, vp, vp, c_i64, ctypes.c_float, vp]
     lib.w4a4_rope_qk_bf16.argtypes = [vp, c_i64, c_i32, vp, c_i64, c_i32, vp, vp, c_i64, c_i32, vp]
     lib.w4a4_layer_norm_bf16.argtypes = [vp, vp, c_i64, c_i32, vp, vp, ctypes.c_float, vp]
+    c_f32, strides = ctypes.c_float, ctypes.POINTER(c_i64)
+    lib.w4a4_rms_norm_quant8.argtypes = [vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, vp, c_i64, c_f32, c_i32, c_i64,
+                                         c_i32, c_i32, vp, vp, c_i64, vp, vp]
+    lib.w4a4_quant8.argtypes = [vp, c_i64, vp, c_i64, c_i32, c_i64, c_i32, vp, c_i64, vp, vp]
+    lib.w4a4_dequant8.argtypes = [vp, c_i64, vp, c_i32, c_i64, c_i32, vp, vp]
+    lib.w4a4_gemm8.argtypes = [vp, c_i64, vp, vp, c_i64, vp, vp, c_i32, c_i64, c_i32, c_i32, vp, vp]
+    lib.w4a4_kv8_append.argtypes = [vp, vp, vp, vp, strides, c_i32, vp, strides, vp, strides, c_i32, vp, c_i64, vp, vp,
+                                    c_i32, c_i32, c_i32, c_i32, vp]
+    lib.w4a4_kv8_values.argtypes = [vp, vp, vp, vp, strides, c_i32, vp, c_i32, c_i32, c_i32, c_i32, vp, vp, vp]
+    lib.w4a4_attention8.argtypes = [vp, strides, vp, vp, vp, vp, strides, c_i32, vp, c_i32, c_i32, c_i32, c_i32, c_i32,
+                                    c_i32, c_i32, c_f32, vp, vp]
     lib.w4a4_last_error.argtypes = [ctypes.c_char_p, ctypes.c_size_t]
     lib.w4a4_device_error.argtypes = [ctypes.POINTER(ctypes.c_uint32), c_i32]
     lib.w4a4_set_wait_limit_ns.argtypes = [c_u64]

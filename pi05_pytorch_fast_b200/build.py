@@ -7,7 +7,7 @@ libw4a4_sm100.so: the kernels and the C ABI (nvcc, sm_100a).  Self-contained
 at run time), so it travels with the source tree to any B200 host with a
 CUDA 12.8+ driver.
 
-_w4a4_ops.so: the pi05_w4a4 torch ops (g++ against the installed torch's
+_w4a4_ops.so: the pi05_w4a4 and pi05_w8a8 torch ops (g++ against the installed torch's
 headers), calling libw4a4_sm100.so through its C ABI; found next to it
 through an $ORIGIN run path.  It must be rebuilt when torch changes.
 """
@@ -26,7 +26,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(PKG_DIR, "libw4a4_sm100.so")
 MAIN_SOURCE = os.path.join(CSRC, "w4a4_sm100.cu")
-OPS_SOURCE = os.path.join(CSRC, "torch_ops.cpp")
+OPS_SOURCES = [os.path.join(CSRC, f) for f in ("torch_ops.cpp", "torch_ops8.cpp")]
 OPS_OUT = os.path.join(PKG_DIR, "_w4a4_ops.so")
 
 NVCC_FLAGS = [
@@ -47,7 +47,7 @@ def _sources() -> list[str]:
 def _ops_sources() -> list[str]:
     import torch
 
-    return [OPS_SOURCE, OUT, torch.__file__,
+    return [*OPS_SOURCES, OUT, torch.__file__,
             *[os.path.join(INCLUDE, f) for f in sorted(os.listdir(INCLUDE)) if f.endswith(".h")]]
 
 
@@ -106,7 +106,7 @@ def build_ops(force: bool = False, verbose: bool = False) -> str:
     for inc in cpp_extension.include_paths():
         cmd += ["-I", inc]
     cmd += ["-I", os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include"),
-            "-o", OPS_OUT + ".tmp", OPS_SOURCE]
+            "-o", OPS_OUT + ".tmp", *OPS_SOURCES]
     for libdir in cpp_extension.library_paths():
         cmd += ["-L", libdir]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-L", PKG_DIR, "-lw4a4_sm100",

@@ -23,6 +23,7 @@ enum DeviceError : unsigned {
   kErrWaitSelfTest = 1u << 4,  // the self-test wait ran out (expected in that test)
   kErrWaitDrain = 1u << 5,     // teardown gave up draining in-flight copies
   kErrBadParams = 1u << 6,     // launch parameters outside the kernel's invariants
+  kErrCacheFull = 1u << 7,     // a cache append past the capacity, or from a start outside it
 };
 
 // The device error word: kernels OR the bits above into it (read and cleared

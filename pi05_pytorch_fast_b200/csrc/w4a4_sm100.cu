@@ -7,6 +7,7 @@
 // their message text where the reference's tests match on it.
 #include "w4a4_sm100.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cstdlib>
 #include <cmath>
@@ -1436,3 +1437,5 @@ int w4a4_selftest_wait_timeout(uint64_t limit_ns, void* stream) {
 int w4a4_version(void) { return 100; }
 
 }  // extern "C"
+
+#include "w8a8_host.cuh"

@@ -1,0 +1,267 @@
+// Launchers and C entry points of the 8-bit serving operators (rows8.cuh,
+// gemm8.cuh, kv8.cuh, attention8.cuh).  Included by w4a4_sm100.cu, whose
+// helpers (fail, launch_kernel, make_map, ...) it uses.
+#pragma once
+
+#include "attention8.cuh"
+#include "gemm8.cuh"
+#include "kv8.cuh"
+#include "rows8.cuh"
+
+namespace w4a4 {
+namespace {
+
+// Calls f with a value of the element type that `dtype` names.
+template <class F>
+int by_dtype(int32_t dtype, bool fp32_too, const char* what, F f) {
+  switch (dtype) {
+    case W4A4_F16: return f(__half{});
+    case W4A4_BF16: return f(__nv_bfloat16{});
+    case W4A4_F32:
+      if (fp32_too) return f(float{});
+      break;
+    default: break;
+  }
+  return fail(W4A4_ERR_INVALID, "%s: unsupported dtype code %d", what, dtype);
+}
+
+int elem_size(int32_t dtype) { return dtype == W4A4_F32 ? 4 : 2; }
+
+// Whether rows of `stride` elements of `size` bytes from p all begin at a
+// multiple of `bytes`.
+bool rows_aligned(const void* p, int64_t stride, int size, int bytes) {
+  return aligned(p, bytes) && (stride * size) % bytes == 0;
+}
+
+template <int OP>
+int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* what) {
+  if (p.rows == 0) return ok();
+  if (p.rows > 0x7fffffffLL) return fail(W4A4_ERR_UNSUPPORTED, "%s: too many rows: %lld", what, (long long)p.rows);
+  const int size = elem_size(dtype);
+  // The 8-element path wants 16-byte vectors of every operand and 8-byte
+  // vectors of codes; anything else goes one element at a time.
+  bool vec = p.h % 8 == 0 && rows_aligned(p.x, p.ldx, size, 16) && rows_aligned(p.codes, p.ldc, 1, 8);
+  if (p.x2) vec = vec && rows_aligned(p.x2, p.ld2, size, 16);
+  if (p.gate) vec = vec && rows_aligned(p.gate, p.gate_stride, size, 16);
+  if (p.gain) vec = vec && rows_aligned(p.gain, p.gain_stride, 4, 16);
+  if (p.shift) vec = vec && rows_aligned(p.shift, p.shift_stride, 4, 16);
+  if (p.total) vec = vec && aligned(p.total, 16);
+  return by_dtype(dtype, true, what, [&](auto tag) {
+    using T = decltype(tag);
+    const dim3 grid(static_cast<unsigned>(p.rows));
+    const auto go = [&](void (*kernel)(const Row8Params), int groups, int vpt) {
+      const int threads = (((groups + vpt - 1) / vpt) + 31) / 32 * 32;
+      return cuda_status(launch_kernel(kernel, grid, dim3(threads), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+    };
+    if (vec && p.h <= kRow8MaxVec) {
+      const int groups = p.h / 8;
+      if (groups <= 256) return go(row8_kernel<T, OP, 8, 1>, groups, 1);
+      if (groups <= 1024) return go(row8_kernel<T, OP, 8, 2>, groups, 2);
+      return go(row8_kernel<T, OP, 8, 4>, groups, 4);
+    }
+    if (p.h <= 1024) return go(row8_kernel<T, OP, 1, 4>, p.h, 4);
+    if (p.h <= kRow8MaxScalar) return go(row8_kernel<T, OP, 1, 16>, p.h, 16);
+    return go(row8_long_kernel<T, OP>, 1024, 1);
+  });
+}
+
+int check_rows8(int64_t rows, int32_t h, const void* x, int64_t ldx, const int8_t* codes, int64_t ldc,
+                const float* scale, const char* what) {
+  if (rows < 0 || h <= 0) return fail(W4A4_ERR_INVALID, "%s: invalid shape [%lld, %d]", what, (long long)rows, h);
+  if (rows == 0) return W4A4_OK;
+  if (!x || !codes || !scale) return fail(W4A4_ERR_INVALID, "%s: null pointer argument", what);
+  if (ldx < h || ldc < h) return fail(W4A4_ERR_INVALID, "%s: row stride below %d", what, h);
+  return W4A4_OK;
+}
+
+int launch_gemm8(const Gemm8Params& p, int32_t dtype, cudaStream_t stream) {
+  return by_dtype(dtype, true, "gemm8", [&](auto tag) {
+    using T = decltype(tag);
+    const dim3 grid((p.n + 31) / 32, static_cast<unsigned>((p.m + 31) / 32));
+    return cuda_status(launch_kernel(gemm8_simple_kernel<T>, grid, dim3(256), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+  });
+}
+
+// Shape and layout of a cache: width a multiple of 64 up to 256, capacity a
+// multiple of 16, strides and bases multiples of 16 bytes.
+int check_cache8(const void* k, const void* v, const void* ks, const void* vs, const int64_t* stride, int32_t batch,
+                 int32_t heads, int32_t width, int32_t capacity, const char* what) {
+  if (batch < 0 || heads <= 0) return fail(W4A4_ERR_INVALID, "%s: invalid batch %d or heads %d", what, batch, heads);
+  if (width <= 0 || width % 64 || width > 256)
+    return fail(W4A4_ERR_UNSUPPORTED, "%s: head width must be 64, 128, 192 or 256, got %d", what, width);
+  if (capacity <= 0 || capacity % kKvBlock)
+    return fail(W4A4_ERR_INVALID, "%s: the capacity must be a positive multiple of %d, got %d", what, kKvBlock, capacity);
+  if (static_cast<int64_t>(batch) * heads > 65535)
+    return fail(W4A4_ERR_UNSUPPORTED, "%s: batch x heads must be at most 65535, got %d x %d", what, batch, heads);
+  if (!stride) return fail(W4A4_ERR_INVALID, "%s: null pointer argument", what);
+  if (batch == 0) return W4A4_OK;
+  if (!k || !v || !ks || !vs) return fail(W4A4_ERR_INVALID, "%s: null pointer argument", what);
+  if (!aligned(k, 16) || !aligned(v, 16) || stride[0] % 16 || stride[1] % 16 || stride[2] % 16)
+    return fail(W4A4_ERR_INVALID, "%s: cache rows must begin at multiples of 16 bytes", what);
+  if (stride[0] < 0 || stride[1] < width || stride[2] < width)
+    return fail(W4A4_ERR_INVALID, "%s: cache strides must be at least the head width", what);
+  return W4A4_OK;
+}
+
+int launch_attention8(const Attn8Params& p, int32_t dtype, cudaStream_t stream) {
+  return by_dtype(dtype, false, "attention8", [&](auto tag) {
+    using T = decltype(tag);
+    const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.q_heads;
+    const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
+    return cuda_status(launch_kernel(attn8_simple_kernel<T>, grid, dim3(128), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+  });
+}
+
+}  // namespace
+}  // namespace w4a4
+
+extern "C" {
+
+int w4a4_rms_norm_quant8(const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* gate,
+                         int64_t gate_stride, const float* gain, int64_t gain_stride, const float* shift,
+                         int64_t shift_stride, float eps, int32_t dtype, int64_t rows, int32_t rows_per_batch,
+                         int32_t h, void* total, int8_t* codes, int64_t ldc, float* scale, void* stream) {
+  if (int e = check_rows8(rows, h, x, ldx, codes, ldc, scale, "rms_norm_quant8")) return e;
+  if (rows_per_batch <= 0) return fail(W4A4_ERR_INVALID, "rms_norm_quant8: rows_per_batch must be positive");
+  if (rows > 0 && !gain) return fail(W4A4_ERR_INVALID, "rms_norm_quant8: null pointer argument");
+  if (delta && ldd < h) return fail(W4A4_ERR_INVALID, "rms_norm_quant8: row stride below %d", h);
+  if (gate && !delta) return fail(W4A4_ERR_INVALID, "rms_norm_quant8: a gate needs a delta");
+  if (gate_stride < 0 || gain_stride < 0 || shift_stride < 0)
+    return fail(W4A4_ERR_INVALID, "rms_norm_quant8: negative stride");
+  Row8Params p{};
+  p.x = x, p.ldx = ldx, p.x2 = delta, p.ld2 = ldd;
+  p.gate = gate, p.gate_stride = gate_stride, p.gain = gain, p.gain_stride = gain_stride;
+  p.shift = shift, p.shift_stride = shift_stride;
+  p.total = total, p.codes = codes, p.ldc = ldc, p.scale = scale;
+  p.rows = rows, p.rows_per_batch = rows_per_batch, p.h = h, p.eps = eps;
+  return launch_row8<kRowNorm>(p, dtype, static_cast<cudaStream_t>(stream), "rms_norm_quant8");
+}
+
+int w4a4_quant8(const void* x, int64_t ldx, const void* up, int64_t ldu, int32_t dtype, int64_t rows, int32_t h,
+                int8_t* codes, int64_t ldc, float* scale, void* stream) {
+  if (int e = check_rows8(rows, h, x, ldx, codes, ldc, scale, "quant8")) return e;
+  if (up && ldu < h) return fail(W4A4_ERR_INVALID, "quant8: row stride below %d", h);
+  Row8Params p{};
+  p.x = x, p.ldx = ldx, p.x2 = up, p.ld2 = ldu;
+  p.codes = codes, p.ldc = ldc, p.scale = scale;
+  p.rows = rows, p.rows_per_batch = 1, p.h = h;
+  return up ? launch_row8<kRowGeglu>(p, dtype, static_cast<cudaStream_t>(stream), "quant8")
+            : launch_row8<kRowQuant>(p, dtype, static_cast<cudaStream_t>(stream), "quant8");
+}
+
+int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t dtype, int64_t rows, int32_t h,
+                  void* out, void* stream) {
+  if (int e = check_rows8(rows, h, out, h, codes, ldc, scale, "dequant8")) return e;
+  if (rows == 0) return ok();
+  const bool vec = h % 8 == 0 && rows_aligned(codes, ldc, 1, 8) && aligned(out, 16);
+  return by_dtype(dtype, true, "dequant8", [&](auto tag) {
+    using T = decltype(tag);
+    const int per = vec ? 2048 : 256;
+    const dim3 grid((h + per - 1) / per, static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
+    const auto kernel = vec ? dequant8_kernel<T, 8> : dequant8_kernel<T, 1>;
+    return cuda_status(launch_kernel(kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), 1, codes, ldc, scale,
+                                     static_cast<T*>(out), rows, h))
+               ? W4A4_ERR_CUDA
+               : ok();
+  });
+}
+
+int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
+               const void* bias, int32_t dtype, int64_t m, int32_t n, int32_t k, void* y, void* stream) {
+  if (m < 0 || n <= 0 || k <= 0)
+    return fail(W4A4_ERR_INVALID, "gemm8: invalid shape M=%lld N=%d K=%d", (long long)m, n, k);
+  if (k >= 131072) return fail(W4A4_ERR_UNSUPPORTED, "gemm8: K must be below 131072 for exact int32 sums, got %d", k);
+  if (m > 65535LL * 32) return fail(W4A4_ERR_UNSUPPORTED, "gemm8: too many rows: %lld", (long long)m);
+  if (m == 0) return ok();
+  if (!a || !sa || !w || !sw || !y) return fail(W4A4_ERR_INVALID, "gemm8: null pointer argument");
+  if (lda < k || ldw < k) return fail(W4A4_ERR_INVALID, "gemm8: row stride below K = %d", k);
+  if (!rows_aligned(a, lda, 1, 16) || !rows_aligned(w, ldw, 1, 16))
+    return fail(W4A4_ERR_INVALID, "gemm8: rows of codes must begin at multiples of 16 bytes");
+  Gemm8Params p{a, w, sa, sw, bias, y, lda, ldw, m, n, k};
+  return launch_gemm8(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, const int64_t* cache_stride,
+                    int32_t capacity, const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                    int32_t dtype, const uint8_t* valid, int64_t valid_stride, const int32_t* start, int32_t* lengths,
+                    int32_t batch, int32_t tokens, int32_t heads, int32_t width, void* stream) {
+  if (int e = check_cache8(k_codes, v_codes, k_scale, v_scale, cache_stride, batch, heads, width, capacity,
+                           "kv8_append"))
+    return e;
+  if (tokens < 0) return fail(W4A4_ERR_INVALID, "kv8_append: invalid token count %d", tokens);
+  if (batch == 0) return ok();
+  if (!start || !lengths || !k_stride || !v_stride || (tokens > 0 && (!k || !v)))
+    return fail(W4A4_ERR_INVALID, "kv8_append: null pointer argument");
+  Kv8Params p{};
+  p.codes[0] = k_codes, p.codes[1] = v_codes, p.scale[0] = k_scale, p.scale[1] = v_scale;
+  p.x[0] = k, p.x[1] = v, p.start = start, p.valid = valid, p.valid_stride = valid_stride, p.lengths = lengths;
+  p.cb = cache_stride[0], p.ct = cache_stride[1], p.ch = cache_stride[2];
+  p.batch = batch, p.tokens = tokens, p.heads = heads, p.width = width, p.capacity = capacity;
+  bool vec = true;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i ? v_stride : k_stride;
+    p.xb[i] = s[0], p.xt[i] = s[1], p.xh[i] = s[2];
+    vec = vec && aligned(p.x[i], 16) && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
+  }
+  return by_dtype(dtype, false, "kv8_append", [&](auto tag) {
+    using T = decltype(tag);
+    // a run of `tokens` slots touches at most ceil((tokens - 1) / 16) + 1 blocks
+    const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(tokens) + 14) / kKvBlock + 1),
+                    static_cast<unsigned>(batch * heads), 2);
+    const auto kernel = vec ? kv8_append_kernel<T, 8> : kv8_append_kernel<T, 1>;
+    return cuda_status(launch_kernel(kernel, grid, dim3(kKvThreads), 0, static_cast<cudaStream_t>(stream), 1, p))
+               ? W4A4_ERR_CUDA
+               : ok();
+  });
+}
+
+int w4a4_kv8_values(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale, const float* v_scale,
+                    const int64_t* cache_stride, int32_t capacity, const int32_t* lengths, int32_t dtype, int32_t batch,
+                    int32_t heads, int32_t width, void* k_out, void* v_out, void* stream) {
+  if (int e = check_cache8(k_codes, v_codes, k_scale, v_scale, cache_stride, batch, heads, width, capacity,
+                           "kv8_values"))
+    return e;
+  if (batch == 0) return ok();
+  if (!lengths || !k_out || !v_out) return fail(W4A4_ERR_INVALID, "kv8_values: null pointer argument");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16))
+    return fail(W4A4_ERR_INVALID, "kv8_values: outputs must be 16-byte aligned");
+  Kv8ValuesParams p{};
+  p.codes[0] = k_codes, p.codes[1] = v_codes, p.scale[0] = k_scale, p.scale[1] = v_scale;
+  p.out[0] = k_out, p.out[1] = v_out, p.lengths = lengths;
+  p.cb = cache_stride[0], p.ct = cache_stride[1], p.ch = cache_stride[2];
+  p.batch = batch, p.heads = heads, p.width = width, p.capacity = capacity;
+  return by_dtype(dtype, true, "kv8_values", [&](auto tag) {
+    using T = decltype(tag);
+    const int64_t groups = static_cast<int64_t>(capacity) * heads * (width / 8);
+    const dim3 grid(static_cast<unsigned>((groups + 255) / 256), static_cast<unsigned>(batch), 2);
+    return cuda_status(launch_kernel(kv8_values_kernel<T>, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), 1, p))
+               ? W4A4_ERR_CUDA
+               : ok();
+  });
+}
+
+int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_codes, const int8_t* v_codes,
+                    const float* k_scale, const float* v_scale, const int64_t* cache_stride, int32_t capacity,
+                    const int32_t* lengths, int32_t dtype, int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads,
+                    int32_t width, int32_t causal, float scale, void* out, void* stream) {
+  if (int e = check_cache8(k_codes, v_codes, k_scale, v_scale, cache_stride, batch, heads, width, capacity,
+                           "attention8"))
+    return e;
+  if (tokens < 0 || q_heads <= 0 || q_heads % heads)
+    return fail(W4A4_ERR_INVALID, "attention8: invalid tokens %d or %d query heads over %d heads", tokens, q_heads, heads);
+  if (batch == 0 || tokens == 0) return ok();
+  if (!q || !q_stride || !lengths || !out) return fail(W4A4_ERR_INVALID, "attention8: null pointer argument");
+  if (!aligned(q, 16) || !aligned(out, 16) || q_stride[0] % 8 || q_stride[1] % 8 || q_stride[2] % 8)
+    return fail(W4A4_ERR_INVALID, "attention8: query rows must begin at multiples of 16 bytes");
+  if (static_cast<int64_t>(batch) * tokens * q_heads > 0x7fffffffLL)
+    return fail(W4A4_ERR_UNSUPPORTED, "attention8: too many query rows");
+  Attn8Params p{};
+  p.q = q, p.out = out, p.k = k_codes, p.v = v_codes, p.ks = k_scale, p.vs = v_scale, p.lengths = lengths;
+  p.qb = q_stride[0], p.qt = q_stride[1], p.qh = q_stride[2];
+  p.cb = cache_stride[0], p.ct = cache_stride[1], p.ch = cache_stride[2];
+  p.batch = batch, p.tokens = tokens, p.q_heads = q_heads, p.heads = heads, p.width = width, p.capacity = capacity;
+  p.causal = causal != 0, p.scale = scale;
+  return launch_attention8(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,742 @@
+"""The 8-bit serving operators (``pi05_pytorch_fast_b200.w8a8``) against plain
+implementations in 64 bits, and their refusals.
+
+Tolerances are derived from the arithmetic that the operators promise: fp32
+inside, exact int32 sums, one rounding to the output's type.  u(dtype) is the
+unit roundoff 2^-p of that rounding."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from pi05_pytorch_fast_b200 import _native as nat
+from pi05_pytorch_fast_b200 import w8a8
+
+DEV = "cuda:0"
+U = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+TINY = {torch.float16: 2.0 ** -25, torch.bfloat16: 1e-38, torch.float32: 1e-38}  # half a step of the subnormals
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, dtype=torch.float64)
+
+
+def on_gpu(t):
+    return None if t is None else t.to(DEV)
+
+
+def within(got, want, tol):
+    """|got - want| <= tol elementwise, got on any device, NaN nowhere."""
+    err = (got.detach().cpu().double() - want).abs()
+    assert torch.isfinite(err).all()
+    over = err - tol
+    assert (over <= 0).all(), f"worst {err[over > 0].max():.3g}, {int((over > 0).sum())} of {err.numel()} too far"
+
+
+def check_rows(codes, scale, y, tol_y):
+    """codes x scale is y to within half a step of its row and what y itself may be off."""
+    amax = y.abs().amax(-1)
+    off = tol_y.amax(-1)
+    within(scale, amax / 127, off / 127 + 2.0 ** -22 * amax / 127)
+    assert int(codes.abs().max()) <= 127
+    step = (amax / 127 + off / 127)[..., None]
+    within(codes.cpu().double() * scale.cpu().double()[..., None], y, 0.5 * step * (1 + 2.0 ** -10) + tol_y + off[..., None])
+
+
+# ------------------------------------------------------------------ norm
+NORM_CASES = [
+    # batch, tokens, h, dtype, delta, gate, gain and shift for each observation
+    (1, 1, 2048, torch.float16, True, False, False),
+    (8, 50, 1024, torch.bfloat16, True, True, True),
+    (3, 5, 1152, torch.bfloat16, False, False, True),
+    (2, 3, 1, torch.float32, True, False, False),
+    (2, 7, 97, torch.float16, True, True, True),
+    (1, 9, 1155, torch.bfloat16, True, True, False),
+    (2, 2, 8192, torch.float16, True, False, False),
+    (1, 2, 16385, torch.float16, True, False, True),
+    (2, 1, 33000, torch.bfloat16, True, True, True),
+    (5, 3, 264, torch.float32, True, True, True),
+]
+
+
+def norm_inputs(b, t, h, dtype, delta, gate, per_obs, seed=0):
+    g = gen(seed)
+    x = (randn(g, b, t, h) * torch.exp(0.6 * randn(g, h))).to(dtype)
+    d = (randn(g, b, t, h) * 2).to(dtype) if delta else None
+    ga = randn(g, b, h).to(dtype) if gate else None
+    gain = (1 + 0.1 * randn(g, *((b, h) if per_obs else (h,)))).float()
+    shift = (0.1 * randn(g, b, h)).float() if per_obs else None
+    return x, d, ga, gain, shift
+
+
+def norm64(x, delta, gate, gain, shift, eps):
+    """(total, y, how far y may be off) in 64 bits."""
+    def wide(p):
+        return p.double() if p.dim() == 1 else p.double()[:, None]
+
+    z, mag = x.double(), x.double().abs()
+    if delta is not None:
+        d = delta.double() * (1 if gate is None else wide(gate))
+        z, mag = z + d, mag + d.abs()
+    rstd = (z.square().mean(-1, keepdim=True) + eps).rsqrt()
+    y = z * rstd * wide(gain)
+    tol = 2.0 ** -17 * y.abs() + 2.0 ** -21 * mag * rstd * wide(gain).abs()
+    if shift is not None:
+        y, tol = y + wide(shift), tol + 2.0 ** -17 * wide(shift).abs()
+    return z, y, tol, mag
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", NORM_CASES)
+def test_rms_norm_quant(case):
+    x, d, ga, gain, shift = norm_inputs(*case)
+    z, y, tol, mag = norm64(x, d, ga, gain, shift, 1e-6)
+    xg = on_gpu(x)
+    codes, scale, total = w8a8.rms_norm_quant(xg, on_gpu(gain), 1e-6, delta=on_gpu(d), gate=on_gpu(ga), shift=on_gpu(shift))
+    if d is None:
+        assert total is xg
+    else:
+        u = U[x.dtype]
+        within(total, z, u * z.abs() + 2.0 ** -22 * mag + TINY[x.dtype])
+    assert codes.dtype == torch.int8 and codes.shape == x.shape and scale.shape == x.shape[:-1]
+    assert codes.stride(-1) == 1 and (x.shape[1] == 1 or codes.stride(-2) % 16 == 0)
+    check_rows(codes, scale, y, tol)
+
+
+@pytest.mark.gpu
+def test_rms_norm_quant_takes_strided_and_misaligned_rows():
+    g = gen(3)
+    big = on_gpu(randn(g, 6, 4, 2 * 520 + 3).half())
+    gain = on_gpu(1 + 0.1 * randn(g, 512).float())
+    for lo in (0, 1, 8, 523):  # aligned or not; the row stride is odd
+        x, d = big[:, :2, lo:lo + 512], big[:, 2:, lo:lo + 512]
+        got = w8a8.rms_norm_quant(x, gain, delta=d)
+        want = w8a8.rms_norm_quant(x.contiguous(), gain, delta=d.contiguous())
+        _, y, tol, _ = norm64(x.cpu(), d.cpu(), None, gain.cpu(), None, 1e-6)
+        check_rows(got[0], got[1], y, tol)
+        assert torch.equal(got[2], want[2])
+
+
+@pytest.mark.gpu
+def test_rows_that_are_zero_tiny_or_not_finite():
+    x = torch.zeros(6, 256)
+    x[1] = 1e-41                       # scale far below the smallest normal number
+    x[2, 3], x[3, 4], x[4, 5] = math.inf, math.nan, -math.inf
+    x[5] = torch.linspace(-1, 1, 256)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        codes, scale = w8a8.quantize(x.to(dtype).to(DEV))
+        codes, scale = codes.cpu(), scale.cpu()
+        assert scale[0] == 0 and not codes[0].any()
+        if dtype == torch.float32:
+            assert scale[1] > 0 and (codes[1].abs() <= 127).all()
+        assert not torch.isfinite(scale[2:5]).any() and not codes[2:5].any()
+        assert not torch.isfinite(w8a8.dequantize(codes.to(DEV), scale.to(DEV), torch.float32)[2:5]).any()
+        check_rows(codes[5:], scale[5:], x[5:].to(dtype).double(), torch.zeros(1, 256, dtype=torch.float64))
+    # the norm of a zero row is its shift
+    shift = on_gpu(torch.linspace(-2, 2, 256)[None])
+    codes, scale, _ = w8a8.rms_norm_quant(torch.zeros(1, 3, 256, device=DEV), torch.ones(1, 256, device=DEV), shift=shift)
+    check_rows(codes, scale, shift.cpu().double().expand(1, 3, 256), torch.full((1, 3, 256), 1e-6, dtype=torch.float64))
+
+
+# ------------------------------------------------------------- quantise
+def gelu64(x):
+    return 0.5 * x * (1 + torch.tanh(math.sqrt(2 / math.pi) * (x + 0.044715 * x ** 3)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,h", [(1, 1), (1, 16), (3, 17), (5, 2048), (2, 4096), (7, 4304), (2, 16384), (1, 16388), (1, 40000)])
+@pytest.mark.parametrize("geglu", [False, True])
+def test_quantize(m, h, dtype, geglu):
+    g = gen(m * 100003 + h)
+    both = (3 * randn(g, m, 2 * h)).to(dtype)
+    x, up = both[:, :h], both[:, h:]  # halves of one product: strided rows
+    v = x.double()
+    tol = torch.zeros_like(v)
+    if geglu:
+        v = gelu64(v) * up.double()
+        # u = 2 sqrt(2/pi)(x + 0.044715 x^3) is off by 2^-21 |u|, which exp turns into a relative
+        # error of that size wherever exp(-u) is not negligible next to 1 (|u| < 88)
+        u = 1.6 * (x.double().abs() + 0.044715 * x.double().abs() ** 3).clamp(max=88)
+        tol = v.abs() * (2.0 ** -20 + 2.0 ** -20 * u) + 1e-37 * up.double().abs()
+    big = on_gpu(both)
+    codes, scale = w8a8.quantize(big[:, :h], up=big[:, h:] if geglu else None)
+    check_rows(codes, scale, v, tol)
+    back = w8a8.dequantize(codes, scale, dtype)
+    assert back.is_contiguous() and back.dtype == dtype
+    exact = codes.cpu().double() * scale.cpu().double()[:, None]
+    within(back, exact, (U[dtype] + 2.0 ** -23) * exact.abs() + TINY[dtype])
+
+
+# --------------------------------------------------------------- linear
+LINEAR_CASES = [
+    # m, n, k, dtype, bias
+    (1, 1, 1, torch.float32, True),
+    (1, 2560, 2048, torch.float16, False),
+    (2, 130, 64, torch.bfloat16, True),
+    (7, 33, 97, torch.float16, True),
+    (16, 256, 4096, torch.bfloat16, False),
+    (17, 1000, 1155, torch.float16, False),
+    (50, 1024, 4096, torch.bfloat16, True),
+    (65, 129, 2064, torch.float32, False),
+    (129, 257, 272, torch.float16, True),
+    (400, 1024, 1024, torch.bfloat16, False),
+    (512, 1152, 4304, torch.bfloat16, True),
+    (600, 520, 130, torch.float16, False),
+    (1000, 999, 144, torch.bfloat16, True),
+    (1111, 2048, 528, torch.float16, False),
+    (300, 130, 16384, torch.float16, False),
+    (3, 70, 131071, torch.float32, False),
+]
+
+
+def codes_rows(g, m, k, low=-127):
+    ld = (k + 15) // 16 * 16
+    return torch.randint(low, 128, (m, ld), generator=g, dtype=torch.int8)[:, :k]
+
+
+def linear64(a, sa, w, sw, bias):
+    acc = a.double() @ w.double().T  # exact: below 2^53
+    prod = acc * sa.double()[:, None] * sw.double()
+    return (prod if bias is None else prod + bias.double()), prod.abs() + (0 if bias is None else bias.double().abs())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype,bias", LINEAR_CASES)
+def test_linear(m, n, k, dtype, bias):
+    g = gen(m + n + k)
+    a, w = codes_rows(g, m, k), codes_rows(g, n, k, low=-128)
+    sa, sw = (torch.rand(m, generator=g) * 0.02 + 0.001), (torch.rand(n, generator=g) * 0.002 + 0.0001)
+    bi = randn(g, n).to(dtype) if bias else None
+    want, mag = linear64(a, sa, w, sw, bi)
+    pad = torch.full((2, max(m, n), (k + 15) // 16 * 16), 77, dtype=torch.int8, device=DEV)  # the pad is not read as K
+    ag, wg = pad[0, :m, :k], pad[1, :n, :k]
+    ag.copy_(a), wg.copy_(w)
+    y = w8a8.linear(ag, on_gpu(sa), w8a8.Int8Weight(wg, on_gpu(sw)), bias=on_gpu(bi), dtype=dtype)
+    assert y.shape == (m, n) and y.dtype == dtype and y.is_contiguous()
+    within(y, want, U[dtype] * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -22 * mag + TINY[dtype])
+    # the same call gives the same bits
+    assert torch.equal(y, w8a8.linear(ag, on_gpu(sa), w8a8.Int8Weight(wg, on_gpu(sw)), bias=on_gpu(bi), dtype=dtype))
+    assert nat.device_error() == 0
+
+
+@pytest.mark.gpu
+def test_linear_takes_leading_dimensions_and_unaligned_rows():
+    g = gen(5)
+    x = on_gpu(randn(g, 2, 3, 5, 96).bfloat16())
+    weight = w8a8.pack_weight(on_gpu(randn(g, 40, 96).float()))
+    codes, scale = w8a8.quantize(x)
+    y = w8a8.linear(codes, scale, weight)
+    assert y.shape == (2, 3, 5, 40)
+    flat = w8a8.linear(codes.view(30, 96), scale.view(30), weight)
+    assert torch.equal(y.view(30, 40), flat)
+    # rows at odd strides and from odd bases are laid out for the call
+    odd = torch.empty(31, 97, dtype=torch.int8, device=DEV)[1:, 1:]
+    odd.copy_(codes.view(30, 96))
+    assert torch.equal(w8a8.linear(odd, scale.view(30), weight), flat)
+    one = torch.empty(97, dtype=torch.int8, device=DEV)[1:]
+    one.copy_(codes.view(30, 96)[7])
+    assert torch.equal(w8a8.linear(one, scale.view(30)[7:8].clone(), weight), flat[7])
+    assert w8a8.linear(codes.view(30, 96)[:0], scale.view(30)[:0], weight).shape == (0, 40)
+
+
+@pytest.mark.gpu
+def test_linear_rows_that_are_not_finite_stay_apart():
+    g = gen(6)
+    x = randn(g, 5, 128).float()
+    x[2, 7] = math.nan
+    x[3] = 0
+    weight = w8a8.pack_weight(on_gpu(randn(g, 24, 128).float()))
+    codes, scale = w8a8.quantize(x.to(DEV))
+    y = w8a8.linear(codes, scale, weight, dtype=torch.float32).cpu()
+    assert y[2].isnan().all() and (y[3] == 0).all() and torch.isfinite(y[[0, 1, 4]]).all()
+
+
+@pytest.mark.gpu
+def test_linear_in_eight_bits_is_near_the_float_product():
+    """pack_weight + quantize + linear against the product of the values
+    themselves: each operand is off by at most half a step, uniformly, so the
+    sum over K is off by about sqrt(K / 12) of a step product."""
+    g = gen(8)
+    m, n, k = 33, 48, 1024
+    x, w = randn(g, m, k).float(), randn(g, n, k).float()
+    codes, scale = w8a8.quantize(on_gpu(x))
+    weight = w8a8.pack_weight(on_gpu(w))
+    y = w8a8.linear(codes, scale, weight, dtype=torch.float32).cpu().double()
+    want = x.double() @ w.double().T
+    sx, sw = x.abs().amax(1).double()[:, None] / 127, w.abs().amax(1).double()[None] / 127
+    sigma = ((sx ** 2 * w.double().square().sum(1)[None] + sw ** 2 * x.double().square().sum(1)[:, None]) / 12).sqrt()
+    assert ((y - want).abs() < 6 * sigma).all()
+
+
+# ---------------------------------------------------------------- cache
+def cache_state(g, b, cap, h, w):
+    codes = torch.randint(-127, 128, (2, b, cap, h, w), generator=g, dtype=torch.int8)
+    scale = torch.rand(2, b, h, cap // 16, generator=g) * 0.02 + 0.01
+    return codes, scale
+
+
+def append_plain(codes, scale, x, start, valid):
+    """One of keys and values, sequence by sequence and block by block, in the
+    fp32 steps the operator defines (numpy-exact): returns new (codes, scale)."""
+    codes, scale = codes.clone(), scale.clone()
+    b, cap, heads, _ = codes.shape
+    inv127 = torch.tensor(1.0) / 127
+    lengths = []
+    for i in range(b):
+        s0 = int(start[i])
+        if s0 < 0 or s0 > cap:
+            lengths.append(min(max(s0, 0), cap))
+            continue
+        new = x[i] if valid is None else x[i][valid[i].bool()]
+        new = new[: cap - s0].float()
+        end = s0 + len(new)
+        lengths.append(end)
+        for j in range(s0 // 16, -(-end // 16)):
+            lo, hi = max(16 * j, s0), min(16 * j + 16, end)
+            if hi <= lo:
+                continue
+            for h in range(heads):
+                part = new[lo - s0:hi - s0, h]
+                now = part.abs().max() * inv127
+                if lo > 16 * j:
+                    was = scale[i, h, j]
+                    now = torch.maximum(now, was)
+                    ratio = was / now if now > 0 else torch.tensor(0.0)
+                    old = codes[i, 16 * j:lo, h].float() * ratio
+                    codes[i, 16 * j:lo, h] = torch.where(torch.isfinite(now), old.round(), 0.0).to(torch.int8)
+                scale[i, h, j] = now
+                fresh = (part / now).round().clamp(-127, 127) if now > 0 and torch.isfinite(now) else part * 0
+                codes[i, lo:hi, h] = torch.nan_to_num(fresh).to(torch.int8)
+    return codes, scale, torch.tensor(lengths, dtype=torch.int32)
+
+
+APPEND_CASES = [
+    # heads, width, capacity, starts, tokens, share valid, dtype
+    (1, 256, 1024, (676, 0, 15, 16, 1023), 1, None, torch.bfloat16),
+    (1, 256, 832, (0, 0), 776, 0.8, torch.float16),
+    (2, 64, 96, (0, 5, 31, 64), 17, None, torch.float16),
+    (4, 128, 64, (3, 17), 40, 0.5, torch.bfloat16),
+    (1, 192, 48, (1, 2, 3), 45, 0.0, torch.bfloat16),
+    (8, 64, 1312, (7,), 1300, 0.97, torch.float16),
+    (1, 128, 16, (0, 16, 9), 7, None, torch.float16),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,width,cap,starts,tokens,share,dtype", APPEND_CASES)
+def test_kv_append(heads, width, cap, starts, tokens, share, dtype):
+    g = gen(cap + tokens)
+    b = len(starts)
+    codes, scale = cache_state(g, b, cap, heads, width)
+    k = (randn(g, b, tokens, heads, width) * torch.exp(randn(g, b, tokens, 1, 1))).to(dtype)
+    v = randn(g, b, tokens, heads, width).to(dtype)
+    valid = None if share is None else torch.rand(b, tokens, generator=g) < share
+    start = torch.tensor(starts, dtype=torch.int32)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    nat.device_error(clear=True)
+    lengths = w8a8.kv_append(cache, on_gpu(k), on_gpu(v), on_gpu(start), valid=on_gpu(valid))
+    want = [append_plain(codes[i], scale[i], x, start, valid) for i, x in enumerate((k, v))]
+    count = torch.full((b,), tokens) if valid is None else valid.sum(1)
+    over = bool((start + count > cap).any())
+    assert nat.device_error(clear=True) == (nat.ERR_CACHE_FULL if over else 0)
+    assert torch.equal(lengths.cpu(), want[0][2])
+    for got_c, got_s, (wc, ws, _) in ((cache.keys, cache.key_scale, want[0]), (cache.values, cache.value_scale, want[1])):
+        assert torch.equal(got_s.cpu(), ws)
+        assert torch.equal(got_c.cpu(), wc)
+    # the same tokens to the same slots again change nothing
+    before = [t.clone() for t in cache]
+    assert torch.equal(w8a8.kv_append(cache, on_gpu(k), on_gpu(v), on_gpu(start), valid=on_gpu(valid)), lengths)
+    assert all(torch.equal(x, y) for x, y in zip(before, cache))
+    nat.device_error(clear=True)
+    # and the values that the cache stands for
+    for dt in (torch.float32, dtype):
+        for got, (wc, ws, wl) in zip(w8a8.kv_values(cache, lengths, dt), want):
+            full = wc.double() * ws.double().repeat_interleave(16, 2).transpose(1, 2)[..., None]
+            full[torch.arange(cap) >= wl[:, None]] = 0
+            within(got, full, (U[dt] + 2.0 ** -23) * full.abs() + TINY[dt])
+
+
+@pytest.mark.gpu
+def test_kv_append_token_by_token_follows_the_plain_form():
+    g = gen(77)
+    x = randn(g, 1, 40, 2, 64).bfloat16() * (1 + torch.arange(40).bfloat16())[None, :, None, None]  # the scale keeps growing
+    cache = w8a8.KVCache8.allocate(1, 40, 2, 64, DEV)
+    assert cache.keys.shape[1] == 48
+    codes, scale = cache.keys.cpu(), cache.key_scale.cpu()
+    lengths = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for t in range(40):
+        codes, scale, _ = append_plain(codes, scale, x[:, t:t + 1], lengths.cpu(), None)
+        lengths = w8a8.kv_append(cache, on_gpu(x[:, t:t + 1]), on_gpu(-x[:, t:t + 1]), lengths)
+    assert int(lengths) == 40
+    assert torch.equal(cache.keys.cpu(), codes) and torch.equal(cache.key_scale.cpu(), scale)
+    assert torch.equal(cache.values.cpu(), -codes)
+
+
+@pytest.mark.gpu
+def test_kv_append_strided_inputs_and_bad_starts():
+    g = gen(78)
+    b, t, heads, width, cap = 3, 9, 2, 64, 64
+    qkv = on_gpu(randn(g, b, t, 4 * heads * width + 3).half())
+    rows = qkv[..., 1:].as_strided((b, t, 2 * heads, width), (qkv.stride(0), qkv.stride(1), width, 1))
+    k, v = rows[:, :, :heads], rows[:, :, heads:]  # odd strides, odd base
+    start = torch.tensor([5, -1, cap + 1], dtype=torch.int32, device=DEV)
+    a, c = (w8a8.KVCache8.allocate(b, cap, heads, width, DEV) for _ in range(2))
+    nat.device_error(clear=True)
+    la = w8a8.kv_append(a, k, v, start)
+    lc = w8a8.kv_append(c, k.contiguous(), v.contiguous(), start)
+    assert nat.device_error(clear=True) == nat.ERR_CACHE_FULL
+    assert la.tolist() == [14, 0, cap] and torch.equal(la, lc)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+    assert a.keys[0].any() and not a.keys[1:].any() and not a.key_scale[1:].any()
+    # no tokens: nothing but the lengths
+    none = w8a8.kv_append(a, k[:, :0], v[:, :0], torch.tensor([5, 0, cap], dtype=torch.int32, device=DEV))
+    assert none.tolist() == [5, 0, cap] and all(torch.equal(x, y) for x, y in zip(a, c))
+    # transposed [b, heads, t, width] inputs
+    lt = w8a8.kv_append(c, k.transpose(1, 2).contiguous().transpose(1, 2), v, start.clamp(0, 5))
+    w8a8.kv_append(a, k, v, start.clamp(0, 5))
+    assert lt.tolist() == [14, 9, 14] and all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+@pytest.mark.gpu
+def test_kv_append_values_that_are_not_finite():
+    b, heads, width = 1, 2, 64
+    cache = w8a8.KVCache8.allocate(b, 48, heads, width, DEV)
+    k = torch.ones(b, 33, heads, width, dtype=torch.float16, device=DEV)
+    k[0, 18, 1, 3] = math.inf
+    v = torch.ones_like(k)
+    v[0, 2, 0, 5] = math.nan
+    lengths = w8a8.kv_append(cache, k, v, torch.zeros(1, dtype=torch.int32, device=DEV))
+    keys, values = w8a8.kv_values(cache, lengths, torch.float32)
+    bad = torch.zeros(1, 48, heads, dtype=torch.bool, device=DEV)
+    bad[0, 16:32, 1] = True
+    assert torch.equal(~torch.isfinite(keys).all(-1), bad)
+    bad[:] = False
+    bad[0, :16, 0] = True
+    assert torch.equal(~torch.isfinite(values).all(-1), bad)
+
+
+# ------------------------------------------------------------ attention
+ATTEND_CASES = [
+    # q heads, heads, width, capacity, lengths, tokens, causal, dtype
+    (8, 1, 256, 784, (776,), 1, False, torch.bfloat16),
+    (8, 1, 256, 688, (678, 640, 50, 1), 50, False, torch.bfloat16),
+    (1, 1, 64, 16, (1, 0, 16), 1, False, torch.float16),
+    (4, 4, 128, 64, (33, 64, 7), 1, True, torch.float16),
+    (16, 2, 128, 4112, (4101, 1027, 16, 15, 0), 1, True, torch.float16),
+    (6, 2, 64, 160, (160, 131, 17), 17, True, torch.bfloat16),
+    (5, 1, 192, 224, (211, 100), 13, True, torch.float16),
+    (8, 1, 256, 1040, (1033, 700), 129, True, torch.bfloat16),
+    (8, 8, 64, 512, (505, 64), 64, True, torch.float16),
+    (2, 1, 64, 96, (20, 3, 0), 33, True, torch.float16),  # more queries than tokens: rows that see nothing
+    (40, 1, 128, 304, (300,), 3, False, torch.bfloat16),
+    (8, 1, 256, 20000, (19991,), 2, True, torch.float16),
+    (32, 4, 64, 2048, (2048, 2000), 4, True, torch.bfloat16),
+]
+
+
+def attention64(q, codes, scale, lengths, causal, softmax_scale):
+    """(out, sum P |v|, largest |score|, keys seen, largest |v|) in 64 bits."""
+    b, t, qh, w = q.shape
+    cap, heads = codes.shape[2:4]
+    kv = codes.double() * scale.double().repeat_interleave(16, 3).transpose(2, 3)[..., None]
+    k, v = (x.repeat_interleave(qh // heads, 2) for x in kv)
+    limit = lengths.long()[:, None].expand(b, t)
+    if causal:
+        limit = limit - t + 1 + torch.arange(t)
+    sees = torch.arange(cap) < limit[..., None]
+    s = torch.einsum("bthw,bchw->bhtc", q.double(), k) * softmax_scale
+    s = s.masked_fill(~sees[:, None], -math.inf)
+    p = torch.nan_to_num(torch.softmax(s, -1))
+    out = torch.einsum("bhtc,bchw->bthw", p, v)
+    mag = torch.einsum("bhtc,bchw->bthw", p, v.abs())
+    top = torch.where(torch.isfinite(s), s.abs(), 0.0).amax(-1).permute(0, 2, 1)[..., None]
+    return out, mag, top, cap, v.abs().max()
+
+
+def attention_tol(dtype, out, mag, top, n, vmax):
+    # the scores are fp32 sums of `width` products (relative error 2^-20 of the largest), exp's argument
+    # carries that error, P is rounded to 11 bits (and to 2^-25 of the row's largest), and l likewise
+    return U[dtype] * out.abs() + (2.0 ** -10 + 2.0 ** -18 * (1 + top)) * mag + n * 2.0 ** -25 * vmax + TINY[dtype]
+
+
+def attention_inputs(qh, heads, width, cap, lengths, tokens, dtype, seed):
+    g = gen(seed)
+    b = len(lengths)
+    codes, scale = cache_state(g, b, cap, heads, width)
+    q = (randn(g, b, tokens, qh, width) * torch.exp(0.5 * randn(g, b, tokens, qh, 1))).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32)
+    return q, codes, scale, n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qh,heads,width,cap,lengths,tokens,causal,dtype", ATTEND_CASES)
+def test_kv_attention(qh, heads, width, cap, lengths, tokens, causal, dtype):
+    q, codes, scale, n = attention_inputs(qh, heads, width, cap, lengths, tokens, dtype, cap + tokens)
+    want = attention64(q, codes, scale, n, causal, width ** -0.5)
+    # what lies past the length is never seen: scales there are NaN
+    past = torch.arange(cap // 16) * 16 >= n[:, None]
+    dirty = scale.masked_fill(past[None, :, None], math.nan)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(dirty.to(DEV)))
+    out = w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), causal=causal)
+    assert out.shape == q.shape and out.dtype == dtype and out.is_contiguous()
+    within(out, want[0], attention_tol(dtype, *want))
+    limit = n.long()[:, None].expand(len(lengths), tokens)
+    if causal:
+        limit = limit - tokens + 1 + torch.arange(tokens)
+    assert not out.cpu()[limit <= 0].any()  # exactly zero where nothing is seen
+    assert torch.equal(out, w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), causal=causal))
+    assert nat.device_error() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 20, 140])
+def test_kv_attention_over_wide_ranges(tokens):
+    """Scales of the blocks and magnitudes of the queries over many orders, and
+    scores that differ by hundreds."""
+    q, codes, scale, n = attention_inputs(8, 2, 128, 640, (633, 320), tokens, torch.bfloat16, 9)
+    g = gen(10)
+    scale[1] *= torch.exp(6 * torch.randn(scale[1].shape, generator=g))
+    q = q * torch.exp(3 * randn(g, 2, tokens, 8, 1)).bfloat16()
+    want = attention64(q, codes, scale, n, True, 0.1)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    out = w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), causal=True, softmax_scale=0.1)
+    within(out, want[0], attention_tol(torch.bfloat16, *want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_kv_attention_strides_and_sentinel_lengths(tokens):
+    q, codes, scale, n = attention_inputs(4, 2, 64, 96, (96, 50), tokens, torch.float16, 21)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    qg, ng = on_gpu(q), on_gpu(n)
+    out = w8a8.kv_attention(qg, cache, ng)
+    # queries [b, heads, tokens, width] seen as [b, tokens, heads, width], from an odd base, reversed rows
+    assert torch.equal(w8a8.kv_attention(qg.transpose(1, 2).contiguous().transpose(1, 2), cache, ng), out)
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view(q.shape).copy_(qg)
+    assert torch.equal(w8a8.kv_attention(odd, cache, ng), out)
+    # a cache of two layers with heads outside tokens
+    big = torch.empty(2, 2, 2, 96, 64, dtype=torch.int8, device=DEV)
+    views = [big[i].transpose(1, 2) for i in range(2)]
+    for view, c in zip(views, codes):
+        view.copy_(c.to(DEV))
+    assert torch.equal(w8a8.kv_attention(qg, w8a8.KVCache8(*views, *cache[2:]), ng), out)
+    # lengths above the capacity count as the capacity, below zero as none
+    ends = torch.tensor([1000, -3], dtype=torch.int32, device=DEV)
+    got = w8a8.kv_attention(qg, cache, ends)
+    assert torch.equal(got[:1], w8a8.kv_attention(qg, cache, torch.tensor([96, 0], dtype=torch.int32, device=DEV))[:1])
+    assert not got[1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_kv_attention_passes_32_bit_offsets(tokens):
+    """A cache whose last sequence begins past 2^32 bytes."""
+    b, cap, heads, width = 3, 64, 1, 256
+    far = (1 << 31) + 4096
+    q, codes, scale, n = attention_inputs(2, heads, width, cap, (64, 63, 49), tokens, torch.bfloat16, 30)
+    pool = torch.empty(2 * far + cap * width, dtype=torch.int8, device=DEV)
+    keys = pool.as_strided((b, cap, heads, width), (far, width, width, 1))
+    values = pool[cap * width:2 * far].new_empty(2 * far + cap * width).as_strided((b, cap, heads, width), (far, width, width, 1))
+    keys.copy_(codes[0].to(DEV)), values.copy_(codes[1].to(DEV))
+    cache = w8a8.KVCache8(keys, values, *(scale.to(DEV)))
+    out = w8a8.kv_attention(on_gpu(q), cache, on_gpu(n))
+    dense = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    assert torch.equal(out, w8a8.kv_attention(on_gpu(q), dense, on_gpu(n)))
+    new = on_gpu(randn(gen(1), b, 3, heads, width).bfloat16())
+    start = torch.tensor([3, 40, 61], dtype=torch.int32, device=DEV)
+    w8a8.kv_append(cache, new, new, start)
+    w8a8.kv_append(dense, new, new, start)
+    assert torch.equal(cache.keys, dense.keys) and torch.equal(cache.value_scale, dense.value_scale)
+
+
+@pytest.mark.gpu
+def test_operators_follow_the_current_stream():
+    """On a stream of its own, behind work that is still running there."""
+    g = gen(40)
+    x = on_gpu(randn(g, 64, 2048).bfloat16())
+    gain = torch.ones(2048, device=DEV)
+    weight = w8a8.pack_weight(on_gpu(randn(g, 256, 2048).bfloat16()))
+    want = w8a8.linear(*w8a8.rms_norm_quant(x, gain)[:2], weight)
+    q, codes, scale, n = attention_inputs(8, 1, 256, 4096, (4096,), 1, torch.bfloat16, 41)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    qg, ng = on_gpu(q), on_gpu(n)
+    want_a = w8a8.kv_attention(qg, cache, ng)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    late_x, late_q = torch.zeros_like(x), torch.zeros_like(qg)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.randn(4096, 4096, device=DEV)
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late_x.copy_(x), late_q.copy_(qg)
+        got = w8a8.linear(*w8a8.rms_norm_quant(late_x, gain)[:2], weight)
+        got_a = w8a8.kv_attention(late_q, cache, ng)
+    side.synchronize()
+    assert torch.equal(got, want) and torch.equal(got_a, want_a)
+
+
+@pytest.mark.gpu
+def test_operators_in_a_cuda_graph():
+    g = gen(50)
+    x = on_gpu(randn(g, 8, 1, 512).bfloat16())
+    gain = torch.ones(512, device=DEV)
+    weight = w8a8.pack_weight(on_gpu(randn(g, 3 * 128, 512).bfloat16()))
+    cache = w8a8.KVCache8.allocate(8, 64, 1, 128, DEV)
+    start = torch.arange(8, dtype=torch.int32, device=DEV) * 6
+
+    def step():
+        codes, scale, _ = w8a8.rms_norm_quant(x, gain)
+        q, k, v = w8a8.linear(codes, scale, weight).view(8, 1, 3, 128).split(1, 2)
+        lengths = w8a8.kv_append(cache, k, v, start)
+        return w8a8.kv_attention(q, cache, lengths, causal=True)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (1, 2):
+        x.copy_(on_gpu(randn(gen(seed), 8, 1, 512).bfloat16()))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, step())
+
+
+# ------------------------------------------------------------- refusals
+def test_ops_refuse_cpu_tensors():
+    x = torch.zeros(2, 64, dtype=torch.bfloat16)
+    codes, scale = torch.zeros(2, 64, dtype=torch.int8), torch.zeros(2)
+    cache = w8a8.KVCache8.allocate(1, 16, 1, 64, "cpu")
+    n = torch.zeros(1, dtype=torch.int32)
+    kv = torch.zeros(1, 1, 1, 64, dtype=torch.float16)
+    for call in (lambda: w8a8.rms_norm_quant(x, torch.ones(64)), lambda: w8a8.quantize(x), lambda: w8a8.pack_weight(x),
+                 lambda: w8a8.dequantize(codes, scale), lambda: w8a8.linear(codes, scale, w8a8.Int8Weight(codes, scale)),
+                 lambda: w8a8.kv_append(cache, kv, kv, n), lambda: w8a8.kv_values(cache, n),
+                 lambda: w8a8.kv_attention(kv, cache, n)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+
+
+def test_fakes_give_shapes_and_strides():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x = torch.empty(2, 3, 97, dtype=torch.bfloat16, device="cuda")
+        codes, scale, total = torch.ops.pi05_w8a8.rms_norm_quant(x, torch.empty(97, device="cuda"), 1e-6, x)
+        assert codes.shape == x.shape and codes.stride() == (336, 112, 1) and codes.dtype == torch.int8
+        assert scale.shape == (2, 3) and total.shape == x.shape and total.dtype == x.dtype
+        y = torch.ops.pi05_w8a8.linear(codes, scale, torch.empty(5, 97, dtype=torch.int8, device="cuda"),
+                                       torch.empty(5, device="cuda"), None, torch.float16)
+        assert y.shape == (2, 3, 5) and y.dtype == torch.float16
+        cache = w8a8.KVCache8.allocate(2, 20, 1, 64, "cuda")
+        n = torch.empty(2, dtype=torch.int32, device="cuda")
+        q = torch.empty(2, 7, 4, 64, dtype=torch.float16, device="cuda")
+        assert torch.ops.pi05_w8a8.kv_append(*cache, q[:, :, :1], q[:, :, :1], n).shape == (2,)
+        assert torch.ops.pi05_w8a8.kv_attention(q, *cache, n, False, 1.0).shape == q.shape
+        assert torch.ops.pi05_w8a8.kv_values(*cache, n, torch.bfloat16)[1].shape == (2, 32, 1, 64)
+
+
+def test_c_abi_argument_checks_without_gpu():
+    lib = nat.lib()
+    fake = 0x10000  # never dereferenced: every check comes first
+
+    def message(status, code):
+        assert status == code
+        return nat.last_error()
+
+    bad = nat.W4A4_ERR_INVALID
+    norm = [fake, 64, None, 0, None, 0, fake, 0, None, 0, 1e-6, nat.BF16, 4, 1, 64, None, fake, 64, fake, None]
+
+    def with_(args, **at):
+        args = list(args)
+        for i, v in at.items():
+            args[int(i[1:])] = v
+        return args
+
+    assert "row stride" in message(lib.w4a4_rms_norm_quant8(*with_(norm, _1=63)), bad)
+    assert "null" in message(lib.w4a4_rms_norm_quant8(*with_(norm, _6=None)), bad)
+    assert "gate needs a delta" in message(lib.w4a4_rms_norm_quant8(*with_(norm, _4=fake)), bad)
+    assert "rows_per_batch" in message(lib.w4a4_rms_norm_quant8(*with_(norm, _13=0)), bad)
+    assert "dtype" in message(lib.w4a4_rms_norm_quant8(*with_(norm, _11=7)), bad)
+    assert lib.w4a4_rms_norm_quant8(*with_(norm, _12=0)) == 0
+    quant = [fake, 64, None, 0, nat.F16, 4, 64, fake, 64, fake, None]
+    assert "shape" in message(lib.w4a4_quant8(*with_(quant, _6=0)), bad)
+    assert "null" in message(lib.w4a4_quant8(*with_(quant, _9=None)), bad)
+    assert "row stride" in message(lib.w4a4_quant8(*with_(quant, _2=fake, _3=8)), bad)
+    assert "row stride" in message(lib.w4a4_dequant8(fake, 63, fake, nat.F16, 4, 64, fake, None), bad)
+    gemm = [fake, 64, fake, fake, 64, fake, None, nat.F16, 4, 8, 64, fake, None]
+    assert "shape" in message(lib.w4a4_gemm8(*with_(gemm, _9=0)), bad)
+    assert "16 bytes" in message(lib.w4a4_gemm8(*with_(gemm, _1=72)), bad)
+    assert "16 bytes" in message(lib.w4a4_gemm8(*with_(gemm, _3=fake + 8)), bad)
+    assert "row stride" in message(lib.w4a4_gemm8(*with_(gemm, _4=48)), bad)
+    assert "131072" in message(lib.w4a4_gemm8(*with_(gemm, _10=131072, _1=131072, _4=131072)), nat.W4A4_ERR_UNSUPPORTED)
+    assert lib.w4a4_gemm8(*with_(gemm, _8=0)) == 0
+    strides = (ctypes.c_int64 * 3)(64 * 32, 64, 64)
+    att = [fake, strides, fake, fake, fake, fake, strides, 32, fake, nat.F16, 1, 1, 4, 2, 64, 0, 1.0, fake, None]
+    assert "query heads" in message(lib.w4a4_attention8(*with_(att, _12=3)), bad)
+    assert "capacity" in message(lib.w4a4_attention8(*with_(att, _7=33)), bad)
+    assert "width" in message(lib.w4a4_attention8(*with_(att, _14=72)), nat.W4A4_ERR_UNSUPPORTED)
+    assert "dtype" in message(lib.w4a4_attention8(*with_(att, _9=nat.F32)), bad)
+    odd = (ctypes.c_int64 * 3)(64 * 32, 72, 64)
+    assert "16 bytes" in message(lib.w4a4_attention8(*with_(att, _6=odd)), bad)
+    assert lib.w4a4_attention8(*with_(att, _11=0)) == 0
+    app = [fake, fake, fake, fake, strides, 32, fake, strides, fake, strides, nat.F16, None, 0, fake, fake, 1, 1, 2, 64, None]
+    assert "null" in message(lib.w4a4_kv8_append(*with_(app, _13=None)), bad)
+    assert "token count" in message(lib.w4a4_kv8_append(*with_(app, _16=-1)), bad)
+    assert "null" in message(lib.w4a4_kv8_values(fake, fake, fake, fake, strides, 32, None, nat.F16, 1, 2, 64, fake, fake, None), bad)
+
+
+@pytest.mark.gpu
+def test_ops_refuse_bad_arguments():
+    x = torch.zeros(2, 3, 64, dtype=torch.bfloat16, device=DEV)
+    ones = torch.ones(64, device=DEV)
+
+    def refuses(match, call):
+        with pytest.raises(RuntimeError, match=match):
+            call()
+
+    refuses("float16, bfloat16 or float32", lambda: w8a8.quantize(x.double()))
+    refuses("non-empty last dimension", lambda: w8a8.quantize(x[..., :0]))
+    refuses("gain must be", lambda: w8a8.rms_norm_quant(x, ones[:63]))
+    refuses("gain must be", lambda: w8a8.rms_norm_quant(x, ones.expand(3, 64)))
+    refuses("gain must be", lambda: w8a8.rms_norm_quant(x, ones.bfloat16()))
+    refuses("gate needs a delta", lambda: w8a8.rms_norm_quant(x, ones, gate=x[:, 0]))
+    refuses("delta must have", lambda: w8a8.rms_norm_quant(x, ones, delta=x.half()))
+    refuses("shift is on cpu", lambda: w8a8.rms_norm_quant(x, ones, shift=torch.ones(64)))
+    refuses("up must have", lambda: w8a8.quantize(x, up=x[:1]))
+    codes, scale = w8a8.quantize(x)
+    weight = w8a8.pack_weight(torch.ones(8, 64, device=DEV))
+    refuses("weight must be", lambda: w8a8.linear(codes[..., :32], scale, weight))
+    refuses("codes must be int8", lambda: w8a8.linear(x, scale, weight))
+    refuses("scale must be", lambda: w8a8.linear(codes, scale[:1], weight))
+    refuses("bias must be", lambda: w8a8.linear(codes, scale, weight, bias=torch.ones(8, device=DEV)))
+    refuses("dtype must be", lambda: w8a8.linear(codes, scale, weight, dtype=torch.float64))
+    refuses("pack_weight expects", lambda: w8a8.pack_weight(ones))
+    cache = w8a8.KVCache8.allocate(2, 32, 2, 64, DEV)
+    n = torch.zeros(2, dtype=torch.int32, device=DEV)
+    kv = torch.zeros(2, 1, 2, 64, dtype=torch.float16, device=DEV)
+    refuses("new keys must be", lambda: w8a8.kv_append(cache, kv[:, :, :1], kv, n))
+    refuses("new values must have", lambda: w8a8.kv_append(cache, kv, kv[:1], n))
+    refuses("new keys must be float16 or bfloat16", lambda: w8a8.kv_append(cache, kv.float(), kv.float(), n))
+    refuses("start must be", lambda: w8a8.kv_append(cache, kv, kv, n.long()))
+    refuses("valid must be", lambda: w8a8.kv_append(cache, kv, kv, n, valid=torch.ones(2, 2, device=DEV)))
+    refuses("q must be", lambda: w8a8.kv_attention(kv[:, :, :1], cache, n))
+    refuses("q must be float16 or bfloat16", lambda: w8a8.kv_attention(kv.float(), cache, n))
+    refuses("lengths must be", lambda: w8a8.kv_attention(kv, cache, n[:1]))
+    refuses("laid out like the keys", lambda: w8a8.kv_values(cache._replace(values=cache.values[:, :16]), n))
+    refuses("multiple of 16", lambda: w8a8.kv_values(cache._replace(keys=cache.keys[:, :20], values=cache.values[:, :20]), n))
+    refuses("cache scales must be", lambda: w8a8.kv_values(cache._replace(key_scale=cache.key_scale[..., :1]), n))
+    wide = w8a8.KVCache8.allocate(2, 32, 2, 72, DEV)
+    refuses("64, 128, 192 or 256", lambda: w8a8.kv_values(wide, n))
