@@ -370,8 +370,8 @@ int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, i
 
 /* The 8-bit cache: codes int8 [batch, capacity, heads, width] for keys and
  * values (cache_stride: elements of batch, token, head; multiples of 16),
- * scales fp32 [batch, heads, capacity / 16] contiguous; width 64, 128, 192 or
- * 256, capacity a multiple of 16.
+ * scales fp32 [batch, heads, capacity / 16] contiguous; width 64, 128 or 256,
+ * capacity a multiple of 16.
  *
  * Writes the valid tokens (valid uint8 [batch, tokens], NULL: all) of k and v
  * ([batch, tokens, heads, width], strides of batch, token, head) without gaps
@@ -396,11 +396,17 @@ int w4a4_kv8_values(const int8_t* k_codes, const int8_t* v_codes, const float* k
  * group of q_heads / heads query heads sharing a key/value head.  causal: query
  * t sees the keys below lengths[b] - tokens + t + 1 (the queries are the
  * cache's last tokens).  A query that sees no key gives zeros.  out like q,
- * contiguous. */
+ * contiguous.  workspace: at least w4a4_attention8_workspace(...) bytes on the
+ * device, 16-byte aligned (NULL when that is 0); its contents do not matter
+ * before or after the call. */
 int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_codes, const int8_t* v_codes,
                     const float* k_scale, const float* v_scale, const int64_t* cache_stride, int32_t capacity,
                     const int32_t* lengths, int32_t dtype, int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads,
-                    int32_t width, int32_t causal, float scale, void* out, void* stream);
+                    int32_t width, int32_t causal, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                    void* stream);
+/* Bytes of workspace of such a call on the current device. */
+int w4a4_attention8_workspace(int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads, int32_t width,
+                              int32_t capacity, int64_t* bytes);
 
 /* Library ABI version (major * 100 + minor). */
 int w4a4_version(void);

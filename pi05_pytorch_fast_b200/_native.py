@@ -65,6 +65,7 @@ EXPORTED_SYMBOLS = (
     "w4a4_kv8_append",
     "w4a4_kv8_values",
     "w4a4_attention8",
+    "w4a4_attention8_workspace",
     "w4a4_last_error",
     "w4a4_device_error",
     "w4a4_set_wait_limit_ns",
@@ -134,7 +135,8 @@ def _declare(lib: ctypes.CDLL) -> None:
                                     c_i32, c_i32, c_i32, c_i32, vp]
     lib.w4a4_kv8_values.argtypes = [vp, vp, vp, vp, strides, c_i32, vp, c_i32, c_i32, c_i32, c_i32, vp, vp, vp]
     lib.w4a4_attention8.argtypes = [vp, strides, vp, vp, vp, vp, strides, c_i32, vp, c_i32, c_i32, c_i32, c_i32, c_i32,
-                                    c_i32, c_i32, c_f32, vp, vp]
+                                    c_i32, c_i32, c_f32, vp, vp, c_i64, vp]
+    lib.w4a4_attention8_workspace.argtypes = [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, strides]
     lib.w4a4_last_error.argtypes = [ctypes.c_char_p, ctypes.c_size_t]
     lib.w4a4_device_error.argtypes = [ctypes.POINTER(ctypes.c_uint32), c_i32]
     lib.w4a4_set_wait_limit_ns.argtypes = [c_u64]

@@ -1,15 +1,36 @@
 // Attention of new queries over the 8-bit key/value cache (kv8.cuh).
 //
-// Query token t of T, head g of the H / heads that share key/value head h:
+// Query token t of T, head g of the G = H / heads that share key/value head h:
 //   S[j] = scale * (q . kc[j]) * ks[j / 16],  P = softmax(S),  O = sum_j P[j] vs[j / 16] vc[j]
 // over the keys j < lengths[b] (causal: j < lengths[b] - T + t + 1, the
 // queries being the last T tokens of the cache).  A query that sees no key
 // gives zeros.
+//
+// Both kernels work on the rows (t, g) of one key/value head as one matrix:
+// the codes go to the tensor cores as fp16 (an int8 is exact in fp16) and the
+// block scales are applied outside the products, ks to the scores and vs to
+// the probabilities.  Numerics they share:
+//  * Q in fp16 times a power of two for each row (bf16 queries keep their 8
+//    bits wherever an element is within 2^28 of the row's largest);
+//  * scores, row maxima, row sums and O in fp32, softmax in base 2;
+//  * the running maximum m of a row moves only when a block exceeds it by more
+//    than 2^8, so that O is rarely rescaled; p = 2^(s - m) <= 2^8;
+//  * p vs / vref is rounded to fp16 for the P V product (11 bits, as the
+//    scores' own error after exp2 is not much smaller).  vref, a running
+//    reference for the value scales, moves (and O is rescaled) when a scale
+//    exceeds it by more than 2^4: p vs / vref <= 2^12 fits fp16, and what
+//    falls below its range is below 2^-24 of the row's largest term.
+// When the keys of a head are split over CTAs, each writes its unnormalised O
+// with (m, l) and attn8_join_kernel adds them up.
 #pragma once
 
+#include "attention.cuh"
 #include "kv8.cuh"
 
 namespace w4a4 {
+
+constexpr float kAttn8Grow = 8.f;      // log2 by which a block may exceed m
+constexpr float kAttn8VGrow = 16.f;    // factor by which a value scale may exceed vref
 
 struct Attn8Params {
   const void* q;  // [batch, tokens, q_heads, width]
@@ -19,58 +40,878 @@ struct Attn8Params {
   const float* ks;
   const float* vs;
   const int32_t* lengths;
+  float* part_o;           // [batch * heads][splits][rows][width]
+  float2* part_ml;         // [batch * heads][splits][rows]
   long long qb, qt, qh;    // query strides (elements)
   long long cb, ct, ch;    // cache strides
-  int batch, tokens, q_heads, heads, width, capacity;
+  int tokens, heads, group, capacity;  // group: query heads of a key/value head
+  int rows;                // tokens * group
+  int splits;
   int causal;
-  float scale;
+  float scale;             // softmax scale * log2(e)
+  unsigned long long wait_limit_ns;
 };
 
-// One warp per query row, one key at a time: right for every case.
-template <typename T>
-__global__ void __launch_bounds__(128) attn8_simple_kernel(const __grid_constant__ Attn8Params p) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Two of four codes, given as code + 128 in the bytes of w, as fp16: 0x6400 |
+// u is 1024 + u, so subtracting 1152 leaves the code, exactly.
+template <int HI>
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t w) {
+  const uint32_t u = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// D (16 x 8, fp32) += A (16 x 16, fp16) B (16 x 8, fp16).
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with rows 8-15 of A zero: only d[0] and d[1] (rows 0-7) are kept.
+__device__ __forceinline__ void mma_16816_half(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  float x, y;
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
+      : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
+      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <bool HALF>
+__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (HALF) mma_16816_half(d, a0, a2, b0, b1);
+  else mma_16816(d, a0, a1, a2, a3, b0, b1);
+}
+
+// Ratio of a block's value scale to the reference, and the reference's move:
+// returns the factor for what was accumulated so far (1: no move).  A scale
+// that is not finite never becomes the reference (rows that do not see its
+// block stay clean); its ratio is NaN.
+__device__ __forceinline__ float move_vref(float vsc, float& vref) {
+  if (!(vsc > kAttn8VGrow * vref) || vsc > 3.4028234e38f) return 1.f;
+  const float f = vref / vsc;
+  vref = vsc;
+  return f;
+}
+__device__ __forceinline__ float vscale_ratio(float vsc, float vref) {
+  if (vsc == 0.f) return 0.f;
+  return vsc <= 3.4028234e38f ? __fdividef(vsc, vref) : __uint_as_float(0x7fc00000u);
+}
+// p times the ratio; keys that are not seen (p = 0) add nothing whatever it is.
+__device__ __forceinline__ float weigh(float p, float rv) { return p == 0.f ? 0.f : p * rv; }
+
+// The power of two by which a row of queries is multiplied so that its largest
+// element lies in [2^14, 2^15) of fp16 (1 for a zero row).
+__device__ __forceinline__ float query_shift(float amax) {
+  const int e = static_cast<int>(__float_as_uint(amax) >> 23);  // biased exponent
+  if (e == 0) return amax == 0.f ? 1.f : 1.7014118e38f;         // subnormal: 2^127
+  return __uint_as_float(static_cast<uint32_t>(max(1, min(254, 254 - e + 14))) << 23);  // 2^(127 - e + 14)
+}
+
+// Keys seen by query token t of an observation with n tokens in its cache.
+__device__ __forceinline__ int keys_seen(const Attn8Params& p, int n, int t) {
+  return p.causal ? max(0, n - p.tokens + t + 1) : n;
+}
+
+// ------------------------------------------------------- few rows (<= 16)
+// The form for single tokens.  One CTA of 8 warps per (split, key/value head);
+// every warp takes every eighth block of 16 keys of the CTA's range on its own,
+// through its own ring of cp.async stages in shared memory (no barrier
+// between warps until the end), with mma.sync m16n8k16: the 16 rows are the
+// heads of the group, so a block's K and V are read once for all of them.
+// The K index of an MMA may be permuted freely when both operands agree, and
+// so may the columns of V; so every lane reads 16 consecutive bytes:
+//  * K: lane (g, t) of a key row g reads dims 64 c + 16 t ... + 15 = four steps
+//    of four dims, Q is read from shared memory in the same order;
+//  * V: lane (g, t) reads dims 16 g ... + 15 of the keys 2t, 2t+1, 2t+8, 2t+9;
+//    pairs of keys are zipped with byte permutes; column n of tile e is dim
+//    16 n + e, so a lane ends with runs of 16 consecutive dims of O.
+// Bound: HBM (2 width bytes per key).  Legacy MMA is enough here: a block costs
+// a warp under 1000 cycles and 8 warps need one each 2800 to keep up.
+template <int D>
+struct Attn8Few {
+  static constexpr int kWarps = 8;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kChunks = D / 16;            // 16-byte chunks of a key
+  static constexpr int kHalfStage = kKvBlock * D;   // K or V of a block
+  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 5 : 8;
+  static constexpr int kRing = kStages * 2 * kHalfStage;  // per warp
+  static constexpr int kPad = D + 4;                // row of the O exchange (floats)
+  static constexpr int kQBytes = 16 * D * 2;
+  static constexpr int kSmem = kQBytes + 16 * 8 + kWarps * 16 * 8 + kWarps * (kRing > 16 * kPad * 4 ? kRing : 16 * kPad * 4);
+  // byte offset of 16-byte chunk c of key row r
+  __device__ static __forceinline__ int k_at(int r, int c) {
+    const int l = r * kChunks + c;
+    return 16 * (D >= 128 ? l ^ ((r & 1) << 2) : l);
+  }
+  __device__ static __forceinline__ int v_at(int r, int c) { return 16 * ((r * kChunks + c) ^ (((r >> 1) & 3) << 1)); }
+};
+
+template <typename T, int D, bool HALF>
+__global__ void __launch_bounds__(Attn8Few<D>::kThreads, 1) attn8_few_kernel(const __grid_constant__ Attn8Params p) {
+  using C = Attn8Few<D>;
+  extern __shared__ __align__(128) uint8_t few_smem[];
+  uint8_t* q_smem = few_smem;                                        // fp16 [16][D], chunk c of row r at c ^ (r & 1)
+  float2* row_info = reinterpret_cast<float2*>(q_smem + C::kQBytes); // score factor, keys seen
+  float2* warp_ml = row_info + 16;                                   // [warps][16]
+  uint8_t* rings = reinterpret_cast<uint8_t*>(warp_ml + C::kWarps * 16);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x, unit = blockIdx.y;
+  const int b = unit / p.heads, h = unit - b * p.heads;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int n = min(max(p.lengths[b], 0), p.capacity);
+  const int nblk = (n + kKvBlock - 1) / kKvBlock;
+  const int per = (nblk + p.splits - 1) / p.splits;
+  const int blk0 = split * per, blk1 = min(nblk, blk0 + per);
+  const int8_t* kc = p.k + b * p.cb + h * p.ch;
+  const int8_t* vc = p.v + b * p.cb + h * p.ch;
+  const float* ks = p.ks + static_cast<long long>(unit) * (p.capacity / kKvBlock);
+  const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
+  uint8_t* ring = rings + warp * C::kRing;
+  const uint32_t ring_addr = smem_addr(ring);
+  // slots up to the end of the cache's last block exist, so whole blocks are read
+  const auto fetch = [&](int blk, int stage) {
+    const int8_t* kb = kc + static_cast<long long>(blk) * kKvBlock * p.ct;
+    const int8_t* vb = vc + static_cast<long long>(blk) * kKvBlock * p.ct;
+    const uint32_t dst = ring_addr + stage * 2 * C::kHalfStage;
+#pragma unroll
+    for (int i = 0; i < kKvBlock * C::kChunks / 32; ++i) {
+      const int l = lane + 32 * i, r = l / C::kChunks, c = l % C::kChunks;
+      cp_async16(dst + C::k_at(r, c), kb + r * p.ct + 16 * c);
+      cp_async16(dst + C::kHalfStage + C::v_at(r, c), vb + r * p.ct + 16 * c);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) {
+    const int blk = blk0 + warp + C::kWarps * i;
+    if (blk < blk1) fetch(blk, i);
+    cp_async_commit();
+  }
+  {
+    // Q: 16 threads per row, D / 16 consecutive elements each
+    constexpr int E = D / 16;
+    const int r = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * E;
+    float v[E];
+    uint32_t key = 0;
+    const int tok = r / p.group, head = h * p.group + r % p.group;
+    const T* src = static_cast<const T*>(p.q) + b * p.qb + tok * p.qt + head * p.qh + e0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = 0.f;
+    if (r < p.rows) {
+      if constexpr (E >= 8) {
+#pragma unroll
+        for (int i = 0; i < E; i += 8) load8(src + i, *reinterpret_cast<float(*)[8]>(&v[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = to_float(src[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) key = max(key, abs_key(v[i]));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) key = max(key, __shfl_xor_sync(0xffffffffu, key, o));
+    const float shift = query_shift(__uint_as_float(key));
+    const float up = p.scale < 0.f ? -shift : shift;  // the factor below is not negative
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+      const int e = e0 + i;
+      *reinterpret_cast<uint32_t*>(q_smem + r * 2 * D + ((((e >> 3) ^ (r & 1)) << 4) | ((e & 7) * 2))) =
+          pack_half2_bits(v[i] * up, v[i + 1] * up);
+    }
+    if ((threadIdx.x & 15) == 0)
+      row_info[r] = make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, tok) : 0));
+  }
+  __syncthreads();
+  constexpr int R = HALF ? 1 : 2;  // rows g, g + 8 of a lane
+  float factor[R], m[R], l[R];
+  int seen[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const float2 info = row_info[g + 8 * i];
+    factor[i] = info.x;
+    seen[i] = __float_as_int(info.y);
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+  }
+  float vref = 0.f;
+  float o[D / 8][4];
+#pragma unroll
+  for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
+
+  int stage = 0;
+  for (int blk = blk0 + warp; blk < blk1; blk += C::kWarps) {
+    const float ksc = __ldg(ks + blk), vsc = __ldg(vs + blk);
+    cp_async_wait<C::kStages - 2>();
+    __syncwarp();
+    {
+      const int next = blk + C::kWarps * (C::kStages - 1);
+      if (next < blk1) fetch(next, stage == 0 ? C::kStages - 1 : stage - 1);
+      cp_async_commit();
+    }
+    const uint8_t* kt = ring + stage * 2 * C::kHalfStage;
+    const uint8_t* vt = kt + C::kHalfStage;
+    stage = stage + 1 == C::kStages ? 0 : stage + 1;
+    // ---- S (rows x 16 keys): keys 2t, 2t + 1 of tile 0, and 8 more in tile 1
+    float s0[4] = {}, s1[4] = {};
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c) {
+      const uint4 k0 = *reinterpret_cast<const uint4*>(kt + C::k_at(g, 4 * c + t));
+      const uint4 k1 = *reinterpret_cast<const uint4*>(kt + C::k_at(g + 8, 4 * c + t));
+      uint32_t qa[8], qb[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int chunk = 8 * c + 2 * t + u;
+        *reinterpret_cast<uint4*>(&qa[4 * u]) =
+            *reinterpret_cast<const uint4*>(q_smem + g * 2 * D + ((chunk ^ (g & 1)) << 4));
+        if constexpr (!HALF)
+          *reinterpret_cast<uint4*>(&qb[4 * u]) =
+              *reinterpret_cast<const uint4*>(q_smem + (g + 8) * 2 * D + ((chunk ^ (g & 1)) << 4));
+        else
+          qb[4 * u] = qb[4 * u + 1] = qb[4 * u + 2] = qb[4 * u + 3] = 0u;
+      }
+      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const uint32_t u0 = w0[s] ^ 0x80808080u, u1 = w1[s] ^ 0x80808080u;
+        mma_rows<HALF>(s0, qa[2 * s], qb[2 * s], qa[2 * s + 1], qb[2 * s + 1], codes_to_half2<0>(u0), codes_to_half2<1>(u0));
+        mma_rows<HALF>(s1, qa[2 * s], qb[2 * s], qa[2 * s + 1], qb[2 * s + 1], codes_to_half2<0>(u1), codes_to_half2<1>(u1));
+      }
+    }
+    // ---- softmax of the block
+    const int j0 = blk * kKvBlock + 2 * t;
+    float f[R];
+    bool grow = false;
+    float pr[R][4];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float fk = factor[i] * ksc;
+      pr[i][0] = j0 < seen[i] ? s0[2 * i] * fk : -INFINITY;
+      pr[i][1] = j0 + 1 < seen[i] ? s0[2 * i + 1] * fk : -INFINITY;
+      pr[i][2] = j0 + 8 < seen[i] ? s1[2 * i] * fk : -INFINITY;
+      pr[i][3] = j0 + 9 < seen[i] ? s1[2 * i + 1] * fk : -INFINITY;
+      float bm = fmaxf(fmaxf(pr[i][0], pr[i][1]), fmaxf(pr[i][2], pr[i][3]));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
+      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+      f[i] = 1.f;
+      if (bm > m[i] + kAttn8Grow) {
+        f[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm);
+        m[i] = bm;
+        l[i] *= f[i];
+        grow = true;
+      }
+    }
+    const float fv = move_vref(vsc, vref);
+    if (__any_sync(0xffffffffu, grow) || fv != 1.f) {
+#pragma unroll
+      for (int e = 0; e < D / 8; ++e)
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          o[e][2 * i] *= f[i] * fv;
+          o[e][2 * i + 1] *= f[i] * fv;
+        }
+    }
+    const float rv = vscale_ratio(vsc, vref);
+    uint32_t pa[R][2];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float nm = m[i] == -INFINITY ? 0.f : -m[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        pr[i][j] = ex2_approx(pr[i][j] + nm);
+        l[i] += pr[i][j];
+      }
+      pa[i][0] = pack_half2_bits(weigh(pr[i][0], rv), weigh(pr[i][1], rv));
+      pa[i][1] = pack_half2_bits(weigh(pr[i][2], rv), weigh(pr[i][3], rv));
+    }
+    const uint32_t a1 = HALF ? 0u : pa[R - 1][0], a3 = HALF ? 0u : pa[R - 1][1];
+    // ---- O += P V
+    constexpr int VW = D >= 128 ? 4 : 2;  // words of a lane's run of dims
+#pragma unroll
+    for (int u = 0; u < (D >= 128 ? D / 128 : 1); ++u) {
+      uint32_t w[4][VW];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 2 * t + (i & 1) + 8 * (i >> 1);
+        if constexpr (VW == 4)
+          *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(vt + C::v_at(r, g + 8 * u));
+        else
+          *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(vt + C::v_at(r, g >> 1) + 8 * (g & 1));
+#pragma unroll
+        for (int x = 0; x < VW; ++x) w[i][x] ^= 0x80808080u;
+      }
+#pragma unroll
+      for (int x = 0; x < VW; ++x) {
+        // keys (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 4x .. 4x + 3, two dims a word
+        const uint32_t z[4] = {__byte_perm(w[0][x], w[1][x], 0x5140), __byte_perm(w[2][x], w[3][x], 0x5140),
+                               __byte_perm(w[0][x], w[1][x], 0x7362), __byte_perm(w[2][x], w[3][x], 0x7362)};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float(&d0)[4] = o[u * 16 + 4 * x + 2 * y];
+          float(&d1)[4] = o[u * 16 + 4 * x + 2 * y + 1];
+          mma_rows<HALF>(d0, pa[0][0], a1, pa[0][1], a3, codes_to_half2<0>(z[2 * y]), codes_to_half2<0>(z[2 * y + 1]));
+          mma_rows<HALF>(d1, pa[0][0], a1, pa[0][1], a3, codes_to_half2<1>(z[2 * y]), codes_to_half2<1>(z[2 * y + 1]));
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+    l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+    if (t == 0) warp_ml[warp * 16 + g + 8 * i] = make_float2(m[i], l[i]);
+  }
+  __syncthreads();  // every warp has left its ring
+  float* xo = reinterpret_cast<float*>(rings) + warp * 16 * C::kPad;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int e = 0; e < D / 8; e += 4) {
+        constexpr int run = D >= 128 ? 16 : 8;
+        const int dim = (e / 16) * 128 + (2 * t + half) * run + e % 16;
+        *reinterpret_cast<float4*>(xo + (g + 8 * i) * C::kPad + dim) =
+            make_float4(o[e][2 * i + half] * vref, o[e + 1][2 * i + half] * vref, o[e + 2][2 * i + half] * vref,
+                        o[e + 3][2 * i + half] * vref);
+      }
+  __syncthreads();
+  const int rows = min(p.rows, HALF ? 8 : 16);
+  for (int i = threadIdx.x; i < rows * (D / 4); i += C::kThreads) {
+    const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, warp_ml[w * 16 + r].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < C::kWarps; ++w) {
+      const float2 ml = warp_ml[w * 16 + r];
+      if (ml.y == 0.f) continue;  // saw nothing (a NaN stays)
+      const float f = ex2_approx(ml.x - mm);
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(rings) + (w * 16 + r) * C::kPad + e);
+      acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
+      acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
+      sum = fmaf(ml.y, f, sum);
+    }
+    if (p.splits > 1) {
+      const long long at = (static_cast<long long>(unit) * p.splits + split) * p.rows + r;
+      *reinterpret_cast<float4*>(p.part_o + at * D + e) = acc;
+      if (e == 0) p.part_ml[at] = make_float2(mm, sum);
+    } else {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const int tok = r / p.group, head = h * p.group + r % p.group;
+      T* dst = static_cast<T*>(p.out) + ((static_cast<long long>(b) * p.tokens + tok) * (p.heads * p.group) + head) * D + e;
+      dst[0] = from_float<T>(acc.x * inv), dst[1] = from_float<T>(acc.y * inv);
+      dst[2] = from_float<T>(acc.z * inv), dst[3] = from_float<T>(acc.w * inv);
+    }
+  }
+}
+
+// ------------------------------------------------------ many rows (> 16)
+// tcgen05: a CTA takes 128 rows (t, g) of one key/value head and a range of
+// its keys, in tiles of 64.  The codes become fp16 in shared memory once per
+// tile and CTA, by eight warps of their own:
+//   warps 0-3   softmax (thread = row = TMEM lane) and the epilogue
+//   warp 4      issues S = Q K^T (M 128, N 64) and O += P V (M 128, N D)
+//   warps 5-8   keys:   16 codes a load -> K-major rows, 128-byte swizzle
+//   warps 9-12  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
+//               permutes), as the second product wants its B operand K-major
+// K and V^T tiles, scores and P are double buffered; O stays in TMEM.  Each
+// converter loads its part of the next tile into registers before it waits
+// for the buffer that the current one goes to.
+// At D = 256 a tile costs the tensor pipe 1024 cycles, the exponentials (16 a
+// cycle) 512, and the conversion about 400 issue slots on each SM
+// sub-partition, so the products bound it.
+template <int D>
+struct Attn8Many {
+  static constexpr int kRows = 128, kKeys = 64;
+  static constexpr int kSlices = D / 64;
+  static constexpr int kQBytes = kRows * D * 2;
+  static constexpr int kKBytes = kKeys * D * 2, kVBytes = D * kKeys * 2;
+  static constexpr int kThreads = 13 * 32;
+  static constexpr int kNumBars = 17;
+  static constexpr int kNeed = kQBytes + 2 * (kKBytes + kVBytes) + kRows * 8 + kNumBars * 8 + 16 + 1024;
+  // two CTAs on an SM only where their TMEM fits beside each other
+  static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
+  static constexpr int kSmem = D == 128 ? (kNeed > 118 * 1024 ? kNeed : 118 * 1024) : kNeed;
+  static constexpr uint32_t kOCol = 0, kSCol = D, kPCol = D + 128;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(const __grid_constant__ Attn8Params p) {
+  using C = Attn8Many<D>;
+  extern __shared__ uint8_t many_smem[];
+  uint8_t* base =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* q_smem = base;                       // [slices][128 rows][128 B]
+  uint8_t* k_ring = base + C::kQBytes;          // [2][slices][64 rows][128 B]
+  uint8_t* v_ring = k_ring + 2 * C::kKBytes;    // [2][D rows][128 B]
+  float2* row_info = reinterpret_cast<float2*>(v_ring + 2 * C::kVBytes);  // score factor, keys seen
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_info + C::kRows);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const auto bar_kfull = [&](int s) { return smem_addr(bars + s); };
+  const auto bar_kempty = [&](int s) { return smem_addr(bars + 2 + s); };
+  const auto bar_vfull = [&](int s) { return smem_addr(bars + 4 + s); };
+  const auto bar_vempty = [&](int s) { return smem_addr(bars + 6 + s); };
+  const auto bar_sfull = [&](int s) { return smem_addr(bars + 8 + s); };
+  const auto bar_sfree = [&](int s) { return smem_addr(bars + 10 + s); };
+  const auto bar_pfull = [&](int s) { return smem_addr(bars + 12 + s); };
+  const auto bar_pfree = [&](int s) { return smem_addr(bars + 14 + s); };
+  const uint32_t bar_o = smem_addr(bars + 16);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.y, unit = blockIdx.z;
+  const int b = unit / p.heads, h = unit - b * p.heads;
+  const int r0 = blockIdx.x * C::kRows;
+  unsigned* err = &g_w4a4_device_error;
+  const uint64_t limit = p.wait_limit_ns;
+
+  pdl_launch_dependents();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_kfull(s), 4);
+      mbar_init(bar_kempty(s), 1);
+      mbar_init(bar_vfull(s), 4);
+      mbar_init(bar_vempty(s), 1);
+      mbar_init(bar_sfull(s), 1);
+      mbar_init(bar_sfree(s), 4);
+      mbar_init(bar_pfull(s), 4);
+      mbar_init(bar_pfree(s), 1);
+    }
+    mbar_init(bar_o, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
+    tmem_relinquish();
+  }
+  pdl_wait();
+  const int n = min(max(p.lengths[b], 0), p.capacity);
+  // the tile's keys: those its last row sees (an earlier row never sees more)
+  const int last = min(p.rows, r0 + C::kRows) - 1;
+  const int kend = keys_seen(p, n, last / p.group);
+  const int ntiles = (kend + C::kKeys - 1) / C::kKeys;
+  const int per = (ntiles + p.splits - 1) / p.splits;
+  const int tile0 = min(ntiles, split * per), nt = min(ntiles, tile0 + per) - tile0;
+  const int nblocks = (n + kKvBlock - 1) / kKvBlock;  // blocks with a scale
+
+  // ---- Q: a row per warp and step, fp16, 128-byte swizzle
+  {
+    constexpr int E = D / 32;  // elements of a lane: 2, 4 or 8
+    constexpr int kSteps = (C::kRows + 12) / 13;
+    uint32_t raw[kSteps][E / 2];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int r = r0 + warp + 13 * i;
+#pragma unroll
+      for (int e = 0; e < E / 2; ++e) raw[i][e] = 0u;
+      if (warp + 13 * i < C::kRows && r < p.rows) {
+        const T* src = static_cast<const T*>(p.q) + b * p.qb + (r / p.group) * p.qt +
+                       (h * p.group + r % p.group) * p.qh + lane * E;
+        if constexpr (E == 8) *reinterpret_cast<uint4*>(raw[i]) = *reinterpret_cast<const uint4*>(src);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(raw[i]) = *reinterpret_cast<const uint2*>(src);
+        else raw[i][0] = *reinterpret_cast<const uint32_t*>(src);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      const int row = warp + 13 * i;
+      if (row >= C::kRows) break;
+      float v[E];
+      uint32_t key = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        v[e] = to_float(reinterpret_cast<const T*>(raw[i])[e]);
+        key = max(key, abs_key(v[e]));
+      }
+      key = __reduce_max_sync(0xffffffffu, key);
+      const float shift = query_shift(__uint_as_float(key));
+      const float up = p.scale < 0.f ? -shift : shift;
+      uint32_t w[E / 2];
+#pragma unroll
+      for (int e = 0; e < E; e += 2) w[e / 2] = pack_half2_bits(v[e] * up, v[e + 1] * up);
+      const int byte = lane * E * 2;  // in the row of D fp16
+      uint8_t* dst = q_smem + (byte >> 7) * (C::kRows * 128) + row * 128 + (((((byte >> 4) & 7) ^ (row & 7)) << 4) | (byte & 15));
+      if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
+      else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w);
+      else *reinterpret_cast<uint32_t*>(dst) = w[0];
+      if (lane == 0) {
+        const int r = r0 + row;
+        row_info[row] =
+            make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, r / p.group) : 0));
+      }
+    }
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 4) {
+    // ------------------------------------------------ MMA issuer (one elected lane)
+    const bool issuer = elect_one();
+    const uint32_t idesc_s = idesc_f16(C::kRows, C::kKeys);
+    const uint32_t idesc_o = idesc_f16(C::kRows, D);
+    const uint64_t qdesc = smem_desc_sw128(smem_addr(q_smem));
+    const auto issue_s = [&](int i) -> bool {
+      const int slot = i & 1;
+      bool ok = mbar_wait_spin(bar_kfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit);
+      if (ok && i >= 2)
+        ok = mbar_wait_spin(bar_sfree(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit);
+      if (!warp_all(ok)) return false;
+      tc_fence_after();
+      const uint64_t kdesc = smem_desc_sw128(smem_addr(k_ring + slot * C::kKBytes));
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint64_t off = static_cast<uint64_t>((kk & 3) * 2);
+        if (issuer)
+          umma_f16_ss(tmem_base + C::kSCol + slot * C::kKeys,
+                      qdesc + static_cast<uint64_t>((kk >> 2) * (C::kRows * 128) >> 4) + off,
+                      kdesc + static_cast<uint64_t>((kk >> 2) * (C::kKeys * 128) >> 4) + off, idesc_s, kk > 0);
+      }
+      if (issuer) {
+        umma_commit(bar_kempty(slot));
+        umma_commit(bar_sfull(slot));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool alive = nt > 0 && issue_s(0);
+    for (int i = 0; alive && i < nt; ++i) {
+      if (i + 1 < nt && !(alive = issue_s(i + 1))) break;
+      const int slot = i & 1;
+      bool ok = mbar_wait_spin(bar_vfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit);
+      if (ok) ok = mbar_wait_spin(bar_pfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit);
+      if (!warp_all(ok)) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      const uint64_t vdesc = smem_desc_sw128(smem_addr(v_ring + slot * C::kVBytes));
+#pragma unroll
+      for (int kk = 0; kk < C::kKeys / 16; ++kk)
+        if (issuer)
+          umma_f16_ts(tmem_base + C::kOCol, tmem_base + C::kPCol + slot * 32 + 8 * kk,
+                      vdesc + static_cast<uint64_t>(kk * 2), idesc_o, (i | kk) != 0);
+      if (issuer) {
+        umma_commit(bar_vempty(slot));
+        umma_commit(bar_pfree(slot));
+      }
+      __syncwarp();
+    }
+    if (issuer) umma_commit(bar_o);  // arrives once every MMA of this CTA has completed
+    __syncwarp();
+    volatile int no_abort = 0;
+    mbar_wait_bounded(bar_o, 0, &no_abort, err, kErrWaitDrain, limit);
+  } else if (warp >= 9) {
+    // ------------------------------------------------ values -> V^T (fp16)
+    constexpr int W = D / 64;  // words of a lane's run of dims: 1, 2 or 4
+    const int kc = lane & 7;   // keys 8 kc .. 8 kc + 7 of a tile
+    const int dim0 = (warp - 9) * (D / 4) + (lane >> 3) * (D / 16);
+    const int8_t* src = p.v + b * p.cb + h * p.ch + dim0;
+    uint32_t w[8][W];
+    const auto load = [&](int i) {
+      const int j0 = (tile0 + i) * C::kKeys + 8 * kc;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+#pragma unroll
+        for (int x = 0; x < W; ++x) w[k][x] = 0u;
+        if (j0 + k < n) {
+          const int8_t* a = src + static_cast<long long>(j0 + k) * p.ct;
+          if constexpr (W == 4) *reinterpret_cast<uint4*>(w[k]) = __ldg(reinterpret_cast<const uint4*>(a));
+          else if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = __ldg(reinterpret_cast<const uint2*>(a));
+          else w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(a));
+        }
+      }
+    };
+    if (nt > 0) load(0);
+    for (int i = 0; i < nt; ++i) {
+      const int slot = i & 1;
+      if (i >= 2 && !warp_all(mbar_wait_spin(bar_vempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)))
+        break;
+      uint8_t* dst = v_ring + slot * C::kVBytes;
+#pragma unroll
+      for (int x = 0; x < W; ++x) {
+        uint32_t lo[4], hi[4];  // pairs of keys of dims 4x, 4x + 1 and 4x + 2, 4x + 3
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t u0 = w[2 * k][x] ^ 0x80808080u, u1 = w[2 * k + 1][x] ^ 0x80808080u;
+          lo[k] = __byte_perm(u0, u1, 0x5140);
+          hi[k] = __byte_perm(u0, u1, 0x7362);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const int dim = dim0 + 4 * x + y;
+          const uint32_t(&z)[4] = y < 2 ? lo : hi;
+          uint4 o;
+          if (y & 1)
+            o = make_uint4(codes_to_half2<1>(z[0]), codes_to_half2<1>(z[1]), codes_to_half2<1>(z[2]), codes_to_half2<1>(z[3]));
+          else
+            o = make_uint4(codes_to_half2<0>(z[0]), codes_to_half2<0>(z[1]), codes_to_half2<0>(z[2]), codes_to_half2<0>(z[3]));
+          *reinterpret_cast<uint4*>(dst + dim * 128 + ((kc ^ (dim & 7)) << 4)) = o;
+        }
+      }
+      if (i + 1 < nt) load(i + 1);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_vfull(slot));
+    }
+  } else if (warp >= 5) {
+    // ------------------------------------------------ keys -> K (fp16)
+    constexpr int U = 2 * C::kSlices;  // (8 keys x 64 dims) units of a warp
+    const int kr = lane >> 2, c4 = lane & 3;
+    const int8_t* src = p.k + b * p.cb + h * p.ch;
+    uint4 w[U];
+    const auto load = [&](int i) {
+      const int j0 = (tile0 + i) * C::kKeys + kr;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int id = warp - 5 + 4 * u, j = j0 + 8 * (id / C::kSlices);
+        w[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (j < n)
+          w[u] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(j) * p.ct + 64 * (id % C::kSlices) + 16 * c4));
+      }
+    };
+    if (nt > 0) load(0);
+    for (int i = 0; i < nt; ++i) {
+      const int slot = i & 1;
+      if (i >= 2 && !warp_all(mbar_wait_spin(bar_kempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)))
+        break;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int id = warp - 5 + 4 * u, row = 8 * (id / C::kSlices) + kr;
+        uint8_t* dst = k_ring + slot * C::kKBytes + (id % C::kSlices) * (C::kKeys * 128) + row * 128;
+        const uint32_t x[4] = {w[u].x ^ 0x80808080u, w[u].y ^ 0x80808080u, w[u].z ^ 0x80808080u, w[u].w ^ 0x80808080u};
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+          *reinterpret_cast<uint4*>(dst + (((2 * c4 + y) ^ (row & 7)) << 4)) =
+              make_uint4(codes_to_half2<0>(x[2 * y]), codes_to_half2<1>(x[2 * y]), codes_to_half2<0>(x[2 * y + 1]),
+                         codes_to_half2<1>(x[2 * y + 1]));
+      }
+      if (i + 1 < nt) load(i + 1);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_kfull(slot));
+    }
+  } else {
+    // ------------------------------------------------ softmax + epilogue (warps 0-3)
+    const int row = warp * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+    const float2 info = row_info[row];
+    const float factor = info.x;
+    const int seen = __float_as_int(info.y);
+    const float* ks = p.ks + static_cast<long long>(unit) * (p.capacity / kKvBlock);
+    const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
+    float m = -INFINITY, l = 0.f, vref = 0.f;
+    bool alive = true;
+    for (int i = 0; alive && i < nt; ++i) {
+      const int slot = i & 1, j0 = (tile0 + i) * C::kKeys, blk = j0 / kKvBlock;
+      float ksc[4], vsc[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const bool has = blk + q < nblocks;
+        ksc[q] = has ? __ldg(ks + blk + q) : 0.f;
+        vsc[q] = has ? __ldg(vs + blk + q) : 0.f;
+      }
+      if (!warp_all(mbar_wait_spin(bar_sfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t raw[64];
+      {
+        const uint32_t t = tmem_base + lane_addr + C::kSCol + slot * C::kKeys;
+        tmem_ld_32x32b_x16(t, *reinterpret_cast<uint32_t(*)[16]>(&raw[0]));
+        tmem_ld_32x32b_x16(t + 16, *reinterpret_cast<uint32_t(*)[16]>(&raw[16]));
+        tmem_ld_32x32b_x16(t + 32, *reinterpret_cast<uint32_t(*)[16]>(&raw[32]));
+        tmem_ld_32x32b_x16(t + 48, *reinterpret_cast<uint32_t(*)[16]>(&raw[48]));
+        tmem_ld_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_sfree(slot));
+      // unseen keys of a row's last tiles: -inf, whatever their block's scale is
+      float bmax = -INFINITY;
+      const int left = seen - j0;
+      if (left >= C::kKeys) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float x = -INFINITY, y = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < 16; c += 2) {
+            x = fmaxf(x, __uint_as_float(raw[16 * q + c]));
+            y = fmaxf(y, __uint_as_float(raw[16 * q + c + 1]));
+          }
+          ksc[q] *= factor;
+          bmax = fmaxf(bmax, fmaxf(x, y) * ksc[q]);  // the factor is not negative
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          ksc[q] *= factor;
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const float v = 16 * q + c < left ? __uint_as_float(raw[16 * q + c]) * ksc[q] : -INFINITY;
+            raw[16 * q + c] = __float_as_uint(v);
+            bmax = fmaxf(bmax, v);
+          }
+          ksc[q] = 1.f;
+        }
+      }
+      float f = 1.f;
+      const bool grow = bmax > m + kAttn8Grow;
+      if (grow) {
+        f = m == -INFINITY ? 0.f : ex2_approx(m - bmax);
+        m = bmax;
+        l *= f;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f *= move_vref(vsc[q], vref);
+      if (i >= 1 && __any_sync(0xffffffffu, f != 1.f)) {
+        // O holds the earlier tiles: wait for the last of them, rescale this warp's rows
+        if (!warp_all(mbar_wait_spin(bar_pfree((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+          alive = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += 16) {
+          uint32_t o[16];
+          const uint32_t t = tmem_base + lane_addr + C::kOCol + c0;
+          tmem_ld_32x32b_x16(t, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+          tmem_st_32x32b_x16(t, o);
+        }
+        tmem_st_wait();
+      }
+      const float nm = m == -INFINITY ? 0.f : -m;
+      uint32_t pw[32];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float rv = vscale_ratio(vsc[q], vref);
+        float s2[2] = {0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float p0 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c]), ksc[q], nm));
+          const float p1 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c + 1]), ksc[q], nm));
+          s2[0] += p0;
+          s2[1] += p1;
+          pw[8 * q + c] = pack_half2_bits(weigh(p0, rv), weigh(p1, rv));
+        }
+        l += s2[0] + s2[1];
+      }
+      if (i >= 2 && !warp_all(mbar_wait_spin(bar_pfree(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+        alive = false;
+        break;
+      }
+      tc_fence_after();
+      tmem_st_32x32b_x32(tmem_base + lane_addr + C::kPCol + slot * 32, pw);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_pfull(slot));
+    }
+    // ---- epilogue: O vref / l, or the unnormalised O with (m, l)
+    const bool ok = alive && warp_all(mbar_wait_bounded(bar_o, 0, abort_flag, err, kErrWaitAccum, limit));
+    tc_fence_after();
+    const int r = r0 + row;
+    const bool part = p.splits > 1;
+    const float f = part ? vref : l == 0.f ? 0.f : vref / l;
+    const long long at = (static_cast<long long>(unit) * p.splits + split) * p.rows + r;
+    const int head = h * p.group + r % p.group;
+    T* dst = static_cast<T*>(p.out) +
+             ((static_cast<long long>(b) * p.tokens + r / p.group) * (p.heads * p.group) + head) * D;
+    if (ok && part && r < p.rows) p.part_ml[at] = make_float2(m, l);
+#pragma unroll 1
+    for (int c0 = 0; c0 < D; c0 += 16) {
+      uint32_t o[16];
+      if (ok && nt > 0) {
+        tmem_ld_32x32b_x16(tmem_base + lane_addr + C::kOCol + c0, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) o[c] = 0u;
+      }
+      if (!ok || r >= p.rows) continue;
+      // a row that saw nothing (l = 0) has P = 0 for every key
+      float v[2][8];
+#pragma unroll
+      for (int c = 0; c < 16; ++c) v[c >> 3][c & 7] = f == 0.f ? 0.f : __uint_as_float(o[c]) * f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (part) store8(p.part_o + at * D + c0 + 8 * c, v[c]);
+        else store8(dst + c0 + 8 * c, v[c]);
+      }
+    }
+  }
+  // every MMA has completed (the issuer waited for bar_o) before TMEM is freed
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::kTmemCols);
+  }
+}
+
+// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one warp per row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attn8_join_kernel(const __grid_constant__ Attn8Params p, long long units) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(p.batch) * p.tokens * p.q_heads) return;
-  const int qh = static_cast<int>(row % p.q_heads);
-  const int t = static_cast<int>(row / p.q_heads % p.tokens);
-  const int b = static_cast<int>(row / p.q_heads / p.tokens);
-  const int h = qh / (p.q_heads / p.heads);
-  const T* q = static_cast<const T*>(p.q) + b * p.qb + t * p.qt + qh * p.qh;
-  const int per = p.width / 32;  // 2, 4, 6 or 8 elements per lane
-  float qv[8], acc[8] = {};
+  const long long i = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (i >= units * p.rows) return;
+  const long long unit = i / p.rows;
+  const int r = static_cast<int>(i - unit * p.rows);
+  const float2* ml = p.part_ml + unit * p.splits * p.rows + r;
+  float mm = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, ml[static_cast<long long>(s) * p.rows].x);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) qv[i] = i < per ? to_float(q[lane + 32 * i]) : 0.f;
-  int keys = min(max(p.lengths[b], 0), p.capacity);
-  if (p.causal) keys = min(keys, keys - p.tokens + t + 1);
-  float m = -INFINITY, l = 0.f;
-  for (int j = 0; j < keys; ++j) {
-    const int8_t* k = p.k + b * p.cb + j * p.ct + h * p.ch;
-    const int8_t* v = p.v + b * p.cb + j * p.ct + h * p.ch;
-    const long long blk = (static_cast<long long>(b) * p.heads + h) * (p.capacity / kKvBlock) + j / kKvBlock;
-    float s = 0.f;
+  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  constexpr int V = D / 32;  // elements of a lane: 2, 4 or 8
+  float acc[V] = {};
+  float sum = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[static_cast<long long>(s) * p.rows];
+    const float* src = p.part_o + ((unit * p.splits + s) * p.rows + r) * D + lane * V;
+    const float f = x.y == 0.f ? 0.f : ex2_approx(x.x - mm);
+    sum = fmaf(x.y, f, sum);
+    float v[V];
+    if constexpr (V == 2) *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < per) s = fmaf(qv[i], static_cast<float>(k[lane + 32 * i]), s);
+      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(src + j);
+    }
+    if (x.y != 0.f) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= p.scale * p.ks[blk];
-    const float mn = fmaxf(m, s);
-    const float a = __expf(m - mn), e = __expf(s - mn);
-    l = l * a + e;
-    m = mn;
-    const float w = e * p.vs[blk];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < per) acc[i] = fmaf(w, static_cast<float>(v[lane + 32 * i]), acc[i] * a);
+      for (int j = 0; j < V; ++j) acc[j] = fmaf(v[j], f, acc[j]);
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* out = static_cast<T*>(p.out) + row * p.width;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int b = static_cast<int>(unit / p.heads), h = static_cast<int>(unit % p.heads);
+  const int tok = r / p.group, head = h * p.group + r % p.group;
+  T* dst = static_cast<T*>(p.out) + ((static_cast<long long>(b) * p.tokens + tok) * (p.heads * p.group) + head) * D + lane * V;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < per) out[lane + 32 * i] = from_float<T>(acc[i] * inv);
+  for (int j = 0; j < V; ++j) dst[j] = from_float<T>(acc[j] * inv);
 }
 
 }  // namespace w4a4

@@ -339,13 +339,19 @@ Tensor kv_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
   Tensor out = at::empty(q.sizes(), q.options());
   if (q.numel() == 0) return out;
   const int64_t qs[3] = {qr.stride(0), qr.stride(1), qr.stride(2)};
+  int64_t bytes = 0;
+  check_status(w4a4_attention8_workspace(as_i32(c.batch, "the batch"), as_i32(q.size(1), "the token count"),
+                                         as_i32(q.size(2), "the query head count"), as_i32(c.heads, "the head count"),
+                                         as_i32(c.width, "the head width"), as_i32(c.capacity, "the capacity"), &bytes));
+  Tensor workspace;
+  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
   check_status(w4a4_attention8(qr.const_data_ptr(), qs, k_cache.const_data_ptr<int8_t>(),
                                v_cache.const_data_ptr<int8_t>(), k_scale.const_data_ptr<float>(),
                                v_scale.const_data_ptr<float>(), c.stride, as_i32(c.capacity, "the capacity"), len, dt,
                                as_i32(c.batch, "the batch"), as_i32(q.size(1), "the token count"),
                                as_i32(q.size(2), "the query head count"), as_i32(c.heads, "the head count"),
                                as_i32(c.width, "the head width"), causal ? 1 : 0, static_cast<float>(scale),
-                               out.data_ptr(), stream_of(q)));
+                               out.data_ptr(), bytes > 0 ? workspace.data_ptr() : nullptr, bytes, stream_of(q)));
   return out;
 }
 

@@ -27,6 +27,19 @@ int by_dtype(int32_t dtype, bool fp32_too, const char* what, F f) {
 
 int elem_size(int32_t dtype) { return dtype == W4A4_F32 ? 4 : 2; }
 
+// Kernels of this file whose dynamic shared memory has been raised, by device
+// and number.
+uint64_t g_attr8_done[kMaxDevices];
+template <class Kernel>
+int ensure_smem_attr8(int dev, int bit, Kernel kernel, int bytes) {
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  if (!(g_attr8_done[dev] >> bit & 1)) {
+    W4A4_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    g_attr8_done[dev] |= 1ull << bit;
+  }
+  return W4A4_OK;
+}
+
 // Whether rows of `stride` elements of `size` bytes from p all begin at a
 // multiple of `bytes`.
 bool rows_aligned(const void* p, int64_t stride, int size, int bytes) {
@@ -82,13 +95,13 @@ int launch_gemm8(const Gemm8Params& p, int32_t dtype, cudaStream_t stream) {
   });
 }
 
-// Shape and layout of a cache: width a multiple of 64 up to 256, capacity a
+// Shape and layout of a cache: width 64, 128 or 256, capacity a
 // multiple of 16, strides and bases multiples of 16 bytes.
 int check_cache8(const void* k, const void* v, const void* ks, const void* vs, const int64_t* stride, int32_t batch,
                  int32_t heads, int32_t width, int32_t capacity, const char* what) {
   if (batch < 0 || heads <= 0) return fail(W4A4_ERR_INVALID, "%s: invalid batch %d or heads %d", what, batch, heads);
-  if (width <= 0 || width % 64 || width > 256)
-    return fail(W4A4_ERR_UNSUPPORTED, "%s: head width must be 64, 128, 192 or 256, got %d", what, width);
+  if (width != 64 && width != 128 && width != 256)
+    return fail(W4A4_ERR_UNSUPPORTED, "%s: head width must be 64, 128 or 256, got %d", what, width);
   if (capacity <= 0 || capacity % kKvBlock)
     return fail(W4A4_ERR_INVALID, "%s: the capacity must be a positive multiple of %d, got %d", what, kKvBlock, capacity);
   if (static_cast<int64_t>(batch) * heads > 65535)
@@ -103,12 +116,62 @@ int check_cache8(const void* k, const void* v, const void* ks, const void* vs, c
   return W4A4_OK;
 }
 
-int launch_attention8(const Attn8Params& p, int32_t dtype, cudaStream_t stream) {
+// How many CTAs the keys of one key/value head are split over, from the
+// cache's capacity (the lengths are on the device; a split without keys writes
+// an empty part).
+constexpr int kAttn8FewRows = 16;
+struct Attn8Plan {
+  bool few;
+  int tiles;   // row tiles of the many-rows form
+  int splits;
+};
+Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, int sms) {
+  Attn8Plan plan{};
+  plan.few = rows <= kAttn8FewRows;
+  plan.tiles = static_cast<int>((rows + 127) / 128);
+  const int64_t work = units * (plan.few ? 1 : plan.tiles);
+  // keys that make a split worth its part of the join
+  const int64_t most = plan.few ? (capacity + 511) / 512 : (capacity + 255) / 256;
+  plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, sms / std::max<int64_t>(work, 1), 256})));
+  return plan;
+}
+
+template <typename T, int D>
+int launch_attention8_d(const Attn8Params& p, const Attn8Plan& plan, int64_t units, int dev, int bit,
+                        cudaStream_t stream) {
+  if (plan.few) {
+    const bool half = p.rows <= 8;
+    const auto kernel = half ? attn8_few_kernel<T, D, true> : attn8_few_kernel<T, D, false>;
+    if (int e = ensure_smem_attr8(dev, bit + (half ? 0 : 1), kernel, Attn8Few<D>::kSmem)) return e;
+    W4A4_CUDA_TRY(launch_kernel(kernel, dim3(p.splits, static_cast<unsigned>(units)), dim3(Attn8Few<D>::kThreads),
+                                Attn8Few<D>::kSmem, stream, 1, p));
+  } else {
+    const auto kernel = attn8_many_kernel<T, D>;
+    if (int e = ensure_smem_attr8(dev, bit + 2, kernel, Attn8Many<D>::kSmem)) return e;
+    W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.tiles, p.splits, static_cast<unsigned>(units)),
+                                dim3(Attn8Many<D>::kThreads), Attn8Many<D>::kSmem, stream, 1, p));
+  }
+  if (p.splits > 1) {
+    const int64_t rows = units * p.rows;
+    W4A4_CUDA_TRY(launch_kernel(attn8_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream, 1, p,
+                                static_cast<long long>(units)));
+  }
+  return ok();
+}
+
+int launch_attention8(const Attn8Params& p, const Attn8Plan& plan, int64_t units, int width, int32_t dtype, int dev,
+                      cudaStream_t stream) {
   return by_dtype(dtype, false, "attention8", [&](auto tag) {
     using T = decltype(tag);
-    const int64_t rows = static_cast<int64_t>(p.batch) * p.tokens * p.q_heads;
-    const dim3 grid(static_cast<unsigned>((rows + 3) / 4));
-    return cuda_status(launch_kernel(attn8_simple_kernel<T>, grid, dim3(128), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+    if constexpr (std::is_same_v<T, float>) return fail(W4A4_ERR_INVALID, "attention8: unsupported dtype");
+    else {
+      const int bit = std::is_same_v<T, __half> ? 0 : 12;
+      switch (width) {
+        case 64: return launch_attention8_d<T, 64>(p, plan, units, dev, bit, stream);
+        case 128: return launch_attention8_d<T, 128>(p, plan, units, dev, bit + 4, stream);
+        default: return launch_attention8_d<T, 256>(p, plan, units, dev, bit + 8, stream);
+      }
+    }
   });
 }
 
@@ -240,13 +303,31 @@ int w4a4_kv8_values(const int8_t* k_codes, const int8_t* v_codes, const float* k
   });
 }
 
+int w4a4_attention8_workspace(int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads, int32_t width,
+                              int32_t capacity, int64_t* bytes) {
+  if (!bytes) return fail(W4A4_ERR_INVALID, "attention8: null pointer argument");
+  if (batch < 0 || tokens < 0 || heads <= 0 || q_heads <= 0 || q_heads % heads || width <= 0 || capacity < 0)
+    return fail(W4A4_ERR_INVALID, "attention8: invalid shape");
+  *bytes = 0;
+  if (batch == 0 || tokens == 0) return ok();
+  int dev, sms;
+  if (int e = current_device(&dev)) return e;
+  if (int e = sm_count(dev, &sms)) return e;
+  const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, sms);
+  if (plan.splits > 1) *bytes = units * plan.splits * rows * (static_cast<int64_t>(width) * 4 + 8);
+  return ok();
+}
+
 int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_codes, const int8_t* v_codes,
                     const float* k_scale, const float* v_scale, const int64_t* cache_stride, int32_t capacity,
                     const int32_t* lengths, int32_t dtype, int32_t batch, int32_t tokens, int32_t q_heads, int32_t heads,
-                    int32_t width, int32_t causal, float scale, void* out, void* stream) {
+                    int32_t width, int32_t causal, float scale, void* out, void* workspace, int64_t workspace_bytes,
+                    void* stream) {
   if (int e = check_cache8(k_codes, v_codes, k_scale, v_scale, cache_stride, batch, heads, width, capacity,
                            "attention8"))
     return e;
+  if (dtype != W4A4_F16 && dtype != W4A4_BF16) return fail(W4A4_ERR_INVALID, "attention8: unsupported dtype code %d", dtype);
   if (tokens < 0 || q_heads <= 0 || q_heads % heads)
     return fail(W4A4_ERR_INVALID, "attention8: invalid tokens %d or %d query heads over %d heads", tokens, q_heads, heads);
   if (batch == 0 || tokens == 0) return ok();
@@ -255,13 +336,27 @@ int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_code
     return fail(W4A4_ERR_INVALID, "attention8: query rows must begin at multiples of 16 bytes");
   if (static_cast<int64_t>(batch) * tokens * q_heads > 0x7fffffffLL)
     return fail(W4A4_ERR_UNSUPPORTED, "attention8: too many query rows");
+  int dev, sms;
+  if (int e = current_device(&dev)) return e;
+  if (int e = sm_count(dev, &sms)) return e;
+  const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, sms);
   Attn8Params p{};
   p.q = q, p.out = out, p.k = k_codes, p.v = v_codes, p.ks = k_scale, p.vs = v_scale, p.lengths = lengths;
   p.qb = q_stride[0], p.qt = q_stride[1], p.qh = q_stride[2];
   p.cb = cache_stride[0], p.ct = cache_stride[1], p.ch = cache_stride[2];
-  p.batch = batch, p.tokens = tokens, p.q_heads = q_heads, p.heads = heads, p.width = width, p.capacity = capacity;
-  p.causal = causal != 0, p.scale = scale;
-  return launch_attention8(p, dtype, static_cast<cudaStream_t>(stream));
+  p.tokens = tokens, p.heads = heads, p.group = q_heads / heads, p.capacity = capacity;
+  p.rows = static_cast<int>(rows), p.splits = plan.splits;
+  p.causal = causal != 0, p.scale = scale * 1.4426950408889634f, p.wait_limit_ns = g_wait_limit_ns.load();
+  if (plan.splits > 1) {
+    const int64_t parts = units * plan.splits * rows, need = parts * (static_cast<int64_t>(width) * 4 + 8);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+      return fail(W4A4_ERR_INVALID, "attention8: needs a 16-byte aligned workspace of %lld bytes, got %lld", (long long)need,
+                  (long long)(workspace ? workspace_bytes : 0));
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + parts * width);
+  }
+  return launch_attention8(p, plan, units, width, dtype, dev, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

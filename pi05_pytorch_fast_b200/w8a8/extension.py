@@ -97,8 +97,8 @@ class Int8Weight(NamedTuple):
 
 
 class KVCache8(NamedTuple):
-    """Keys and values int8 [batch, capacity, heads, width] (width 64, 128, 192
-    or 256) and their scales fp32 [batch, heads, capacity / 16].  How many
+    """Keys and values int8 [batch, capacity, heads, width] (width 64, 128 or
+    256) and their scales fp32 [batch, heads, capacity / 16].  How many
     tokens of each sequence are filled is the caller's: an int32 tensor
     [batch] on the device, given to and returned by ``kv_append``."""
 

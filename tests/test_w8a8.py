@@ -325,7 +325,7 @@ APPEND_CASES = [
     (1, 256, 832, (0, 0), 776, 0.8, torch.float16),
     (2, 64, 96, (0, 5, 31, 64), 17, None, torch.float16),
     (4, 128, 64, (3, 17), 40, 0.5, torch.bfloat16),
-    (1, 192, 48, (1, 2, 3), 45, 0.0, torch.bfloat16),
+    (1, 64, 48, (1, 2, 3), 45, 0.0, torch.bfloat16),
     (8, 64, 1312, (7,), 1300, 0.97, torch.float16),
     (1, 128, 16, (0, 16, 9), 7, None, torch.float16),
 ]
@@ -433,7 +433,7 @@ ATTEND_CASES = [
     (4, 4, 128, 64, (33, 64, 7), 1, True, torch.float16),
     (16, 2, 128, 4112, (4101, 1027, 16, 15, 0), 1, True, torch.float16),
     (6, 2, 64, 160, (160, 131, 17), 17, True, torch.bfloat16),
-    (5, 1, 192, 224, (211, 100), 13, True, torch.float16),
+    (5, 1, 256, 224, (211, 100), 13, True, torch.float16),
     (8, 1, 256, 1040, (1033, 700), 129, True, torch.bfloat16),
     (8, 8, 64, 512, (505, 64), 64, True, torch.float16),
     (2, 1, 64, 96, (20, 3, 0), 33, True, torch.float16),  # more queries than tokens: rows that see nothing
@@ -684,7 +684,7 @@ def test_c_abi_argument_checks_without_gpu():
     assert "131072" in message(lib.w4a4_gemm8(*with_(gemm, _10=131072, _1=131072, _4=131072)), nat.W4A4_ERR_UNSUPPORTED)
     assert lib.w4a4_gemm8(*with_(gemm, _8=0)) == 0
     strides = (ctypes.c_int64 * 3)(64 * 32, 64, 64)
-    att = [fake, strides, fake, fake, fake, fake, strides, 32, fake, nat.F16, 1, 1, 4, 2, 64, 0, 1.0, fake, None]
+    att = [fake, strides, fake, fake, fake, fake, strides, 32, fake, nat.F16, 1, 1, 4, 2, 64, 0, 1.0, fake, None, 0, None]
     assert "query heads" in message(lib.w4a4_attention8(*with_(att, _12=3)), bad)
     assert "capacity" in message(lib.w4a4_attention8(*with_(att, _7=33)), bad)
     assert "width" in message(lib.w4a4_attention8(*with_(att, _14=72)), nat.W4A4_ERR_UNSUPPORTED)
@@ -739,4 +739,4 @@ def test_ops_refuse_bad_arguments():
     refuses("multiple of 16", lambda: w8a8.kv_values(cache._replace(keys=cache.keys[:, :20], values=cache.values[:, :20]), n))
     refuses("cache scales must be", lambda: w8a8.kv_values(cache._replace(key_scale=cache.key_scale[..., :1]), n))
     wide = w8a8.KVCache8.allocate(2, 32, 2, 72, DEV)
-    refuses("64, 128, 192 or 256", lambda: w8a8.kv_values(wide, n))
+    refuses("64, 128 or 256", lambda: w8a8.kv_values(wide, n))
