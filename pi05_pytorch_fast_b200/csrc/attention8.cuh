@@ -56,6 +56,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -73,25 +76,9 @@ __device__ __forceinline__ uint32_t codes_to_half2(uint32_t w) {
 // D (16 x 8, fp32) += A (16 x 16, fp16) B (16 x 8, fp16).
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The same with rows 8-15 of A zero: only d[0] and d[1] (rows 0-7) are kept.
-__device__ __forceinline__ void mma_16816_half(float (&d)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  float x, y;
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %9, %9};"
-      : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
-      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
-}
-template <bool HALF>
-__device__ __forceinline__ void mma_rows(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  if constexpr (HALF) mma_16816_half(d, a0, a2, b0, b1);
-  else mma_16816(d, a0, a1, a2, a3, b0, b1);
 }
 
 // Ratio of a block's value scale to the reference, and the reference's move:
@@ -125,32 +112,39 @@ __device__ __forceinline__ int keys_seen(const Attn8Params& p, int n, int t) {
 }
 
 // ------------------------------------------------------- few rows (<= 16)
-// The form for single tokens.  One CTA of 8 warps per (split, key/value head);
-// every warp takes every eighth block of 16 keys of the CTA's range on its own,
-// through its own ring of cp.async stages in shared memory (no barrier
-// between warps until the end), with mma.sync m16n8k16: the 16 rows are the
-// heads of the group, so a block's K and V are read once for all of them.
-// The K index of an MMA may be permuted freely when both operands agree, and
-// so may the columns of V; so every lane reads 16 consecutive bytes:
-//  * K: lane (g, t) of a key row g reads dims 64 c + 16 t ... + 15 = four steps
-//    of four dims, Q is read from shared memory in the same order;
-//  * V: lane (g, t) reads dims 16 g ... + 15 of the keys 2t, 2t+1, 2t+8, 2t+9;
+// The form for single tokens.  The warps of all CTAs of one key/value head
+// (splits x kWarps) take its steps of 256 / D blocks of 16 keys in turn, each
+// on its own, through its own ring of cp.async stages of 8 KB, with mma.sync
+// m16n8k16: the 16 rows are the heads of the group, so a block's K and V are
+// read once for all of them.  The K index of an MMA may be permuted freely
+// when both operands agree, and so may the columns of V; so every lane reads
+// 16 consecutive bytes:
+//  * K: lane (g, t) of a key row g holds dims 64 c + 16 t ... + 15 = four steps
+//    of four dims, and Q's fragments are kept in the same order;
+//  * V: lane (g, t) holds dims 16 g ... + 15 of the keys 2t, 2t+1, 2t+8, 2t+9;
 //    pairs of keys are zipped with byte permutes; column n of tile e is dim
 //    16 n + e, so a lane ends with runs of 16 consecutive dims of O.
-// Bound: HBM (2 width bytes per key).  Legacy MMA is enough here: a block costs
-// a warp under 1000 cycles and 8 warps need one each 2800 to keep up.
-template <int D>
+// P goes in as the sum of two fp16, its rounding and the rest: with at most 8
+// rows (HALF) the rest takes the idle rows 8-15 of the same MMA, with more it
+// is a second one.  Bound: HBM (2 width bytes per key); legacy MMA is enough
+// for it.  Which warp takes which keys does not depend on the lengths, so the
+// first loads are under way before the length has arrived.
+template <int D, bool HALF>
 struct Attn8Few {
-  static constexpr int kWarps = 8;
+  static constexpr int kWarps = 8, kStages = 3;
   static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kRowsMax = HALF ? 8 : 16;
+  static constexpr int kBlocks = 256 / D;           // token blocks of a step
   static constexpr int kChunks = D / 16;            // 16-byte chunks of a key
-  static constexpr int kHalfStage = kKvBlock * D;   // K or V of a block
-  static constexpr int kStages = D == 256 ? 3 : D == 128 ? 5 : 8;
-  static constexpr int kRing = kStages * 2 * kHalfStage;  // per warp
+  static constexpr int kHalfStage = kKvBlock * 256; // K or V of a step
+  static constexpr int kStage = 2 * kHalfStage + 64;  // K, V, scales
+  static constexpr int kRing = kStages * kStage;    // of a warp
   static constexpr int kPad = D + 4;                // row of the O exchange (floats)
   static constexpr int kQBytes = 16 * D * 2;
-  static constexpr int kSmem = kQBytes + 16 * 8 + kWarps * 16 * 8 + kWarps * (kRing > 16 * kPad * 4 ? kRing : 16 * kPad * 4);
-  // byte offset of 16-byte chunk c of key row r
+  static constexpr int kExchange = (kWarps + 1) * kRowsMax * kPad * 4;  // in the rings, when they are idle
+  static constexpr int kSmem = kQBytes + 16 * 8 + (kWarps + 1) * kRowsMax * 8 + kWarps * kRing;
+  static_assert(kExchange <= kWarps * kRing, "the exchange must fit the rings");
+  // byte offset of 16-byte chunk c of key row r: swizzled so that the reads below hit every bank once
   __device__ static __forceinline__ int k_at(int r, int c) {
     const int l = r * kChunks + c;
     return 16 * (D >= 128 ? l ^ ((r & 1) << 2) : l);
@@ -158,47 +152,93 @@ struct Attn8Few {
   __device__ static __forceinline__ int v_at(int r, int c) { return 16 * ((r * kChunks + c) ^ (((r >> 1) & 3) << 1)); }
 };
 
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+// 4 consecutive results, rounded once.
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, const float4& v) {
+  if constexpr (std::is_same_v<T, __half>) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2_bits(v.x, v.y), pack_half2_bits(v.z, v.w));
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  }
+}
+// Row r of a key/value head's rows (unit = batch x heads) in the output.
+__device__ __forceinline__ long long out_row(const Attn8Params& p, int b, int h, int r) {
+  return (static_cast<long long>(b) * p.tokens + r / p.group) * (p.heads * p.group) + h * p.group + r % p.group;
+}
+
 template <typename T, int D, bool HALF>
-__global__ void __launch_bounds__(Attn8Few<D>::kThreads, 1) attn8_few_kernel(const __grid_constant__ Attn8Params p) {
-  using C = Attn8Few<D>;
+__global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
+    attn8_few_kernel(const __grid_constant__ Attn8Params p) {
+  using C = Attn8Few<D, HALF>;
   extern __shared__ __align__(128) uint8_t few_smem[];
   uint8_t* q_smem = few_smem;                                        // fp16 [16][D], chunk c of row r at c ^ (r & 1)
   float2* row_info = reinterpret_cast<float2*>(q_smem + C::kQBytes); // score factor, keys seen
-  float2* warp_ml = row_info + 16;                                   // [warps][16]
-  uint8_t* rings = reinterpret_cast<uint8_t*>(warp_ml + C::kWarps * 16);
+  float2* warp_ml = row_info + 16;                                   // [warps + 1][rows]; the last is the CTA's
+  uint8_t* rings = reinterpret_cast<uint8_t*>(warp_ml + (C::kWarps + 1) * C::kRowsMax);
+  float* xo = reinterpret_cast<float*>(rings);                       // [warps + 1][rows][kPad], after the last step
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x, unit = blockIdx.y;
   const int b = unit / p.heads, h = unit - b * p.heads;
   pdl_launch_dependents();
   pdl_wait();
-  const int n = min(max(p.lengths[b], 0), p.capacity);
-  const int nblk = (n + kKvBlock - 1) / kKvBlock;
-  const int per = (nblk + p.splits - 1) / p.splits;
-  const int blk0 = split * per, blk1 = min(nblk, blk0 + per);
   const int8_t* kc = p.k + b * p.cb + h * p.ch;
   const int8_t* vc = p.v + b * p.cb + h * p.ch;
-  const float* ks = p.ks + static_cast<long long>(unit) * (p.capacity / kKvBlock);
-  const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
+  const int blocks = p.capacity / kKvBlock;
+  const float* ks = p.ks + static_cast<long long>(unit) * blocks;
+  const float* vs = p.vs + static_cast<long long>(unit) * blocks;
+  constexpr int KC = D / 64;                   // 64-dim chunks of a key
+  constexpr int VU = D >= 128 ? D / 128 : 1;   // runs of dims of a lane
+  constexpr int VW = D >= 128 ? 4 : 2;         // words of a run
+  constexpr int NB = C::kBlocks;
   uint8_t* ring = rings + warp * C::kRing;
-  const uint32_t ring_addr = smem_addr(ring);
-  // slots up to the end of the cache's last block exist, so whole blocks are read
-  const auto fetch = [&](int blk, int stage) {
-    const int8_t* kb = kc + static_cast<long long>(blk) * kKvBlock * p.ct;
-    const int8_t* vb = vc + static_cast<long long>(blk) * kKvBlock * p.ct;
-    const uint32_t dst = ring_addr + stage * 2 * C::kHalfStage;
+  // a step's keys, values and scales into a stage (every slot of a block exists, the capacity being a multiple of 16)
+  const auto fetch = [&](int step, int stage) {
+    const uint32_t dst = smem_addr(ring) + stage * C::kStage;
+    const int blk = step * NB;
+    const int rows = min(blocks - blk, NB) * kKvBlock;
+    const int r0 = lane / C::kChunks, c = lane % C::kChunks;
+    const long long at = (static_cast<long long>(blk) * kKvBlock + r0) * p.ct + 16 * c;
+    const int8_t* kb = kc + at;
+    const int8_t* vb = vc + at;
+    constexpr int kStep = 32 / C::kChunks;  // rows of a warp's instruction
 #pragma unroll
-    for (int i = 0; i < kKvBlock * C::kChunks / 32; ++i) {
-      const int l = lane + 32 * i, r = l / C::kChunks, c = l % C::kChunks;
-      cp_async16(dst + C::k_at(r, c), kb + r * p.ct + 16 * c);
-      cp_async16(dst + C::kHalfStage + C::v_at(r, c), vb + r * p.ct + 16 * c);
+    for (int i = 0; i < kKvBlock * NB / kStep; ++i) {
+      const int r = r0 + kStep * i;
+      if (NB == 1 || r < rows) {
+        cp_async16(dst + C::k_at(r, c), kb + i * kStep * p.ct);
+        cp_async16(dst + C::kHalfStage + C::v_at(r, c), vb + i * kStep * p.ct);
+      }
     }
+    if (lane < 2 * NB && blk + (lane >> 1) < blocks)
+      cp_async4(dst + 2 * C::kHalfStage + 4 * lane, (lane & 1 ? vs : ks) + blk + (lane >> 1));
   };
+  const int stride = p.splits * C::kWarps;
+  int step = split * C::kWarps + warp;
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) {
-    const int blk = blk0 + warp + C::kWarps * i;
-    if (blk < blk1) fetch(blk, i);
+    if ((step + i * stride) * NB < blocks) fetch(step + i * stride, i);
     cp_async_commit();
   }
+  const int n = min(max(p.lengths[b], 0), p.capacity);
+  const int nblk = (n + kKvBlock - 1) / kKvBlock;
+  const int nsteps = (nblk + NB - 1) / NB;
   {
     // Q: 16 threads per row, D / 16 consecutive elements each
     constexpr int E = D / 16;
@@ -251,68 +291,91 @@ __global__ void __launch_bounds__(Attn8Few<D>::kThreads, 1) attn8_few_kernel(con
   for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
 
   int stage = 0;
-  for (int blk = blk0 + warp; blk < blk1; blk += C::kWarps) {
-    const float ksc = __ldg(ks + blk), vsc = __ldg(vs + blk);
+  for (; step < nsteps; step += stride) {
     cp_async_wait<C::kStages - 2>();
     __syncwarp();
     {
-      const int next = blk + C::kWarps * (C::kStages - 1);
-      if (next < blk1) fetch(next, stage == 0 ? C::kStages - 1 : stage - 1);
+      const int next = step + stride * (C::kStages - 1);
+      if (next < nsteps) fetch(next, stage == 0 ? C::kStages - 1 : stage - 1);
       cp_async_commit();
     }
-    const uint8_t* kt = ring + stage * 2 * C::kHalfStage;
+    const uint8_t* kt = ring + stage * C::kStage;
     const uint8_t* vt = kt + C::kHalfStage;
+    const float2* sc = reinterpret_cast<const float2*>(vt + C::kHalfStage);
     stage = stage + 1 == C::kStages ? 0 : stage + 1;
-    // ---- S (rows x 16 keys): keys 2t, 2t + 1 of tile 0, and 8 more in tile 1
-    float s0[4] = {}, s1[4] = {};
+    // ---- S (rows x 16 NB keys): tile 2q + i has keys 16q + 8i + 2t, + 1
+    float s[2 * NB][4] = {};
+    float s2[NB == 1 ? 2 : 1][4] = {};  // D = 256: a second accumulator halves the chain of dependent products
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(kt + C::k_at(g, 4 * c + t));
-      const uint4 k1 = *reinterpret_cast<const uint4*>(kt + C::k_at(g + 8, 4 * c + t));
+    for (int c = 0; c < KC; ++c) {
       uint32_t qa[8], qb[8];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const int chunk = 8 * c + 2 * t + u;
-        *reinterpret_cast<uint4*>(&qa[4 * u]) =
-            *reinterpret_cast<const uint4*>(q_smem + g * 2 * D + ((chunk ^ (g & 1)) << 4));
+        const int at = ((8 * c + 2 * t + u) ^ (g & 1)) << 4;
+        *reinterpret_cast<uint4*>(&qa[4 * u]) = *reinterpret_cast<const uint4*>(q_smem + g * 2 * D + at);
         if constexpr (!HALF)
-          *reinterpret_cast<uint4*>(&qb[4 * u]) =
-              *reinterpret_cast<const uint4*>(q_smem + (g + 8) * 2 * D + ((chunk ^ (g & 1)) << 4));
+          *reinterpret_cast<uint4*>(&qb[4 * u]) = *reinterpret_cast<const uint4*>(q_smem + (g + 8) * 2 * D + at);
         else
           qb[4 * u] = qb[4 * u + 1] = qb[4 * u + 2] = qb[4 * u + 3] = 0u;
       }
-      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint32_t u0 = w0[s] ^ 0x80808080u, u1 = w1[s] ^ 0x80808080u;
-        mma_rows<HALF>(s0, qa[2 * s], qb[2 * s], qa[2 * s + 1], qb[2 * s + 1], codes_to_half2<0>(u0), codes_to_half2<1>(u0));
-        mma_rows<HALF>(s1, qa[2 * s], qb[2 * s], qa[2 * s + 1], qb[2 * s + 1], codes_to_half2<0>(u1), codes_to_half2<1>(u1));
+      for (int i = 0; i < 2 * NB; ++i) {
+        const uint4 k = *reinterpret_cast<const uint4*>(kt + C::k_at(8 * i + g, 4 * c + t));
+        const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t u = w[x] ^ 0x80808080u;
+          mma_16816(NB == 1 && (x & 1) ? s2[i & 1] : s[i], qa[2 * x], qb[2 * x], qa[2 * x + 1], qb[2 * x + 1],
+                    codes_to_half2<0>(u), codes_to_half2<1>(u));
+        }
       }
     }
-    // ---- softmax of the block
-    const int j0 = blk * kKvBlock + 2 * t;
+    if constexpr (NB == 1) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] += s2[i][j];
+    }
+    // ---- softmax of the step
+    const int j0 = step * NB * kKvBlock + 2 * t;
+    float vsc[NB];
+    float bm[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) bm[i] = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+      const bool has = step * NB + q < nblk;  // past the length: what the stage holds is not a scale
+      const float2 x = sc[q];
+      vsc[q] = has ? x.y : 0.f;
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float fk = has ? factor[i] * x.x : 0.f;
+        const int left = seen[i] - j0 - 16 * q;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float& v = s[2 * q + (j >> 1)][2 * i + (j & 1)];
+          v = (j & 1) + 8 * (j >> 1) < left ? v * fk : -INFINITY;
+          bm[i] = fmaxf(bm[i], v);
+        }
+      }
+    }
     float f[R];
     bool grow = false;
-    float pr[R][4];
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const float fk = factor[i] * ksc;
-      pr[i][0] = j0 < seen[i] ? s0[2 * i] * fk : -INFINITY;
-      pr[i][1] = j0 + 1 < seen[i] ? s0[2 * i + 1] * fk : -INFINITY;
-      pr[i][2] = j0 + 8 < seen[i] ? s1[2 * i] * fk : -INFINITY;
-      pr[i][3] = j0 + 9 < seen[i] ? s1[2 * i + 1] * fk : -INFINITY;
-      float bm = fmaxf(fmaxf(pr[i][0], pr[i][1]), fmaxf(pr[i][2], pr[i][3]));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 1));
-      bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, 2));
+      bm[i] = fmaxf(bm[i], __shfl_xor_sync(0xffffffffu, bm[i], 1));
+      bm[i] = fmaxf(bm[i], __shfl_xor_sync(0xffffffffu, bm[i], 2));
       f[i] = 1.f;
-      if (bm > m[i] + kAttn8Grow) {
-        f[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm);
-        m[i] = bm;
+      if (bm[i] > m[i] + kAttn8Grow) {
+        f[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm[i]);
+        m[i] = bm[i];
         l[i] *= f[i];
         grow = true;
       }
     }
-    const float fv = move_vref(vsc, vref);
+    float fv = 1.f;
+#pragma unroll
+    for (int q = 0; q < NB; ++q) fv *= move_vref(vsc[q], vref);
     if (__any_sync(0xffffffffu, grow) || fv != 1.f) {
 #pragma unroll
       for (int e = 0; e < D / 8; ++e)
@@ -320,103 +383,161 @@ __global__ void __launch_bounds__(Attn8Few<D>::kThreads, 1) attn8_few_kernel(con
         for (int i = 0; i < R; ++i) {
           o[e][2 * i] *= f[i] * fv;
           o[e][2 * i + 1] *= f[i] * fv;
+          if constexpr (HALF) {  // rows 8-15 hold what the rest of P adds to rows 0-7
+            o[e][2] *= f[0] * fv;
+            o[e][3] *= f[0] * fv;
+          }
         }
     }
-    const float rv = vscale_ratio(vsc, vref);
-    uint32_t pa[R][2];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const float nm = m[i] == -INFINITY ? 0.f : -m[i];
+    for (int q = 0; q < NB; ++q) {
+      const float rv = vscale_ratio(vsc[q], vref);
+      uint32_t ph[R][2], pl[R][2];  // P and the rest of its rounding: [rows][keys]
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        pr[i][j] = ex2_approx(pr[i][j] + nm);
-        l[i] += pr[i][j];
+      for (int i = 0; i < R; ++i) {
+        const float nm = m[i] == -INFINITY ? 0.f : -m[i];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float p0 = ex2_approx(s[2 * q + j][2 * i] + nm), p1 = ex2_approx(s[2 * q + j][2 * i + 1] + nm);
+          l[i] += p0 + p1;
+          const float w0 = weigh(p0, rv), w1 = weigh(p1, rv);
+          const __half2 hi = __floats2half2_rn(w0, w1);
+          const float2 back = __half22float2(hi);
+          ph[i][j] = *reinterpret_cast<const uint32_t*>(&hi);
+          pl[i][j] = pack_half2_bits(w0 - back.x, w1 - back.y);
+        }
       }
-      pa[i][0] = pack_half2_bits(weigh(pr[i][0], rv), weigh(pr[i][1], rv));
-      pa[i][1] = pack_half2_bits(weigh(pr[i][2], rv), weigh(pr[i][3], rv));
-    }
-    const uint32_t a1 = HALF ? 0u : pa[R - 1][0], a3 = HALF ? 0u : pa[R - 1][1];
-    // ---- O += P V
-    constexpr int VW = D >= 128 ? 4 : 2;  // words of a lane's run of dims
+      // ---- O += P V
 #pragma unroll
-    for (int u = 0; u < (D >= 128 ? D / 128 : 1); ++u) {
-      uint32_t w[4][VW];
+      for (int u = 0; u < VU; ++u) {
+        uint32_t vr[4][VW];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 2 * t + (i & 1) + 8 * (i >> 1);
-        if constexpr (VW == 4)
-          *reinterpret_cast<uint4*>(w[i]) = *reinterpret_cast<const uint4*>(vt + C::v_at(r, g + 8 * u));
-        else
-          *reinterpret_cast<uint2*>(w[i]) = *reinterpret_cast<const uint2*>(vt + C::v_at(r, g >> 1) + 8 * (g & 1));
+        for (int i = 0; i < 4; ++i) {
+          const int r = 16 * q + 2 * t + (i & 1) + 8 * (i >> 1);
+          if constexpr (VW == 4)
+            *reinterpret_cast<uint4*>(vr[i]) = *reinterpret_cast<const uint4*>(vt + C::v_at(r, g + 8 * u));
+          else
+            *reinterpret_cast<uint2*>(vr[i]) = *reinterpret_cast<const uint2*>(vt + C::v_at(r, g >> 1) + 8 * (g & 1));
+        }
 #pragma unroll
-        for (int x = 0; x < VW; ++x) w[i][x] ^= 0x80808080u;
-      }
+        for (int x = 0; x < VW; ++x) {
+          uint32_t w[4];
 #pragma unroll
-      for (int x = 0; x < VW; ++x) {
-        // keys (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 4x .. 4x + 3, two dims a word
-        const uint32_t z[4] = {__byte_perm(w[0][x], w[1][x], 0x5140), __byte_perm(w[2][x], w[3][x], 0x5140),
-                               __byte_perm(w[0][x], w[1][x], 0x7362), __byte_perm(w[2][x], w[3][x], 0x7362)};
+          for (int i = 0; i < 4; ++i) w[i] = vr[i][x] ^ 0x80808080u;
+          // keys (2t, 2t + 1) and (2t + 8, 2t + 9) of dims 4x .. 4x + 3, two dims a word
+          const uint32_t z[4] = {__byte_perm(w[0], w[1], 0x5140), __byte_perm(w[2], w[3], 0x5140),
+                                 __byte_perm(w[0], w[1], 0x7362), __byte_perm(w[2], w[3], 0x7362)};
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          float(&d0)[4] = o[u * 16 + 4 * x + 2 * y];
-          float(&d1)[4] = o[u * 16 + 4 * x + 2 * y + 1];
-          mma_rows<HALF>(d0, pa[0][0], a1, pa[0][1], a3, codes_to_half2<0>(z[2 * y]), codes_to_half2<0>(z[2 * y + 1]));
-          mma_rows<HALF>(d1, pa[0][0], a1, pa[0][1], a3, codes_to_half2<1>(z[2 * y]), codes_to_half2<1>(z[2 * y + 1]));
+          for (int y = 0; y < 2; ++y) {
+            float(&d0)[4] = o[u * 16 + 4 * x + 2 * y];
+            float(&d1)[4] = o[u * 16 + 4 * x + 2 * y + 1];
+            const uint32_t b0 = codes_to_half2<0>(z[2 * y]), b1 = codes_to_half2<0>(z[2 * y + 1]);
+            const uint32_t c0 = codes_to_half2<1>(z[2 * y]), c1 = codes_to_half2<1>(z[2 * y + 1]);
+            if constexpr (HALF) {
+              mma_16816(d0, ph[0][0], pl[0][0], ph[0][1], pl[0][1], b0, b1);
+              mma_16816(d1, ph[0][0], pl[0][0], ph[0][1], pl[0][1], c0, c1);
+            } else {
+              mma_16816(d0, ph[0][0], ph[R - 1][0], ph[0][1], ph[R - 1][1], b0, b1);
+              mma_16816(d1, ph[0][0], ph[R - 1][0], ph[0][1], ph[R - 1][1], c0, c1);
+              mma_16816(d0, pl[0][0], pl[R - 1][0], pl[0][1], pl[R - 1][1], b0, b1);
+              mma_16816(d1, pl[0][0], pl[R - 1][0], pl[0][1], pl[R - 1][1], c0, c1);
+            }
+          }
         }
       }
     }
   }
   cp_async_wait<0>();
+  __syncthreads();  // every warp has left its ring
+  // ---- the CTA's warps: O, m and l of each through shared memory
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (t == 0) warp_ml[warp * 16 + g + 8 * i] = make_float2(m[i], l[i]);
-  }
-  __syncthreads();  // every warp has left its ring
-  float* xo = reinterpret_cast<float*>(rings) + warp * 16 * C::kPad;
-#pragma unroll
-  for (int i = 0; i < R; ++i)
+    if (t == 0) warp_ml[warp * C::kRowsMax + g + 8 * i] = make_float2(m[i], l[i]);
+    float* row = xo + (warp * C::kRowsMax + g + 8 * i) * C::kPad;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int e = 0; e < D / 8; e += 4) {
         constexpr int run = D >= 128 ? 16 : 8;
         const int dim = (e / 16) * 128 + (2 * t + half) * run + e % 16;
-        *reinterpret_cast<float4*>(xo + (g + 8 * i) * C::kPad + dim) =
-            make_float4(o[e][2 * i + half] * vref, o[e + 1][2 * i + half] * vref, o[e + 2][2 * i + half] * vref,
-                        o[e + 3][2 * i + half] * vref);
+        float4 x;
+        float* xs = &x.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          xs[j] = (HALF ? o[e + j][half] + o[e + j][2 + half] : o[e + j][2 * i + half]) * vref;
+        *reinterpret_cast<float4*>(row + dim) = x;
       }
+  }
   __syncthreads();
-  const int rows = min(p.rows, HALF ? 8 : 16);
-  for (int i = threadIdx.x; i < rows * (D / 4); i += C::kThreads) {
+  const int ranks = static_cast<int>(cluster_nctarank());
+  const bool direct = p.splits == 1;          // this CTA has all the keys
+  const bool clustered = !direct && ranks == p.splits;
+  const int items = p.rows * (D / 4);
+  for (int i = threadIdx.x; i < items; i += C::kThreads) {
     const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, warp_ml[w * 16 + r].x);
+    for (int w = 0; w < C::kWarps; ++w) mm = fmaxf(mm, warp_ml[w * C::kRowsMax + r].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < C::kWarps; ++w) {
-      const float2 ml = warp_ml[w * 16 + r];
+      const float2 ml = warp_ml[w * C::kRowsMax + r];
       if (ml.y == 0.f) continue;  // saw nothing (a NaN stays)
       const float f = ex2_approx(ml.x - mm);
-      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<float*>(rings) + (w * 16 + r) * C::kPad + e);
+      const float4 x = *reinterpret_cast<const float4*>(xo + (w * C::kRowsMax + r) * C::kPad + e);
       acc.x = fmaf(x.x, f, acc.x), acc.y = fmaf(x.y, f, acc.y);
       acc.z = fmaf(x.z, f, acc.z), acc.w = fmaf(x.w, f, acc.w);
       sum = fmaf(ml.y, f, sum);
     }
-    if (p.splits > 1) {
+    if (direct) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store4(static_cast<T*>(p.out) + out_row(p, b, h, r) * D + e,
+             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    } else if (clustered) {
+      *reinterpret_cast<float4*>(xo + (C::kWarps * C::kRowsMax + r) * C::kPad + e) = acc;
+      if (e == 0) warp_ml[C::kWarps * C::kRowsMax + r] = make_float2(mm, sum);
+    } else {
       const long long at = (static_cast<long long>(unit) * p.splits + split) * p.rows + r;
       *reinterpret_cast<float4*>(p.part_o + at * D + e) = acc;
       if (e == 0) p.part_ml[at] = make_float2(mm, sum);
-    } else {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int tok = r / p.group, head = h * p.group + r % p.group;
-      T* dst = static_cast<T*>(p.out) + ((static_cast<long long>(b) * p.tokens + tok) * (p.heads * p.group) + head) * D + e;
-      dst[0] = from_float<T>(acc.x * inv), dst[1] = from_float<T>(acc.y * inv);
-      dst[2] = from_float<T>(acc.z * inv), dst[3] = from_float<T>(acc.w * inv);
     }
+  }
+  if (clustered) {
+    // ---- the cluster's CTAs: each finishes its share of the results, reading the others' shared memory
+    cluster_sync();
+    const uint32_t ml0 = smem_addr(warp_ml + C::kWarps * C::kRowsMax), xo0 = smem_addr(xo + C::kWarps * C::kRowsMax * C::kPad);
+    for (int i = split * C::kThreads + threadIdx.x; i < items; i += ranks * C::kThreads) {
+      const int r = i / (D / 4), e = (i - r * (D / 4)) * 4;
+      float2 ml[8];
+      float4 x[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= ranks) break;
+        ml[c] = ld_cluster_v2(mapa_shared(ml0 + r * 8, c));
+        x[c] = ld_cluster_v4(mapa_shared(xo0 + (r * C::kPad + e) * 4, c));
+      }
+      float mm = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        if (c < ranks) mm = fmaxf(mm, ml[c].x);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        if (c >= ranks || ml[c].y == 0.f) continue;
+        const float f = ex2_approx(ml[c].x - mm);
+        acc.x = fmaf(x[c].x, f, acc.x), acc.y = fmaf(x[c].y, f, acc.y);
+        acc.z = fmaf(x[c].z, f, acc.z), acc.w = fmaf(x[c].w, f, acc.w);
+        sum = fmaf(ml[c].y, f, sum);
+      }
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      store4(static_cast<T*>(p.out) + out_row(p, b, h, r) * D + e,
+             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+    }
+    cluster_sync();  // no CTA leaves while another may still read its shared memory
   }
 }
 
@@ -871,47 +992,61 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   }
 }
 
-// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one warp per row.
+// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one CTA of 4 warps
+// per row, each warp every fourth part; the parts' O and (m, l) are loaded
+// together (at most 256 parts: 64 a warp).
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attn8_join_kernel(const __grid_constant__ Attn8Params p, long long units) {
+__global__ void __launch_bounds__(128) attn8_join_kernel(const __grid_constant__ Attn8Params p) {
+  __shared__ float red[4][D];
+  __shared__ float2 red_ml[4];
   pdl_launch_dependents();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long i = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (i >= units * p.rows) return;
-  const long long unit = i / p.rows;
-  const int r = static_cast<int>(i - unit * p.rows);
-  const float2* ml = p.part_ml + unit * p.splits * p.rows + r;
-  float mm = -INFINITY;
-  for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, ml[static_cast<long long>(s) * p.rows].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, o));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x, unit = blockIdx.y;
   constexpr int V = D / 32;  // elements of a lane: 2, 4 or 8
+  const long long first = static_cast<long long>(unit) * p.splits * p.rows + r;
   float acc[V] = {};
-  float sum = 0.f;
+  float m = -INFINITY, sum = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < p.splits; ++s) {
-    const float2 x = ml[static_cast<long long>(s) * p.rows];
-    const float* src = p.part_o + ((unit * p.splits + s) * p.rows + r) * D + lane * V;
-    const float f = x.y == 0.f ? 0.f : ex2_approx(x.x - mm);
-    sum = fmaf(x.y, f, sum);
+  for (int s = warp; s < p.splits; s += 4) {
+    const float2 ml = p.part_ml[first + static_cast<long long>(s) * p.rows];
+    const float* src = p.part_o + (first + static_cast<long long>(s) * p.rows) * D + lane * V;
     float v[V];
     if constexpr (V == 2) *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
     else {
 #pragma unroll
       for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(src + j);
     }
-    if (x.y != 0.f) {
+    if (ml.y == 0.f) continue;  // saw nothing (a NaN stays)
+    const float mn = fmaxf(m, ml.x);
+    const float fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fn = ex2_approx(ml.x - mn);
+    m = mn;
+    sum = sum * fo + ml.y * fn;
 #pragma unroll
-      for (int j = 0; j < V; ++j) acc[j] = fmaf(v[j], f, acc[j]);
-    }
+    for (int j = 0; j < V; ++j) acc[j] = acc[j] * fo + v[j] * fn;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int b = static_cast<int>(unit / p.heads), h = static_cast<int>(unit % p.heads);
-  const int tok = r / p.group, head = h * p.group + r % p.group;
-  T* dst = static_cast<T*>(p.out) + ((static_cast<long long>(b) * p.tokens + tok) * (p.heads * p.group) + head) * D + lane * V;
 #pragma unroll
-  for (int j = 0; j < V; ++j) dst[j] = from_float<T>(acc[j] * inv);
+  for (int j = 0; j < V; ++j) red[warp][lane * V + j] = acc[j];
+  if (lane == 0) red_ml[warp] = make_float2(m, sum);
+  __syncthreads();
+  if (threadIdx.x >= D / 4) return;
+  const int e = threadIdx.x * 4;
+  float mm = -INFINITY, total = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, red_ml[w].x);
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float2 ml = red_ml[w];
+    if (ml.y == 0.f) continue;
+    const float f = ex2_approx(ml.x - mm);
+    x.x = fmaf(red[w][e], f, x.x), x.y = fmaf(red[w][e + 1], f, x.y);
+    x.z = fmaf(red[w][e + 2], f, x.z), x.w = fmaf(red[w][e + 3], f, x.w);
+    total = fmaf(ml.y, f, total);
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  const int b = unit / p.heads, h = unit - b * p.heads;
+  store4(static_cast<T*>(p.out) + out_row(p, b, h, r) * D + e, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
 }  // namespace w4a4

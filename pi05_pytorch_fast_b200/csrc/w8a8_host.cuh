@@ -131,7 +131,7 @@ Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, int sms) {
   plan.tiles = static_cast<int>((rows + 127) / 128);
   const int64_t work = units * (plan.few ? 1 : plan.tiles);
   // keys that make a split worth its part of the join
-  const int64_t most = plan.few ? (capacity + 511) / 512 : (capacity + 255) / 256;
+  const int64_t most = plan.few ? (capacity + 127) / 128 : (capacity + 255) / 256;
   plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, sms / std::max<int64_t>(work, 1), 256})));
   return plan;
 }
@@ -140,22 +140,26 @@ template <typename T, int D>
 int launch_attention8_d(const Attn8Params& p, const Attn8Plan& plan, int64_t units, int dev, int bit,
                         cudaStream_t stream) {
   if (plan.few) {
-    const bool half = p.rows <= 8;
-    const auto kernel = half ? attn8_few_kernel<T, D, true> : attn8_few_kernel<T, D, false>;
-    if (int e = ensure_smem_attr8(dev, bit + (half ? 0 : 1), kernel, Attn8Few<D>::kSmem)) return e;
-    W4A4_CUDA_TRY(launch_kernel(kernel, dim3(p.splits, static_cast<unsigned>(units)), dim3(Attn8Few<D>::kThreads),
-                                Attn8Few<D>::kSmem, stream, 1, p));
+    const auto go = [&](auto half_tag, int nr) {
+      constexpr bool HALF = decltype(half_tag)::value;
+      using C = Attn8Few<D, HALF>;
+      const auto kernel = attn8_few_kernel<T, D, HALF>;
+      if (int e = ensure_smem_attr8(dev, nr, kernel, C::kSmem)) return e;
+      // up to 8 CTAs of a key/value head form a cluster and join their parts themselves
+      W4A4_CUDA_TRY(launch_kernel(kernel, dim3(p.splits, static_cast<unsigned>(units)), dim3(C::kThreads), C::kSmem,
+                                  stream, p.splits <= 8 ? p.splits : 1, p));
+      return static_cast<int>(W4A4_OK);
+    };
+    if (int e = p.rows <= 8 ? go(std::true_type{}, bit) : go(std::false_type{}, bit + 1)) return e;
   } else {
     const auto kernel = attn8_many_kernel<T, D>;
     if (int e = ensure_smem_attr8(dev, bit + 2, kernel, Attn8Many<D>::kSmem)) return e;
     W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.tiles, p.splits, static_cast<unsigned>(units)),
                                 dim3(Attn8Many<D>::kThreads), Attn8Many<D>::kSmem, stream, 1, p));
   }
-  if (p.splits > 1) {
-    const int64_t rows = units * p.rows;
-    W4A4_CUDA_TRY(launch_kernel(attn8_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream, 1, p,
-                                static_cast<long long>(units)));
-  }
+  if (p.splits > (plan.few ? 8 : 1))
+    W4A4_CUDA_TRY(launch_kernel(attn8_join_kernel<T, D>, dim3(static_cast<unsigned>(p.rows), static_cast<unsigned>(units)),
+                                dim3(128), 0, stream, 1, p));
   return ok();
 }
 
