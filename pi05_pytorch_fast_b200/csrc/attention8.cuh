@@ -29,6 +29,11 @@
 
 namespace w4a4 {
 
+// At least 117 KB of shared memory for a CTA with TMEM, so that no two of them
+// share an SM: a CTA of a cluster that waited for columns which another
+// cluster's CTA holds could wait for good, each cluster's other half being
+// blocked by the other.
+constexpr int kOneCtaSmem = 117 * 1024;
 constexpr float kAttn8Grow = 8.f;      // log2 by which a block may exceed m
 constexpr float kAttn8VGrow = 16.f;    // factor by which a value scale may exceed vref
 
@@ -565,9 +570,8 @@ struct Attn8Many {
   static constexpr int kThreads = 13 * 32;
   static constexpr int kNumBars = 17;
   static constexpr int kNeed = kQBytes + 2 * (kKBytes + kVBytes) + kRows * 8 + kNumBars * 8 + 16 + 1024;
-  // two CTAs on an SM only where their TMEM fits beside each other
   static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
-  static constexpr int kSmem = D == 128 ? (kNeed > 118 * 1024 ? kNeed : 118 * 1024) : kNeed;
+  static constexpr int kSmem = kNeed > kOneCtaSmem ? kNeed : kOneCtaSmem;
   static constexpr uint32_t kOCol = 0, kSCol = D, kPCol = D + 128;
 };
 

@@ -201,6 +201,11 @@ Rows tma_rows(Rows r, const char* what) {
   return {t, r.m, ld};
 }
 
+// A vector from a multiple of 16 bytes (copied if it is a view that is not).
+Tensor aligned16(const Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0 ? t : t.clone();
+}
+
 Tensor linear(const Tensor& codes, const Tensor& scale, const Tensor& weight, const Tensor& weight_scale,
               const OptTensor& bias, at::ScalarType dtype) {
   const int32_t dt = dtype_code(dtype, true, "dtype");
@@ -223,9 +228,10 @@ Tensor linear(const Tensor& codes, const Tensor& scale, const Tensor& weight, co
   if (a.m == 0) return y;
   a = tma_rows(a, "codes");
   w = tma_rows(w, "weight");
+  const Tensor sw = aligned16(weight_scale), b = bias.has_value() ? aligned16(*bias) : Tensor();
   check_status(w4a4_gemm8(static_cast<const int8_t*>(a.data()), a.ld, scale.const_data_ptr<float>(),
-                          static_cast<const int8_t*>(w.data()), w.ld, weight_scale.const_data_ptr<float>(),
-                          bias.has_value() ? bias->const_data_ptr() : nullptr, dt, a.m, as_i32(n, "N"), as_i32(k, "K"),
+                          static_cast<const int8_t*>(w.data()), w.ld, sw.const_data_ptr<float>(),
+                          bias.has_value() ? b.const_data_ptr() : nullptr, dt, a.m, as_i32(n, "N"), as_i32(k, "K"),
                           y.data_ptr(), stream_of(codes)));
   return y;
 }

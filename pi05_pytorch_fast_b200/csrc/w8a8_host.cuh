@@ -87,11 +87,76 @@ int check_rows8(int64_t rows, int32_t h, const void* x, int64_t ldx, const int8_
   return W4A4_OK;
 }
 
-int launch_gemm8(const Gemm8Params& p, int32_t dtype, cudaStream_t stream) {
+// How a product runs: on CTA pairs, or in tiles of 128 channels x tok_tile
+// tokens whose K is split over clusters of `split` CTAs.
+struct Gemm8Plan {
+  bool pair;
+  int tok_tile, split, stages;
+  int n_tok_tiles, n_w_tiles;
+};
+Gemm8Plan gemm8_plan(int64_t m, int n, int k, int sms) {
+  Gemm8Plan plan{};
+  const int k_steps = (k + 127) / 128;
+  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  plan.pair = m > 256 && pair_tiles >= sms / 4;
+  if (plan.pair) {
+    plan.n_tok_tiles = static_cast<int>((m + 255) / 256);
+    plan.n_w_tiles = (n + 255) / 256;
+    return plan;
+  }
+  const int64_t tiles = (m + 127) / 128;
+  plan.tok_tile = static_cast<int>(((m + tiles - 1) / tiles + 15) / 16 * 16);
+  plan.n_tok_tiles = static_cast<int>((m + plan.tok_tile - 1) / plan.tok_tile);
+  plan.n_w_tiles = (n + 127) / 128;
+  const int64_t work = static_cast<int64_t>(plan.n_tok_tiles) * plan.n_w_tiles;
+  plan.split = 1;
+  while (plan.split < 8 && work * plan.split * 2 <= sms + sms / 8 && k_steps >= 4 * plan.split) plan.split *= 2;
+  const int steps = (k_steps + plan.split - 1) / plan.split;
+  const int step_bytes = kG8ABytes + plan.tok_tile * kG8StepBytes;
+  plan.stages = std::max(1, std::min({steps, kG8MaxStages, 200 * 1024 / step_bytes}));
+  return plan;
+}
+
+// Tiled map of int8 rows {k, rows} with boxes of 128 bytes x `box` rows,
+// 128-byte swizzle, zeros outside.  Encoded for each call.
+int gemm8_map(CUtensorMap* out, const int8_t* ptr, int k, int64_t rows, int64_t ld, int box) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(ld)};
+  const cuuint32_t boxes[2] = {128, static_cast<cuuint32_t>(box)}, estr[2] = {1, 1};
+  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(ptr), dims, strides, boxes, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? W4A4_OK
+                           : fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for int8 [%lld, %d], row stride %lld",
+                                  static_cast<int>(r), (long long)rows, k, (long long)ld);
+}
+
+int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
+                 const void* bias, int32_t dtype, int64_t m, int32_t n, int32_t k, void* y, cudaStream_t stream) {
+  int dev, sms;
+  if (int e = current_device(&dev)) return e;
+  if (int e = sm_count(dev, &sms)) return e;
+  const Gemm8Plan plan = gemm8_plan(m, n, k, sms);
+  Gemm8Params p;
+  if (int e = gemm8_map(&p.tmap_a, a, k, m, lda, plan.pair ? 128 : plan.tok_tile)) return e;
+  if (int e = gemm8_map(&p.tmap_w, w, k, n, ldw, 128)) return e;
+  p.sa = sa, p.sw = sw, p.bias = bias, p.y = y, p.m = m, p.n = n;
+  p.k_steps = (k + 127) / 128, p.tok_tile = plan.tok_tile, p.stages = plan.stages;
+  p.n_tok_tiles = plan.n_tok_tiles, p.n_w_tiles = plan.n_w_tiles, p.wait_limit_ns = g_wait_limit_ns.load();
   return by_dtype(dtype, true, "gemm8", [&](auto tag) {
     using T = decltype(tag);
-    const dim3 grid((p.n + 31) / 32, static_cast<unsigned>((p.m + 31) / 32));
-    return cuda_status(launch_kernel(gemm8_simple_kernel<T>, grid, dim3(256), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+    const int bit = 24 + 2 * (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 1 : 2);
+    if (plan.pair) {
+      if (int e = ensure_smem_attr8(dev, bit, gemm8_pair_kernel<T>, kG8PairSmem)) return e;
+      const int pairs = std::min(sms / 2, plan.n_tok_tiles * plan.n_w_tiles);
+      W4A4_CUDA_TRY(launch_kernel(gemm8_pair_kernel<T>, dim3(2 * pairs), dim3(kG8PairThreads), kG8PairSmem, stream, 2, p));
+    } else {
+      if (int e = ensure_smem_attr8(dev, bit + 1, gemm8_tile_kernel<T>, kSmemLimit)) return e;
+      W4A4_CUDA_TRY(launch_kernel(gemm8_tile_kernel<T>, dim3(plan.split * plan.n_tok_tiles * plan.n_w_tiles),
+                                  dim3(kG8TileThreads), gemm8_tile_smem(plan.tok_tile, plan.stages), stream, plan.split, p));
+    }
+    return ok();
   });
 }
 
@@ -238,14 +303,16 @@ int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, i
   if (m < 0 || n <= 0 || k <= 0)
     return fail(W4A4_ERR_INVALID, "gemm8: invalid shape M=%lld N=%d K=%d", (long long)m, n, k);
   if (k >= 131072) return fail(W4A4_ERR_UNSUPPORTED, "gemm8: K must be below 131072 for exact int32 sums, got %d", k);
-  if (m > 65535LL * 32) return fail(W4A4_ERR_UNSUPPORTED, "gemm8: too many rows: %lld", (long long)m);
+  if (m > 0x7fffff00LL) return fail(W4A4_ERR_UNSUPPORTED, "gemm8: too many rows: %lld", (long long)m);
   if (m == 0) return ok();
   if (!a || !sa || !w || !sw || !y) return fail(W4A4_ERR_INVALID, "gemm8: null pointer argument");
   if (lda < k || ldw < k) return fail(W4A4_ERR_INVALID, "gemm8: row stride below K = %d", k);
   if (!rows_aligned(a, lda, 1, 16) || !rows_aligned(w, ldw, 1, 16))
     return fail(W4A4_ERR_INVALID, "gemm8: rows of codes must begin at multiples of 16 bytes");
-  Gemm8Params p{a, w, sa, sw, bias, y, lda, ldw, m, n, k};
-  return launch_gemm8(p, dtype, static_cast<cudaStream_t>(stream));
+  if (!aligned(sw, 16)) return fail(W4A4_ERR_INVALID, "gemm8: channel scales must be 16-byte aligned");
+  if (!aligned(y, 32) || (bias && !aligned(bias, 16)))
+    return fail(W4A4_ERR_INVALID, "gemm8: y must be 32-byte and bias 16-byte aligned");
+  return launch_gemm8(a, lda, sa, w, ldw, sw, bias, dtype, m, n, k, y, static_cast<cudaStream_t>(stream));
 }
 
 int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, const int64_t* cache_stride,
