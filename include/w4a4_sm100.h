@@ -364,8 +364,8 @@ int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t 
 
 /* y[m, n] = (sum_k a[m, k] w[n, k]) sa[m] sw[n] + bias[n]: a int8 [m, k] and w
  * int8 [n, k], rows at multiples of 16 bytes (k itself arbitrary, below
- * 131072); y [m, n] contiguous (32-byte aligned) and bias (or NULL) of type
- * dtype; sw and bias 16-byte aligned. */
+ * 131072); y [m, n] contiguous and bias (or NULL) of type
+ * dtype; y, sw and bias 16-byte aligned. */
 int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
                const void* bias, int32_t dtype, int64_t m, int32_t n, int32_t k, void* y, void* stream);
 

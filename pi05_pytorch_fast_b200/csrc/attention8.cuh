@@ -175,7 +175,9 @@ __device__ __forceinline__ uint32_t cluster_nctarank() {
 // 4 consecutive results, rounded once.
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, const float4& v) {
-  if constexpr (std::is_same_v<T, __half>) {
+  if constexpr (std::is_same_v<T, float>) {
+    *reinterpret_cast<float4*>(dst) = v;
+  } else if constexpr (std::is_same_v<T, __half>) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_half2_bits(v.x, v.y), pack_half2_bits(v.z, v.w));
   } else {
     const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);

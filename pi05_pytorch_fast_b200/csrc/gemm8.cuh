@@ -6,11 +6,11 @@
 // to the output's type.  K is walked in steps of 128 bytes (one 128-byte
 // swizzle row); TMA fills what lies past K, M or N with zeros.
 //
+//  * gemm8_few_kernel: up to 16 tokens, without TMEM or TMA (see there).
 //  * gemm8_tile_kernel: one tile of 128 channels x T tokens (T <= 256, a
 //    multiple of 16) for each cluster of up to 8 CTAs, which split K between
 //    them and add their sums through distributed shared memory.  Channels are
-//    the MMA's M side, so that few tokens cost few columns.  For one token up
-//    to some hundred it is bound by the weights' way from HBM, or by latency.
+//    the MMA's M side, so that few tokens cost few columns.
 //  * gemm8_pair_kernel: persistent CTA pairs (cta_group::2), tiles of 256
 //    tokens x 256 channels, the accumulators double buffered so that a tile's
 //    epilogue runs under the next one's products.  Bound by the tensor pipe.
@@ -24,6 +24,7 @@ namespace w4a4 {
 struct alignas(64) Gemm8Params {
   CUtensorMap tmap_a;  // tokens: int8 {k, m}, box {128, T or 128}, SW128
   CUtensorMap tmap_w;  // weights: int8 {k, n}, box {128, 128}, SW128
+  CUtensorMap tmap_y;  // output {n, m}, box {64 bytes, 32}, SW64 (pair kernel, tma_store)
   const float* sa;
   const float* sw;
   const void* bias;    // output type, or NULL
@@ -34,6 +35,7 @@ struct alignas(64) Gemm8Params {
   int tok_tile;        // T (tile kernel)
   int stages;
   int n_tok_tiles, n_w_tiles;
+  int tma_store;       // rows of y begin at multiples of 16 bytes
   unsigned long long wait_limit_ns;
 };
 
@@ -41,39 +43,35 @@ constexpr int kG8StepBytes = 128;             // K bytes of a step
 constexpr int kG8ABytes = 128 * kG8StepBytes;  // 16 KB of weights (or tokens) of a step
 constexpr int kG8MaxStages = 12;
 
-// (sum of products) -> y: eight consecutive channels of one token.
+// Scales and biases of four consecutive channels from n on (zero past N).
 template <typename T>
-__device__ __forceinline__ void g8_store8(const Gemm8Params& p, long long m, int n, const int (&acc)[8], float sa) {
-  float v[8];
-  T* dst = static_cast<T*>(p.y) + m * p.n + n;
-  if (n + 8 <= p.n && p.n % 8 == 0) {
-    float w[8];
-    load8(p.sw + n, w);
+struct G8Channels {
+  float w[4], b[4];
+  bool vec;  // the four exist, and rows of y keep vectors of four aligned
+  __device__ __forceinline__ G8Channels(const Gemm8Params& p, int n) : vec(n + 4 <= p.n && p.n % 4 == 0) {
+    const T* bias = static_cast<const T*>(p.bias);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = static_cast<float>(acc[i]) * sa * w[i];
-    if (p.bias) {
-      float b[8];
-      load8(static_cast<const T*>(p.bias) + n, b);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += b[i];
+    for (int i = 0; i < 4; ++i) {
+      w[i] = n + i < p.n ? __ldg(p.sw + n + i) : 0.f;
+      b[i] = bias && n + i < p.n ? to_float(bias[n + i]) : 0.f;
     }
-    store8(dst, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n + i < p.n) {
-        float x = static_cast<float>(acc[i]) * sa * __ldg(p.sw + n + i);
-        if (p.bias) x += to_float(static_cast<const T*>(p.bias)[n + i]);
-        dst[i] = from_float<T>(x);
-      }
   }
-}
+  // sums of one token -> y
+  __device__ __forceinline__ void store(const Gemm8Params& p, long long m, int n, const int4& acc, float sa) const {
+    const float4 v = make_float4(fmaf(static_cast<float>(acc.x) * sa, w[0], b[0]), fmaf(static_cast<float>(acc.y) * sa, w[1], b[1]),
+                                 fmaf(static_cast<float>(acc.z) * sa, w[2], b[2]), fmaf(static_cast<float>(acc.w) * sa, w[3], b[3]));
+    T* dst = static_cast<T*>(p.y) + m * p.n + n;
+    if (vec) {
+      store4(dst, v);
+    } else {
+      const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < p.n) dst[i] = from_float<T>(x[i]);
+    }
+  }
+};
 
-__device__ __forceinline__ int4 ld_cluster_i4(uint32_t addr) {
-  int4 v;
-  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t cluster_size() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
@@ -81,14 +79,16 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 
 // Shared memory: the ring of `stages` (16 KB of weights, T rows of tokens),
-// which the sums [T][128] take over once the products are done; barriers.
+// which the sums [T][128] and what the other CTAs of the cluster send take
+// over once the products are done; token scales; barriers.
 constexpr int kG8TileThreads = 256;
+constexpr int kG8TileMax = 256;  // tokens
 __host__ __device__ constexpr int gemm8_tile_ring(int tok_tile, int stages) {
-  const int ring = stages * (kG8ABytes + tok_tile * kG8StepBytes), sums = tok_tile * 512;
+  const int ring = stages * (kG8ABytes + tok_tile * kG8StepBytes), sums = 2 * tok_tile * 512;
   return ring > sums ? ring : sums;
 }
 __host__ __device__ constexpr int gemm8_tile_smem(int tok_tile, int stages) {
-  const int need = gemm8_tile_ring(tok_tile, stages) + (2 * kG8MaxStages + 1) * 8 + 16 + 1024;
+  const int need = gemm8_tile_ring(tok_tile, stages) + kG8TileMax * 4 + (2 * kG8MaxStages + 2) * 8 + 16 + 1024;
   return need > kOneCtaSmem ? need : kOneCtaSmem;
 }
 
@@ -102,12 +102,13 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
   uint8_t* w_ring = base;                    // [S][16 KB]
   uint8_t* t_ring = base + S * kG8ABytes;    // [S][T x 128]
   int* sums = reinterpret_cast<int*>(base);  // [T][128], after the products
-  uint64_t* bars = reinterpret_cast<uint64_t*>(base + gemm8_tile_ring(p.tok_tile, S));
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kG8MaxStages + 1);
+  float* tok_scale = reinterpret_cast<float*>(base + gemm8_tile_ring(p.tok_tile, S));  // [256]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(tok_scale + kG8TileMax);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kG8MaxStages + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const auto bar_full = [&](int s) { return smem_addr(bars + s); };
   const auto bar_empty = [&](int s) { return smem_addr(bars + kG8MaxStages + s); };
-  const uint32_t bar_acc = smem_addr(bars + 2 * kG8MaxStages);
+  const uint32_t bar_acc = smem_addr(bars + 2 * kG8MaxStages), bar_recv = smem_addr(bars + 2 * kG8MaxStages + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / ranks;
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
       mbar_init(bar_empty(s), 1);
     }
     mbar_init(bar_acc, 1);
+    mbar_init(bar_recv, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&p.tmap_a);
@@ -185,48 +187,69 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
     if (issuer) umma_commit(bar_acc);
     __syncwarp();
   }
+  // scales and biases for the results below, under the products
+  const G8Channels<T> channels(p, n0 + 4 * lane);  // a lane's four channels of the tile
+  if (threadIdx.x < p.tok_tile) tok_scale[threadIdx.x] = m0 + threadIdx.x < p.m ? __ldg(p.sa + m0 + threadIdx.x) : 0.f;
   volatile int no_abort = 0;
   mbar_wait_bounded(bar_acc, 0, &no_abort, err, kErrWaitAccum, limit);
   tc_fence_after();
   __syncthreads();  // the producer has seen its copies land: the ring is free
   // ---- sums to shared memory: lane = channel, so a column's 128 are one line
-  const bool aborted = *abort_flag != 0;
+  const int share = p.tok_tile / ranks;  // tokens that each CTA of the cluster finishes
   {
     const int quarter = warp & 3;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
-    for (int c = (warp >> 2) * 16; c < p.tok_tile; c += 32) {
-      uint32_t r[16];
-      if (steps > 0) {
-        tmem_ld_32x32b_x16(tmem_base + lane_addr + c, r);
-        tmem_ld_wait();
-      } else {
+    for (int c0 = (warp >> 2) * 16; c0 < p.tok_tile; c0 += 64) {
+      uint32_t r[2][16];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = 0u;
+      for (int i = 0; i < 2; ++i) {
+        if (steps > 0 && c0 + 32 * i < p.tok_tile) {
+          tmem_ld_32x32b_x16(tmem_base + lane_addr + c0 + 32 * i, r[i]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[i][j] = 0u;
+        }
       }
+      tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + quarter * 32 + lane] = static_cast<int>(r[j]);
+      for (int i = 0; i < 2; ++i)
+        if (c0 + 32 * i < p.tok_tile)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) sums[(c0 + 32 * i + j) * 128 + quarter * 32 + lane] = static_cast<int>(r[i][j]);
     }
   }
   tc_fence_before();
-  if (ranks > 1) cluster_sync();
-  else __syncthreads();
-  // ---- the cluster's CTAs finish a share of the tile each
-  const uint32_t sums0 = smem_addr(sums);
-  for (int i = rank * kG8TileThreads + threadIdx.x; i < p.tok_tile * 16; i += ranks * kG8TileThreads) {
-    const int t = i >> 4, c = (i & 15) * 8;
-    const long long m = m0 + t;
-    const int n = n0 + c;
-    if (m >= p.m || n >= p.n) continue;
-    int acc[8] = {};
-    for (int r = 0; r < ranks; ++r) {
-      const uint32_t at = ranks > 1 ? mapa_shared(sums0 + (t * 128 + c) * 4, r) : sums0 + (t * 128 + c) * 4;
-      const int4 x = ld_cluster_i4(at), y = ld_cluster_i4(at + 16);
-      acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
-      acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
-    }
-    if (!aborted) g8_store8<T>(p, m, n, acc, __ldg(p.sa + m));
+  const int first = rank * share;
+  int* recv = sums + p.tok_tile * 128;  // [ranks - 1][share][128]
+  if (ranks > 1) {
+    // ---- every CTA sends each other one its share of the sums, one bulk copy
+    // each (remote loads move an eighth of what these do)
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(bar_recv, static_cast<uint32_t>((ranks - 1) * share * 512));
+    fence_proxy_async_smem();
+    cluster_sync();  // sums written, barriers armed, rings free in all of them
+    if (warp == 0 && lane < ranks && lane != rank)
+      bulk_copy_s2cluster(mapa_shared(smem_addr(recv + (rank < lane ? rank : rank - 1) * share * 128), lane),
+                          smem_addr(sums + lane * share * 128), static_cast<uint32_t>(share * 512),
+                          mapa_shared(bar_recv, lane));
+    __syncwarp();
+    mbar_wait_bounded_cl(bar_recv, 0, &no_abort, err, kErrWaitAccum, limit);
+  } else {
+    __syncthreads();
   }
-  if (ranks > 1) cluster_sync();  // no CTA leaves while another may still read its sums
+  const bool aborted = *abort_flag != 0;
+  const int4* own = reinterpret_cast<const int4*>(sums + first * 128) + lane;
+  const int4* others = reinterpret_cast<const int4*>(recv) + lane;
+#pragma unroll 4
+  for (int t = warp; t < share; t += 8) {
+    int4 acc = own[t * 32];
+    for (int r = 0; r + 1 < ranks; ++r) {
+      const int4 x = others[(r * share + t) * 32];
+      acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    }
+    const long long m = m0 + first + t;
+    if (!aborted && m < p.m && n0 + 4 * lane < p.n) channels.store(p, m, n0 + 4 * lane, acc, tok_scale[first + t]);
+  }
+  if (ranks > 1) cluster_sync();  // no CTA leaves before its copies have been received
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
@@ -234,47 +257,136 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
   }
 }
 
+// -------------------------------------------------------- few tokens (<= 16)
+// One CTA of 8 warps per 8 NT channels; the warps share K in runs of 64 bytes
+// and add their sums through shared memory.  mma.sync m16n8k32: the 16 rows are
+// the tokens, the 8 columns weight rows; as K may be permuted when both
+// operands agree, lane (g, t) loads 16 consecutive bytes of row g at 64 c + 16 t
+// of both straight from global memory, two steps of MMA, with no set-up before
+// the first weight is asked for.  Bound: the weights' way from HBM, and for a
+// small product the launch and one trip to memory.
+constexpr int kG8FewTokens = 16;
+
+__device__ __forceinline__ void mma_s8_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                             uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct Gemm8FewParams {
+  const int8_t* a;
+  const int8_t* w;
+  const float* sa;
+  const float* sw;
+  const void* bias;
+  void* y;
+  long long lda, ldw;
+  int m, n, k;
+};
+
+// 16 bytes of a row of k bytes at byte e, zeros past k (rows begin at multiples of 16 bytes and the
+// last vector of a row that ends inside it is still within the row's stride).
+__device__ __forceinline__ uint4 g8_load_tail(const int8_t* row, int e, int k) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (e < k) {
+    v = __ldg(reinterpret_cast<const uint4*>(row + e));
+    uint32_t* w = &v.x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int bytes = k - e - 4 * i;
+      if (bytes <= 0) w[i] = 0u;
+      else if (bytes < 4) w[i] &= (1u << (8 * bytes)) - 1u;
+    }
+  }
+  return v;
+}
+
+template <typename T, bool HALF, int NT>
+__global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ Gemm8FewParams p) {
+  constexpr int R = HALF ? 8 : 16;
+  __shared__ int part[8][R][8 * NT];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 8 * NT;
+  int acc[NT][4] = {};
+  // rows that do not exist read the last one: their sums are not used
+  const int8_t* a0 = p.a + min(g, p.m - 1) * p.lda + 16 * t;
+  const int8_t* a1 = p.a + min(g + 8, p.m - 1) * p.lda + 16 * t;
+  const int8_t* w[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) w[i] = p.w + static_cast<long long>(min(n0 + 8 * i + g, p.n - 1)) * p.ldw + 16 * t;
+  const int full = p.k / 64;  // runs of 64 bytes: warp, warp + 8, ...
+  const auto product = [&](const uint4& x0, const uint4& x1, const uint4 (&b)[NT]) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      mma_s8_16832(acc[i], x0.x, x1.x, x0.y, x1.y, b[i].x, b[i].y);
+      mma_s8_16832(acc[i], x0.z, x1.z, x0.w, x1.w, b[i].z, b[i].w);
+    }
+  };
+  constexpr int U = 4;  // runs whose loads are under way together
+  int c = warp;
+  for (; c + 8 * (U - 1) < full; c += 8 * U) {
+    uint4 x0[U], x1[U], b[U][NT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = 64 * (c + 8 * u);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) b[u][i] = __ldg(reinterpret_cast<const uint4*>(w[i] + e));
+      x0[u] = __ldg(reinterpret_cast<const uint4*>(a0 + e));
+      x1[u] = HALF ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>(a1 + e));
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) product(x0[u], x1[u], b[u]);
+  }
+  for (; 64 * c < p.k; c += 8) {
+    const int e = 64 * c;
+    uint4 b[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) b[i] = g8_load_tail(w[i], e, p.k - 16 * t);
+    const uint4 x0 = g8_load_tail(a0, e, p.k - 16 * t);
+    const uint4 x1 = HALF ? make_uint4(0u, 0u, 0u, 0u) : g8_load_tail(a1, e, p.k - 16 * t);
+    product(x0, x1, b);
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    *reinterpret_cast<int2*>(&part[warp][g][8 * i + 2 * t]) = make_int2(acc[i][0], acc[i][1]);
+    if constexpr (!HALF) *reinterpret_cast<int2*>(&part[warp][g + 8][8 * i + 2 * t]) = make_int2(acc[i][2], acc[i][3]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < R * 8 * NT; i += 256) {
+    const int r = i / (8 * NT), n = n0 + i % (8 * NT);
+    if (r >= p.m || n >= p.n) continue;
+    int sum = 0;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) sum += part[x][r][i % (8 * NT)];
+    const float b = p.bias ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+    static_cast<T*>(p.y)[static_cast<long long>(r) * p.n + n] =
+        from_float<T>(fmaf(static_cast<float>(sum) * __ldg(p.sa + r), __ldg(p.sw + n), b));
+  }
+}
+
 // ---------------------------------------------------------------- CTA pairs
 // Tiles of 256 tokens (128 in each CTA: the MMA's M side) x 256 channels (128
 // weight rows in each CTA's shared memory).  Warp 0 loads, warp 1 of the
-// leader issues, warps 2-9 are the epilogue: thread = token row, so a thread
-// turns runs of 16 channels into 32-byte stores without shared memory (whose
-// bandwidth the products and the copies share).
-constexpr int kG8PairStages = 6;
+// leader issues, warps 2-9 are the epilogue: thread = token row, a warp takes
+// 32 tokens x 128 channels in boxes of 64 bytes a row, which TMA stores carry
+// off while the next box is converted.  The next tile's scales are loaded under
+// this tile's epilogue.
+constexpr int kG8PairStages = 5;
 constexpr int kG8PairWarps = 10;
 constexpr int kG8PairThreads = 32 * kG8PairWarps;
-constexpr int kG8PairSmem = kG8PairStages * 2 * kG8ABytes + 8 * 2 * 128 * 4 + (2 * kG8PairStages + 5) * 8 + 16 + 1024;
+constexpr int kG8PairSmem = kG8PairStages * 2 * kG8ABytes + 8 * 4096 + 8 * 2 * 128 * 4 + (2 * kG8PairStages + 5) * 8 + 16 + 1024;
 
-// 32 bytes: 16 values of 2 bytes, or 8 of 4.
-__device__ __forceinline__ void st_global_v8(void* p, const uint32_t (&r)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(src), "r"(x), "r"(y)
                : "memory");
 }
-__device__ __forceinline__ void g8_store16(__half* dst, const float (&v)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = pack_half2_bits(v[2 * i], v[2 * i + 1]);
-  st_global_v8(dst, r);
-}
-__device__ __forceinline__ void g8_store16(__nv_bfloat16* dst, const float (&v)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-    r[i] = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  st_global_v8(dst, r);
-}
-__device__ __forceinline__ void g8_store16(float* dst, const float (&v)[16]) {
-  uint32_t r[8];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = __float_as_uint(v[8 * h + i]);
-    st_global_v8(dst + 8 * h, r);
-  }
-}
+// Waits until at most one committed bulk group of this thread has yet to read its source.
+__device__ __forceinline__ void bulk_wait_group_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 
 template <typename T>
 __global__ void __launch_bounds__(kG8PairThreads, 1) gemm8_pair_kernel(const __grid_constant__ Gemm8Params p) {
@@ -283,7 +395,8 @@ __global__ void __launch_bounds__(kG8PairThreads, 1) gemm8_pair_kernel(const __g
   constexpr int S = kG8PairStages;
   uint8_t* t_ring = base;                        // [S][128 tokens x 128]
   uint8_t* w_ring = base + S * kG8ABytes;        // [S][128 weight rows x 128]
-  float* chan = reinterpret_cast<float*>(base + 2 * S * kG8ABytes);  // [epilogue warp][scale, bias][128 channels]
+  uint8_t* out_stage = base + 2 * S * kG8ABytes;  // [epilogue warp][2][32 rows][64 B], 64-byte swizzle
+  float* chan = reinterpret_cast<float*>(out_stage + 8 * 4096);  // [epilogue warp][scale, bias][128 channels]
   uint64_t* bars = reinterpret_cast<uint64_t*>(chan + 8 * 2 * 128);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -413,66 +526,98 @@ __global__ void __launch_bounds__(kG8PairThreads, 1) gemm8_pair_kernel(const __g
   } else {
     // ------------------------------------------------ epilogue (warps 2-9, both CTAs)
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const int row = quarter * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     float* sc = chan + (warp - 2) * 256;
-    const bool wide = p.n % 16 == 0;
+    uint8_t* stage = out_stage + (warp - 2) * 4096;
+    constexpr int W = 64 / sizeof(T);   // columns of a box: 32, or 16 of fp32
+    constexpr int V = 16 / sizeof(T);   // of a 16-byte chunk
+    constexpr int NC = 128 / W;
+    // scales and biases of a tile: lane's four channels (32 apart) and its token
+    float cs[4], cb[4], sa = 0.f;
+    const auto load_scales = [&](int tile) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = tile_n(tile) + half * 128 + 32 * j + lane;
+        cs[j] = n < p.n ? __ldg(p.sw + n) : 0.f;
+        cb[j] = p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+      }
+      const long long m = tile_m(tile) + quarter * 32 + lane;
+      sa = m < p.m ? __ldg(p.sa + m) : 0.f;
+    };
+    if (pair < total) load_scales(pair);
     int count = 0;
     for (int tile = pair; tile < total; tile += n_pairs, ++count) {
-      const int buf = count & 1, n0 = tile_n(tile);
-      const long long m = tile_m(tile) + row;
-      // scales and biases of this warp's four runs of 32 channels, before the sums are ready
+      const int buf = count & 1, n0 = tile_n(tile) + half * 128;  // the warp's 128 channels
+      const long long m0 = tile_m(tile) + quarter * 32;           // and 32 tokens
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int n = n0 + (2 * j + half) * 32 + lane;
-        sc[32 * j + lane] = n < p.n ? __ldg(p.sw + n) : 0.f;
-        sc[128 + 32 * j + lane] = p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+        sc[32 * j + lane] = cs[j];
+        sc[128 + 32 * j + lane] = cb[j];
       }
-      const float sa = m < p.m ? __ldg(p.sa + m) : 0.f;
+      const float sat = sa;
       __syncwarp();
+      if (tile + n_pairs < total) load_scales(tile + n_pairs);
       if (!warp_all(mbar_wait_bounded_cl(bar_accfull(buf), (count >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) break;
       tc_fence_after();
-      T* dst = static_cast<T*>(p.y) + m * p.n + n0;
-      const uint32_t acc = tmem_base + lane_addr + buf * 256;
+      const uint32_t acc = tmem_base + lane_addr + buf * 256 + half * 128;
+      uint32_t r[2][W];
+      const auto load_acc = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // 32 columns at a time, alternately by the two warps of a quarter
-        const int c = (2 * j + half) * 32;
-        uint32_t r[32];
-        tmem_ld_32x32b_x16(acc + c, *reinterpret_cast<uint32_t(*)[16]>(&r[0]));
-        tmem_ld_32x32b_x16(acc + c + 16, *reinterpret_cast<uint32_t(*)[16]>(&r[16]));
+        for (int c = 0; c < W; c += 16)
+          tmem_ld_32x32b_x16(acc + i * W + c, *reinterpret_cast<uint32_t(*)[16]>(&r[i & 1][c]));
+      };
+      load_acc(0);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
         tmem_ld_wait();
-        if (j == 3) {
+        if (i + 1 < NC) {
+          load_acc(i + 1);
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_remote(mapa_shared(bar_accempty(buf), 0));
         }
-        if (m >= p.m) continue;
+        uint8_t* box = stage + (i & 1) * 2048;
+        bulk_wait_group_read1();  // (lane 0) the store of the box before last has read it
+        __syncwarp();
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int n = n0 + c + 16 * q;
-          if (n >= p.n) continue;
-          float v[16];
+        for (int x = 0; x < W; x += V) {
+          float v[V];
 #pragma unroll
-          for (int x = 0; x < 16; x += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(sc + 32 * j + 16 * q + x);
-            const float4 b = *reinterpret_cast<const float4*>(sc + 128 + 32 * j + 16 * q + x);
-            v[x] = fmaf(static_cast<float>(static_cast<int>(r[16 * q + x])) * sa, w.x, b.x);
-            v[x + 1] = fmaf(static_cast<float>(static_cast<int>(r[16 * q + x + 1])) * sa, w.y, b.y);
-            v[x + 2] = fmaf(static_cast<float>(static_cast<int>(r[16 * q + x + 2])) * sa, w.z, b.z);
-            v[x + 3] = fmaf(static_cast<float>(static_cast<int>(r[16 * q + x + 3])) * sa, w.w, b.w);
+          for (int y = 0; y < V; y += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(sc + i * W + x + y);
+            const float4 b = *reinterpret_cast<const float4*>(sc + 128 + i * W + x + y);
+            const uint32_t* q = &r[i & 1][x + y];
+            v[y] = fmaf(static_cast<float>(static_cast<int>(q[0])) * sat, w.x, b.x);
+            v[y + 1] = fmaf(static_cast<float>(static_cast<int>(q[1])) * sat, w.y, b.y);
+            v[y + 2] = fmaf(static_cast<float>(static_cast<int>(q[2])) * sat, w.z, b.z);
+            v[y + 3] = fmaf(static_cast<float>(static_cast<int>(q[3])) * sat, w.w, b.w);
           }
-          if (wide) {
-            g8_store16(dst + c + 16 * q, v);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 16; ++x)
-              if (n + x < p.n) dst[c + 16 * q + x] = from_float<T>(v[x]);
+          T* dst = reinterpret_cast<T*>(box + lane * 64 + (((x / V) ^ ((lane >> 1) & 3)) << 4));
+          if constexpr (V == 8) store8(dst, v);
+          else *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        const int n = n0 + i * W;
+        if (p.tma_store) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (n < p.n && m0 < p.m) tma_store_2d(&p.tmap_y, smem_addr(box), n, static_cast<int>(m0));
+            bulk_commit_group();
           }
+        } else {
+          // rows that do not begin at multiples of 16 bytes: a row of the box at a time
+          __syncwarp();
+          for (int q = 0; q < 32; ++q)
+            if (m0 + q < p.m && lane < W && n + lane < p.n)
+              static_cast<T*>(p.y)[(m0 + q) * p.n + n + lane] = *reinterpret_cast<const T*>(
+                  box + q * 64 + (((lane / V) ^ ((q >> 1) & 3)) << 4) + (lane % V) * sizeof(T));
+          __syncwarp();
         }
       }
     }
+    bulk_wait_group0();  // the stores have been performed
   }
   // ---- both CTAs are done (remote arrivals and products too) before the pair frees its TMEM
   tc_fence_before();

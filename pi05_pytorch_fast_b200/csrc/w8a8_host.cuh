@@ -117,19 +117,23 @@ Gemm8Plan gemm8_plan(int64_t m, int n, int k, int sms) {
   return plan;
 }
 
-// Tiled map of int8 rows {k, rows} with boxes of 128 bytes x `box` rows,
-// 128-byte swizzle, zeros outside.  Encoded for each call.
-int gemm8_map(CUtensorMap* out, const int8_t* ptr, int k, int64_t rows, int64_t ld, int box) {
+// Tiled map of rows of `k` elements of `size` bytes with boxes of bx elements x
+// by rows, zeros outside.  Encoded for each call.
+int gemm8_map(CUtensorMap* out, const void* ptr, CUtensorMapDataType type, int64_t k, int64_t rows, int64_t stride_bytes,
+              int bx, int by, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)}, strides[1] = {static_cast<cuuint64_t>(ld)};
-  const cuuint32_t boxes[2] = {128, static_cast<cuuint32_t>(box)}, estr[2] = {1, 1};
-  const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(ptr), dims, strides, boxes, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
+  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(bx), static_cast<cuuint32_t>(by)}, estr[2] = {1, 1};
+  const CUresult r = fn(out, type, 2, const_cast<void*>(ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? W4A4_OK
-                           : fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for int8 [%lld, %d], row stride %lld",
-                                  static_cast<int>(r), (long long)rows, k, (long long)ld);
+                           : fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%lld, %lld], row stride %lld bytes",
+                                  static_cast<int>(r), (long long)rows, (long long)k, (long long)stride_bytes);
+}
+int gemm8_codes_map(CUtensorMap* out, const int8_t* ptr, int k, int64_t rows, int64_t ld, int box) {
+  return gemm8_map(out, ptr, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, rows, ld, 128, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
@@ -137,10 +141,22 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
   int dev, sms;
   if (int e = current_device(&dev)) return e;
   if (int e = sm_count(dev, &sms)) return e;
+  if (m <= kG8FewTokens) {
+    const Gemm8FewParams f{a, w, sa, sw, bias, y, lda, ldw, static_cast<int>(m), n, k};
+    return by_dtype(dtype, true, "gemm8", [&](auto tag) {
+      using T = decltype(tag);
+      const bool wide = n >= 32 * sms;  // enough CTAs with 16 channels each: half the reads of the tokens
+      const auto kernel = m <= 8 ? (wide ? gemm8_few_kernel<T, true, 2> : gemm8_few_kernel<T, true, 1>)
+                                 : (wide ? gemm8_few_kernel<T, false, 2> : gemm8_few_kernel<T, false, 1>);
+      const int per = wide ? 16 : 8;
+      W4A4_CUDA_TRY(launch_kernel(kernel, dim3((n + per - 1) / per), dim3(256), 0, stream, 1, f));
+      return ok();
+    });
+  }
   const Gemm8Plan plan = gemm8_plan(m, n, k, sms);
   Gemm8Params p;
-  if (int e = gemm8_map(&p.tmap_a, a, k, m, lda, plan.pair ? 128 : plan.tok_tile)) return e;
-  if (int e = gemm8_map(&p.tmap_w, w, k, n, ldw, 128)) return e;
+  if (int e = gemm8_codes_map(&p.tmap_a, a, k, m, lda, plan.pair ? 128 : plan.tok_tile)) return e;
+  if (int e = gemm8_codes_map(&p.tmap_w, w, k, n, ldw, 128)) return e;
   p.sa = sa, p.sw = sw, p.bias = bias, p.y = y, p.m = m, p.n = n;
   p.k_steps = (k + 127) / 128, p.tok_tile = plan.tok_tile, p.stages = plan.stages;
   p.n_tok_tiles = plan.n_tok_tiles, p.n_w_tiles = plan.n_w_tiles, p.wait_limit_ns = g_wait_limit_ns.load();
@@ -148,6 +164,14 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     using T = decltype(tag);
     const int bit = 24 + 2 * (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 1 : 2);
     if (plan.pair) {
+      p.tma_store = n * sizeof(T) % 16 == 0;
+      if (p.tma_store)
+        if (int e = gemm8_map(&p.tmap_y, y,
+                              std::is_same_v<T, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                              : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                              n, m, static_cast<int64_t>(n) * sizeof(T), 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B))
+          return e;
       if (int e = ensure_smem_attr8(dev, bit, gemm8_pair_kernel<T>, kG8PairSmem)) return e;
       const int pairs = std::min(sms / 2, plan.n_tok_tiles * plan.n_w_tiles);
       W4A4_CUDA_TRY(launch_kernel(gemm8_pair_kernel<T>, dim3(2 * pairs), dim3(kG8PairThreads), kG8PairSmem, stream, 2, p));
@@ -310,8 +334,8 @@ int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, i
   if (!rows_aligned(a, lda, 1, 16) || !rows_aligned(w, ldw, 1, 16))
     return fail(W4A4_ERR_INVALID, "gemm8: rows of codes must begin at multiples of 16 bytes");
   if (!aligned(sw, 16)) return fail(W4A4_ERR_INVALID, "gemm8: channel scales must be 16-byte aligned");
-  if (!aligned(y, 32) || (bias && !aligned(bias, 16)))
-    return fail(W4A4_ERR_INVALID, "gemm8: y must be 32-byte and bias 16-byte aligned");
+  if (!aligned(y, 16) || (bias && !aligned(bias, 16)))
+    return fail(W4A4_ERR_INVALID, "gemm8: y and bias must be 16-byte aligned");
   return launch_gemm8(a, lda, sa, w, ldw, sw, bias, dtype, m, n, k, y, static_cast<cudaStream_t>(stream));
 }
 
