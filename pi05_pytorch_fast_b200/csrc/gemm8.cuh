@@ -83,12 +83,12 @@ __device__ __forceinline__ uint32_t cluster_size() {
 // over once the products are done; token scales; barriers.
 constexpr int kG8TileThreads = 256;
 constexpr int kG8TileMax = 256;  // tokens
-__host__ __device__ constexpr int gemm8_tile_ring(int tok_tile, int stages) {
-  const int ring = stages * (kG8ABytes + tok_tile * kG8StepBytes), sums = 2 * tok_tile * 512;
+__host__ __device__ constexpr int gemm8_tile_ring(int tok_tile, int stages, bool split) {
+  const int ring = stages * (kG8ABytes + tok_tile * kG8StepBytes), sums = (split ? 2 : 1) * tok_tile * 512;
   return ring > sums ? ring : sums;
 }
-__host__ __device__ constexpr int gemm8_tile_smem(int tok_tile, int stages) {
-  const int need = gemm8_tile_ring(tok_tile, stages) + kG8TileMax * 4 + (2 * kG8MaxStages + 2) * 8 + 16 + 1024;
+__host__ __device__ constexpr int gemm8_tile_smem(int tok_tile, int stages, bool split) {
+  const int need = gemm8_tile_ring(tok_tile, stages, split) + kG8TileMax * 4 + (2 * kG8MaxStages + 2) * 8 + 16 + 1024;
   return need > kOneCtaSmem ? need : kOneCtaSmem;
 }
 
@@ -99,10 +99,11 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
   extern __shared__ uint8_t g8_smem[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(g8_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   const int S = p.stages, tok_bytes = p.tok_tile * kG8StepBytes;
+  const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
   uint8_t* w_ring = base;                    // [S][16 KB]
   uint8_t* t_ring = base + S * kG8ABytes;    // [S][T x 128]
   int* sums = reinterpret_cast<int*>(base);  // [T][128], after the products
-  float* tok_scale = reinterpret_cast<float*>(base + gemm8_tile_ring(p.tok_tile, S));  // [256]
+  float* tok_scale = reinterpret_cast<float*>(base + gemm8_tile_ring(p.tok_tile, S, ranks > 1));  // [256]
   uint64_t* bars = reinterpret_cast<uint64_t*>(tok_scale + kG8TileMax);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kG8MaxStages + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -110,7 +111,6 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
   const auto bar_empty = [&](int s) { return smem_addr(bars + kG8MaxStages + s); };
   const uint32_t bar_acc = smem_addr(bars + 2 * kG8MaxStages), bar_recv = smem_addr(bars + 2 * kG8MaxStages + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
   const int tile = blockIdx.x / ranks;
   const int wt = tile / p.n_tok_tiles, tt = tile - wt * p.n_tok_tiles;
   const int n0 = wt * 128;
@@ -187,24 +187,54 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
     if (issuer) umma_commit(bar_acc);
     __syncwarp();
   }
-  // scales and biases for the results below, under the products
-  const G8Channels<T> channels(p, n0 + 4 * lane);  // a lane's four channels of the tile
+  // scales for the results below, under the products
+  const int quarter = warp & 3;
+  const uint32_t tacc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
   if (threadIdx.x < p.tok_tile) tok_scale[threadIdx.x] = m0 + threadIdx.x < p.m ? __ldg(p.sa + m0 + threadIdx.x) : 0.f;
   volatile int no_abort = 0;
-  mbar_wait_bounded(bar_acc, 0, &no_abort, err, kErrWaitAccum, limit);
-  tc_fence_after();
-  __syncthreads();  // the producer has seen its copies land: the ring is free
-  // ---- sums to shared memory: lane = channel, so a column's 128 are one line
-  const int share = p.tok_tile / ranks;  // tokens that each CTA of the cluster finishes
-  {
-    const int quarter = warp & 3;
-    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+  if (ranks == 1) {
+    // ---- straight from TMEM: thread = channel, a column = a token, so a warp
+    // writes 32 consecutive channels of one token at a time
+    const int n = n0 + quarter * 32 + lane;
+    const float sw = n < p.n ? __ldg(p.sw + n) : 0.f;
+    const float bias = p.bias && n < p.n ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
+    __syncthreads();  // tok_scale
+    const bool good = mbar_wait_bounded(bar_acc, 0, &no_abort, err, kErrWaitAccum, limit) && !*abort_flag;
+    tc_fence_after();
+    const int rows = static_cast<int>(min(static_cast<long long>(p.tok_tile), p.m - m0));
+    T* dst = static_cast<T*>(p.y) + m0 * p.n + n;
+    for (int c0 = (warp >> 2) * 16; c0 < p.tok_tile; c0 += 64) {
+      uint32_t r[2][16];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (c0 + 32 * i < p.tok_tile) tmem_ld_32x32b_x16(tacc + c0 + 32 * i, r[i]);
+      tmem_ld_wait();
+      if (!good || n >= p.n) continue;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int t = c0 + 32 * i + j;
+          if (t < rows)
+            dst[static_cast<long long>(t) * p.n] =
+                from_float<T>(fmaf(static_cast<float>(static_cast<int>(r[i][j])) * tok_scale[t], sw, bias));
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+  } else {
+    const G8Channels<T> channels(p, n0 + 4 * lane);  // a lane's four channels of the tile
+    mbar_wait_bounded(bar_acc, 0, &no_abort, err, kErrWaitAccum, limit);
+    tc_fence_after();
+    __syncthreads();  // the producer has seen its copies land: the ring is free
+    // ---- sums to shared memory: lane = channel, so a column's 128 are one line
+    const int share = p.tok_tile / ranks;  // tokens that each CTA of the cluster finishes
     for (int c0 = (warp >> 2) * 16; c0 < p.tok_tile; c0 += 64) {
       uint32_t r[2][16];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if (steps > 0 && c0 + 32 * i < p.tok_tile) {
-          tmem_ld_32x32b_x16(tmem_base + lane_addr + c0 + 32 * i, r[i]);
+          tmem_ld_32x32b_x16(tacc + c0 + 32 * i, r[i]);
         } else {
 #pragma unroll
           for (int j = 0; j < 16; ++j) r[i][j] = 0u;
@@ -217,13 +247,11 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
 #pragma unroll
           for (int j = 0; j < 16; ++j) sums[(c0 + 32 * i + j) * 128 + quarter * 32 + lane] = static_cast<int>(r[i][j]);
     }
-  }
-  tc_fence_before();
-  const int first = rank * share;
-  int* recv = sums + p.tok_tile * 128;  // [ranks - 1][share][128]
-  if (ranks > 1) {
+    tc_fence_before();
     // ---- every CTA sends each other one its share of the sums, one bulk copy
-    // each (remote loads move an eighth of what these do)
+    // each (loads from remote shared memory move a fraction of what these do)
+    const int first = rank * share;
+    int* recv = sums + p.tok_tile * 128;  // [ranks - 1][share][128]
     if (threadIdx.x == 0) mbar_arrive_expect_tx(bar_recv, static_cast<uint32_t>((ranks - 1) * share * 512));
     fence_proxy_async_smem();
     cluster_sync();  // sums written, barriers armed, rings free in all of them
@@ -233,24 +261,23 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
                           mapa_shared(bar_recv, lane));
     __syncwarp();
     mbar_wait_bounded_cl(bar_recv, 0, &no_abort, err, kErrWaitAccum, limit);
-  } else {
-    __syncthreads();
-  }
-  const bool aborted = *abort_flag != 0;
-  const int4* own = reinterpret_cast<const int4*>(sums + first * 128) + lane;
-  const int4* others = reinterpret_cast<const int4*>(recv) + lane;
-#pragma unroll 4
-  for (int t = warp; t < share; t += 8) {
-    int4 acc = own[t * 32];
-    for (int r = 0; r + 1 < ranks; ++r) {
-      const int4 x = others[(r * share + t) * 32];
-      acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+    const bool aborted = *abort_flag != 0;
+    const int4* own = reinterpret_cast<const int4*>(sums + first * 128) + lane;
+    const int4* others = reinterpret_cast<const int4*>(recv) + lane;
+#pragma unroll 2
+    for (int t = warp; t < share; t += 8) {
+      int4 acc = own[t * 32];
+#pragma unroll
+      for (int r = 0; r < 7; ++r) {
+        if (r + 1 >= ranks) break;
+        const int4 x = others[(r * share + t) * 32];
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+      }
+      const long long m = m0 + first + t;
+      if (!aborted && m < p.m && n0 + 4 * lane < p.n) channels.store(p, m, n0 + 4 * lane, acc, tok_scale[first + t]);
     }
-    const long long m = m0 + first + t;
-    if (!aborted && m < p.m && n0 + 4 * lane < p.n) channels.store(p, m, n0 + 4 * lane, acc, tok_scale[first + t]);
+    cluster_sync();  // no CTA leaves before its copies have been received
   }
-  if (ranks > 1) cluster_sync();  // no CTA leaves before its copies have been received
-  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem_base, cols);
@@ -258,7 +285,7 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
 }
 
 // -------------------------------------------------------- few tokens (<= 16)
-// One CTA of 8 warps per 8 NT channels; the warps share K in runs of 64 bytes
+// One CTA of 8 or 16 warps per 8 NT channels; the warps share K in runs of 64 bytes
 // and add their sums through shared memory.  mma.sync m16n8k32: the 16 rows are
 // the tokens, the 8 columns weight rows; as K may be permuted when both
 // operands agree, lane (g, t) loads 16 consecutive bytes of row g at 64 c + 16 t
@@ -302,10 +329,10 @@ __device__ __forceinline__ uint4 g8_load_tail(const int8_t* row, int e, int k) {
   return v;
 }
 
-template <typename T, bool HALF, int NT>
-__global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ Gemm8FewParams p) {
+template <typename T, bool HALF, int NT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) gemm8_few_kernel(const __grid_constant__ Gemm8FewParams p) {
   constexpr int R = HALF ? 8 : 16;
-  __shared__ int part[8][R][8 * NT];
+  __shared__ int part[WARPS][R][8 * NT];
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -317,7 +344,7 @@ __global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ 
   const int8_t* w[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) w[i] = p.w + static_cast<long long>(min(n0 + 8 * i + g, p.n - 1)) * p.ldw + 16 * t;
-  const int full = p.k / 64;  // runs of 64 bytes: warp, warp + 8, ...
+  const int full = p.k / 64;  // runs of 64 bytes: warp, warp + WARPS, ...
   const auto product = [&](const uint4& x0, const uint4& x1, const uint4 (&b)[NT]) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -327,11 +354,11 @@ __global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ 
   };
   constexpr int U = 4;  // runs whose loads are under way together
   int c = warp;
-  for (; c + 8 * (U - 1) < full; c += 8 * U) {
+  for (; c + WARPS * (U - 1) < full; c += WARPS * U) {
     uint4 x0[U], x1[U], b[U][NT];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int e = 64 * (c + 8 * u);
+      const int e = 64 * (c + WARPS * u);
 #pragma unroll
       for (int i = 0; i < NT; ++i) b[u][i] = __ldg(reinterpret_cast<const uint4*>(w[i] + e));
       x0[u] = __ldg(reinterpret_cast<const uint4*>(a0 + e));
@@ -340,7 +367,7 @@ __global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ 
 #pragma unroll
     for (int u = 0; u < U; ++u) product(x0[u], x1[u], b[u]);
   }
-  for (; 64 * c < p.k; c += 8) {
+  for (; 64 * c < p.k; c += WARPS) {
     const int e = 64 * c;
     uint4 b[NT];
 #pragma unroll
@@ -355,12 +382,12 @@ __global__ void __launch_bounds__(256) gemm8_few_kernel(const __grid_constant__ 
     if constexpr (!HALF) *reinterpret_cast<int2*>(&part[warp][g + 8][8 * i + 2 * t]) = make_int2(acc[i][2], acc[i][3]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < R * 8 * NT; i += 256) {
+  for (int i = threadIdx.x; i < R * 8 * NT; i += 32 * WARPS) {
     const int r = i / (8 * NT), n = n0 + i % (8 * NT);
     if (r >= p.m || n >= p.n) continue;
     int sum = 0;
 #pragma unroll
-    for (int x = 0; x < 8; ++x) sum += part[x][r][i % (8 * NT)];
+    for (int x = 0; x < WARPS; ++x) sum += part[x][r][i % (8 * NT)];
     const float b = p.bias ? to_float(static_cast<const T*>(p.bias)[n]) : 0.f;
     static_cast<T*>(p.y)[static_cast<long long>(r) * p.n + n] =
         from_float<T>(fmaf(static_cast<float>(sum) * __ldg(p.sa + r), __ldg(p.sw + n), b));

@@ -68,10 +68,12 @@ Rows rows_of(const Tensor& x) {
   return {t, m, m > 1 ? t.stride(0) : h};
 }
 
-// int8 of x's shape whose rows begin at multiples of 16 bytes.
+// int8 of x's shape whose rows begin at multiples of 128 bytes, the product's
+// steps (a step of an unaligned row takes two lines of L2), or of 16 bytes
+// where a row is no longer than that.
 Tensor empty_codes(const Tensor& x, int64_t m, int64_t* ld) {
   const int64_t h = x.size(-1);
-  *ld = (h + 15) / 16 * 16;
+  *ld = h <= 128 ? (h + 15) / 16 * 16 : (h + 127) / 128 * 128;
   const auto opts = x.options().dtype(at::kChar);
   if (*ld == h) return at::empty(x.sizes(), opts);
   std::vector<int64_t> stride(x.dim(), 1);
@@ -195,7 +197,7 @@ Rows tma_rows(Rows r, const char* what) {
   TORCH_WARN_ONCE("pi05_w8a8.linear: rows of ", what,
                   " do not begin at multiples of 16 bytes; copying them on every call. quantize, rms_norm_quant and "
                   "pack_weight lay them out.");
-  const int64_t ld = (k + 15) / 16 * 16;
+  const int64_t ld = (k + 127) / 128 * 128;
   Tensor t = at::empty({r.m, ld}, r.t.options()).narrow(1, 0, k);
   t.copy_(r.t);
   return {t, r.m, ld};

@@ -87,34 +87,80 @@ int check_rows8(int64_t rows, int32_t h, const void* x, int64_t ldx, const int8_
   return W4A4_OK;
 }
 
-// How a product runs: on CTA pairs, or in tiles of 128 channels x tok_tile
-// tokens whose K is split over clusters of `split` CTAs.
+// How a product of more than 16 tokens runs: on CTA pairs, or in tiles of 128
+// channels x tok_tile tokens whose K is split over clusters of `split` CTAs.
 struct Gemm8Plan {
   bool pair;
   int tok_tile, split, stages;
   int n_tok_tiles, n_w_tiles;
 };
-Gemm8Plan gemm8_plan(int64_t m, int n, int k, int sms) {
-  Gemm8Plan plan{};
+
+// The cheapest of the two kernels' launch shapes, by a model in us fitted to
+// graph-timed runs on a B200 of 30 shapes (17 .. 2,048 tokens, K 64 .. 16,384, N 64
+// .. 16,384) in every shape that the kernels allow:
+//   tile: a wave costs 4.0 + 0.012 T (set-up, first loads, epilogue) and a step
+//   of K 0.16 + 0.0006 T; splitting K adds 1.2 + 0.012 T for the exchange;
+//   pair: 6.0, and a wave its steps at 0.27 or its epilogue at 2.4.
+// The choice is within 8 % of the best measured shape for 27 of them.  One
+// CTA runs on an SM; `fit[i]` is how many clusters of 1 << i CTAs fit the
+// device at once (148, 74, 33 and 15 on a B200: whole clusters in a GPC).
+Gemm8Plan gemm8_plan(int64_t m, int n, int k, const int (&fit)[4]) {
+  Gemm8Plan best{};
+  double cost = 1e300;
   const int k_steps = (k + 127) / 128;
-  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
-  plan.pair = m > 256 && pair_tiles >= sms / 4;
-  if (plan.pair) {
-    plan.n_tok_tiles = static_cast<int>((m + 255) / 256);
-    plan.n_w_tiles = (n + 255) / 256;
-    return plan;
+  const auto waves = [](int64_t tiles, int at_once) { return static_cast<double>((tiles + at_once - 1) / at_once); };
+  const int n_w_tiles = (n + 127) / 128;
+  // fewer token tiles than this would exceed 256 tokens, more would be below 16
+  const int64_t most = std::min<int64_t>((m + 15) / 16, (m + 255) / 256 + 64);
+  for (int64_t tiles = (m + 255) / 256; tiles <= most; ++tiles) {
+    const int t = static_cast<int>(((m + tiles - 1) / tiles + 15) / 16 * 16);
+    const int n_tok_tiles = static_cast<int>((m + t - 1) / t);
+    for (int i = 0; i < 4; ++i) {
+      const int split = 1 << i;
+      if (fit[i] < 1 || (split > 1 && (split > k_steps || t > 128))) continue;
+      const int steps = (k_steps + split - 1) / split;
+      const double c = waves(static_cast<int64_t>(n_tok_tiles) * n_w_tiles, fit[i]) * (4.0 + 0.012 * t + steps * (0.16 + 0.0006 * t)) +
+                       (split > 1 ? 1.2 + 0.012 * t : 0.0);
+      if (c < cost - 1e-9) {
+        cost = c;
+        best = {false, t, split, 0, n_tok_tiles, n_w_tiles};
+      }
+    }
   }
-  const int64_t tiles = (m + 127) / 128;
-  plan.tok_tile = static_cast<int>(((m + tiles - 1) / tiles + 15) / 16 * 16);
-  plan.n_tok_tiles = static_cast<int>((m + plan.tok_tile - 1) / plan.tok_tile);
-  plan.n_w_tiles = (n + 127) / 128;
-  const int64_t work = static_cast<int64_t>(plan.n_tok_tiles) * plan.n_w_tiles;
-  plan.split = 1;
-  while (plan.split < 8 && work * plan.split * 2 <= sms + sms / 8 && k_steps >= 4 * plan.split) plan.split *= 2;
-  const int steps = (k_steps + plan.split - 1) / plan.split;
-  const int step_bytes = kG8ABytes + plan.tok_tile * kG8StepBytes;
-  plan.stages = std::max(1, std::min({steps, kG8MaxStages, 200 * 1024 / step_bytes}));
-  return plan;
+  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  if (6.0 + waves(pair_tiles, fit[1]) * std::max(0.27 * k_steps, 2.4) < cost) {
+    best = {true, 0, 1, 0, static_cast<int>((m + 255) / 256), (n + 255) / 256};
+    return best;
+  }
+  const int steps = (k_steps + best.split - 1) / best.split;
+  best.stages = std::max(1, std::min({steps, kG8MaxStages, 200 * 1024 / (kG8ABytes + best.tok_tile * kG8StepBytes)}));
+  return best;
+}
+
+// Clusters of 1, 2, 4 and 8 CTAs of the tile kernel that the device runs at once.
+int g_gemm8_fit[kMaxDevices][4];
+int gemm8_fit(int dev, int sms, int (&fit)[4]) {
+  std::lock_guard<std::mutex> lk(g_dev_mu);
+  int(&f)[4] = g_gemm8_fit[dev];
+  if (f[0] == 0) {
+    W4A4_CUDA_TRY(cudaFuncSetAttribute(gemm8_tile_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
+    for (int i = 1; i < 4; ++i) {
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(8 << i);
+      cfg.blockDim = dim3(kG8TileThreads);
+      cfg.dynamicSmemBytes = kOneCtaSmem;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      W4A4_CUDA_TRY(cudaOccupancyMaxActiveClusters(&f[i], gemm8_tile_kernel<__half>, &cfg));
+    }
+    f[0] = sms;
+  }
+  std::copy(f, f + 4, fit);
+  return W4A4_OK;
 }
 
 // Tiled map of rows of `k` elements of `size` bytes with boxes of bx elements x
@@ -145,15 +191,22 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     const Gemm8FewParams f{a, w, sa, sw, bias, y, lda, ldw, static_cast<int>(m), n, k};
     return by_dtype(dtype, true, "gemm8", [&](auto tag) {
       using T = decltype(tag);
-      const bool wide = n >= 32 * sms;  // enough CTAs with 16 channels each: half the reads of the tokens
-      const auto kernel = m <= 8 ? (wide ? gemm8_few_kernel<T, true, 2> : gemm8_few_kernel<T, true, 1>)
-                                 : (wide ? gemm8_few_kernel<T, false, 2> : gemm8_few_kernel<T, false, 1>);
+      // 16 channels a CTA where that leaves enough CTAs (the tokens are read half as often), and twice the
+      // warps, to have enough loads under way, where there are few CTAs and a long K
+      const bool wide = n >= 32 * sms, deep = !wide && k >= 4096;
+      const auto by_shape = [&](auto half_tag) {
+        constexpr bool H = decltype(half_tag)::value;
+        return deep ? gemm8_few_kernel<T, H, 1, 16> : wide ? gemm8_few_kernel<T, H, 2, 8> : gemm8_few_kernel<T, H, 1, 8>;
+      };
+      const auto kernel = m <= 8 ? by_shape(std::true_type{}) : by_shape(std::false_type{});
       const int per = wide ? 16 : 8;
-      W4A4_CUDA_TRY(launch_kernel(kernel, dim3((n + per - 1) / per), dim3(256), 0, stream, 1, f));
+      W4A4_CUDA_TRY(launch_kernel(kernel, dim3((n + per - 1) / per), dim3(deep ? 512 : 256), 0, stream, 1, f));
       return ok();
     });
   }
-  const Gemm8Plan plan = gemm8_plan(m, n, k, sms);
+  int fit[4];
+  if (int e = gemm8_fit(dev, sms, fit)) return e;
+  const Gemm8Plan plan = gemm8_plan(m, n, k, fit);
   Gemm8Params p;
   if (int e = gemm8_codes_map(&p.tmap_a, a, k, m, lda, plan.pair ? 128 : plan.tok_tile)) return e;
   if (int e = gemm8_codes_map(&p.tmap_w, w, k, n, ldw, 128)) return e;
@@ -178,7 +231,7 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     } else {
       if (int e = ensure_smem_attr8(dev, bit + 1, gemm8_tile_kernel<T>, kSmemLimit)) return e;
       W4A4_CUDA_TRY(launch_kernel(gemm8_tile_kernel<T>, dim3(plan.split * plan.n_tok_tiles * plan.n_w_tiles),
-                                  dim3(kG8TileThreads), gemm8_tile_smem(plan.tok_tile, plan.stages), stream, plan.split, p));
+                                  dim3(kG8TileThreads), gemm8_tile_smem(plan.tok_tile, plan.stages, plan.split > 1), stream, plan.split, p));
     }
     return ok();
   });

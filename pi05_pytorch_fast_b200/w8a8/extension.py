@@ -19,12 +19,13 @@ from ..w4a4 import extension as _w4a4
 CACHE_BLOCK = nat.KV8_BLOCK  # cache tokens that share a scale
 
 
-def _rows16(shape) -> int:
-    return (shape[-1] + 15) // 16 * 16
+def _code_stride(h: int) -> int:
+    """Row stride of codes: a multiple of 128 bytes, or of 16 for short rows."""
+    return (h + 15) // 16 * 16 if h <= 128 else (h + 127) // 128 * 128
 
 
 def _fake_codes(x: torch.Tensor) -> torch.Tensor:
-    ld = _rows16(x.shape)
+    ld = _code_stride(x.shape[-1])
     if ld == x.shape[-1]:
         return torch.empty(x.shape, dtype=torch.int8, device=x.device)
     stride, step = [1], ld
