@@ -13,9 +13,12 @@
 // a row with an infinity or NaN gets a non-finite scale and zero codes, so that
 // its values (code x scale) are NaN and the fault stays visible.
 //
-// Bound: HBM (a norm row of bf16 moves 7 bytes per element at about 30
-// instructions).  A row is read once and stays in registers through both
-// reductions, one CTA of h / (8 VPT) threads per row.
+// Bound: HBM.  A row is read once and stays in registers through both
+// reductions, one CTA of h / (8 VPT) threads to a row; a CTA takes several rows
+// in turn, and asks for the next one's vectors before it reduces this one, so
+// that loads are under way all the time.  The arithmetic is two lanes wide
+// (f32x2) and codes come from one multiply-add, as at the memory's rate there
+// are about 25 issue slots for an element of the GeGLU.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -120,47 +123,75 @@ __device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
 
 // gelu(x) = x / (1 + exp(-2 u)), u = sqrt(2/pi) (x + 0.044715 x^3): the tanh
 // form 0.5 x (1 + tanh u) with 1 + tanh u = 2 / (1 + exp(-2 u)), which does not
-// cancel for negative u.
-__device__ __forceinline__ float gelu_tanh_f32(float x) {
-  const float u2 = 1.5957691216057308f * fmaf(0.044715f * x * x, x, x);
-  return __fdividef(x, 1.0f + __expf(-u2));
+// cancel for negative u.  exp(-2 u) = 2^(x (a + b x^2)).
+constexpr float kGeluA = -2.302208198f;  // -2 sqrt(2/pi) log2(e)
+constexpr float kGeluB = -0.1029432397f; // 0.044715 of it
+__device__ __forceinline__ float fast_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float2 gelu_tanh_f32x2(float2 x) {
+  const float2 q = __ffma2_rn(make_float2(kGeluB, kGeluB), __fmul2_rn(x, x), make_float2(kGeluA, kGeluA));
+  const float2 a = __fmul2_rn(x, q);
+  const float2 d = __fadd2_rn(make_float2(fast_ex2(a.x), fast_ex2(a.y)), make_float2(1.f, 1.f));
+  return __fmul2_rn(x, make_float2(fast_rcp(d.x), fast_rcp(d.y)));
 }
 
-// How codes of a value are formed from a row's (block's) scale: a multiply by
-// the reciprocal, which can move a value within an ulp of a rounding tie to
-// the other side, or, for scales whose reciprocal would overflow, a division.
+// How codes of a value are formed from a row's scale.  fast: v / scale rounded
+// by the addition of 1.5 x 2^23, whose sum holds the code in its low byte (a
+// value within an ulp of a tie may go to the other side; |v| <= 127.0001 scale,
+// so nothing needs a clamp).  Scales that are zero, not finite, or so small
+// that the reciprocal overflows take the slow way.
 struct Coder {
   float mul, div;
+  bool fast;
   __device__ __forceinline__ explicit Coder(float scale) {
     const bool finite = scale <= 3.4028234e38f;  // false for NaN
     const bool tiny = scale < 7.8886091e-31f;    // 2^-100
-    mul = finite && !tiny ? __frcp_rn(scale) : 0.f;
-    div = finite && tiny && scale > 0.f ? scale : 0.f;
+    fast = finite && !tiny;
+    mul = fast ? __frcp_rn(scale) : 0.f;
+    div = finite && scale > 0.f ? scale : 0.f;
   }
-  __device__ __forceinline__ int operator()(float v) const {
-    float t = v * mul;
-    if (div != 0.f) t = __fdiv_rn(v, div);
-    // a NaN (a non-finite row: inf * 0) becomes code 0
-    return t == t ? __float2int_rn(fminf(fmaxf(t, -127.f), 127.f)) : 0;
+  // the code in the low byte
+  __device__ __forceinline__ uint32_t quick(float v) const { return __float_as_uint(fmaf(v, mul, 12582912.f)); }
+  __device__ __forceinline__ uint32_t slow(float v) const {
+    const float t = div > 0.f ? __fdiv_rn(v, div) : 0.f;
+    return t == t ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(t, -127.f), 127.f))) : 0u;
   }
 };
 
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+// Low bytes of four words.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 template <int W>
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[W], const Coder& code) {
-  if constexpr (W == 8) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack4(code(v[0]), code(v[1]), code(v[2]), code(v[3])),
-                                              pack4(code(v[4]), code(v[5]), code(v[6]), code(v[7])));
+  uint32_t c[W];
+  if (code.fast) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) c[i] = code.quick(v[i]);
   } else {
-    *p = static_cast<int8_t>(code(v[0]));
+#pragma unroll
+    for (int i = 0; i < W; ++i) c[i] = code.slow(v[i]);
   }
+  if constexpr (W == 8) *reinterpret_cast<uint2*>(p) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+  else *p = static_cast<int8_t>(c[0]);
 }
 
 // |v| as an unsigned key: ordered like the value, infinity above every finite
 // value and NaN above infinity, so a maximum of keys keeps a NaN.
 __device__ __forceinline__ uint32_t abs_key(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// max(m, |v|), a NaN of either side kept.
+__device__ __forceinline__ float max_abs(float m, float v) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
+  return m;
+}
 
 // Reductions over a CTA of whole warps; `red` has 32 words; every thread gets
 // the result.  Two calls in a row need different buffers.
@@ -186,102 +217,171 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return __reduce_max_sync(0xffffffffu, v);
 }
 
-// x (and delta / up) at element e of a row -> the value before the norm.
-template <int OP, int W, typename T>
-__device__ __forceinline__ void row8_load(const Row8Params& p, const T* x, const T* x2, const T* gate, int e,
-                                          float (&v)[W]) {
-  load_w<W>(x + e, v);
-  if constexpr (OP == kRowGeglu) {
-    float u[W];
-    load_w<W>(x2 + e, u);
+// W elements as they lie in memory, to be asked for early and unpacked later.
+template <typename T, int W>
+struct RawVec {
+  static constexpr int kWords = W * sizeof(T) / 16;
+  uint4 q[kWords > 0 ? kWords : 1];
+  T one;
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWords > 0) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = gelu_tanh_f32(v[i]) * u[i];
-  } else if constexpr (OP == kRowNorm) {
-    if (x2) {
-      float d[W];
-      load_w<W>(x2 + e, d);
-      if (gate) {
-        float g[W];
-        load_w<W>(gate + e, g);
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = fmaf(g[i], d[i], v[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i) v[i] += d[i];
-      }
+      for (int i = 0; i < kWords; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      one = *p;
     }
   }
-}
+  __device__ __forceinline__ void unpack(float (&v)[W]) const {
+    if constexpr (kWords > 0) load8(reinterpret_cast<const T*>(q), v);
+    else v[0] = to_float(one);
+  }
+};
 
 template <int W>
-__device__ __forceinline__ void row8_norm(const float* gain, const float* shift, int e, float rstd, float (&v)[W]) {
-  float g[W];
-  load_w<W>(gain + e, g);
-  if (shift) {
-    float b[W];
-    load_w<W>(shift + e, b);
+__device__ __forceinline__ void mul_w(float (&v)[W], const float (&u)[W]) {
+  if constexpr (W == 8) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = fmaf(v[i] * rstd, g[i], b[i]);
+    for (int i = 0; i < 8; i += 2) {
+      const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(u[i], u[i + 1]));
+      v[i] = r.x, v[i + 1] = r.y;
+    }
   } else {
+    v[0] *= u[0];
+  }
+}
+// v = a v + b
+template <int W>
+__device__ __forceinline__ void fma_w(float (&v)[W], const float (&a)[W], const float (&b)[W]) {
+  if constexpr (W == 8) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) v[i] = v[i] * rstd * g[i];
+    for (int i = 0; i < 8; i += 2) {
+      const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(v[i], v[i + 1]), make_float2(b[i], b[i + 1]));
+      v[i] = r.x, v[i + 1] = r.y;
+    }
+  } else {
+    v[0] = fmaf(a[0], v[0], b[0]);
+  }
+}
+template <int W>
+__device__ __forceinline__ void gelu_w(float (&v)[W]) {
+  if constexpr (W == 8) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+      const float2 r = gelu_tanh_f32x2(make_float2(v[i], v[i + 1]));
+      v[i] = r.x, v[i + 1] = r.y;
+    }
+  } else {
+    v[0] = gelu_tanh_f32x2(make_float2(v[0], 0.f)).x;
   }
 }
 
-// One row per CTA, held in registers: thread t has the W-element groups
-// t, t + blockDim, ... (VPT of them).
-template <typename T, int OP, int W, int VPT>
-__global__ void __launch_bounds__(1024) row8_kernel(const __grid_constant__ Row8Params p) {
-  __shared__ float red_sum[32];
-  __shared__ uint32_t red_max[32];
-  pdl_launch_dependents();
-  pdl_wait();
-  const long long row = blockIdx.x;
-  const long long obs = row / p.rows_per_batch;
-  const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-  const T* x2 = p.x2 ? static_cast<const T*>(p.x2) + row * p.ld2 : nullptr;
-  const T* gate = p.gate ? static_cast<const T*>(p.gate) + obs * p.gate_stride : nullptr;
-  const int groups = (p.h + W - 1) / W;  // W = 8: h is a multiple of 8
-  float v[VPT][W];
-  float ss = 0.f;
+// x and delta / up of W elements -> the value before the norm (v + gate u).
+template <int OP, int W>
+__device__ __forceinline__ void row8_combine(float (&v)[W], float (&u)[W], bool has, bool gated, const float (&gate)[W]) {
+  if constexpr (OP == kRowGeglu) {
+    gelu_w<W>(v);
+    mul_w<W>(v, u);
+  } else if constexpr (OP == kRowNorm) {
+    if (has) {
+      if (gated) {
+        fma_w<W>(u, gate, v);
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int g = threadIdx.x + j * blockDim.x;
-    if (g < groups) {
-      row8_load<OP, W, T>(p, x, x2, gate, g * W, v[j]);
-      if constexpr (OP == kRowNorm) {
-        if (p.total) store_w<W>(static_cast<T*>(p.total) + row * p.h + g * W, v[j]);
+        for (int i = 0; i < W; ++i) v[i] = u[i];
+      } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) ss = fmaf(v[j][i], v[j][i], ss);
+        for (int i = 0; i < W; ++i) v[i] += u[i];
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < W; ++i) v[j][i] = 0.f;
     }
   }
-  if constexpr (OP == kRowNorm) {
-    const float rstd = rsqrtf(block_sum(ss, red_sum) / static_cast<float>(p.h) + p.eps);
-    const float* gain = p.gain + obs * p.gain_stride;
-    const float* shift = p.shift ? p.shift + obs * p.shift_stride : nullptr;
+}
+
+// One row of a CTA at a time, held in registers: thread t has the W-element
+// groups t, t + blockDim, ... (VPT of them).  A CTA takes consecutive rows, so
+// that an observation's gain, shift and gate come from L1 after its first row.
+template <typename T, int OP, int W, int VPT, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant__ Row8Params p) {
+  __shared__ float red_sum[32];
+  __shared__ uint32_t red_max[2][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int groups = (p.h + W - 1) / W;  // W = 8: h is a multiple of 8
+  const bool has2 = p.x2 != nullptr;
+  RawVec<T, W> rx[VPT], ru[VPT];
+  const auto fetch = [&](long long row) {
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* x2 = static_cast<const T*>(p.x2) + row * p.ld2;
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int g = threadIdx.x + j * blockDim.x;
-      if (g < groups) row8_norm<W>(gain, shift, g * W, rstd, v[j]);
+      if (g < groups) {
+        rx[j].load(x + g * W);
+        if (OP != kRowQuant && has2) ru[j].load(x2 + g * W);
+      }
     }
+  };
+  long long row = p.rows * blockIdx.x / gridDim.x;
+  const long long end = p.rows * (blockIdx.x + 1) / gridDim.x;
+  fetch(row);
+  for (int turn = 0; row < end; ++row, turn ^= 1) {
+    const long long obs = OP == kRowNorm ? row / p.rows_per_batch : 0;
+    const T* gate = static_cast<const T*>(p.gate) + obs * p.gate_stride;
+    float v[VPT][W];
+    float ss[2] = {0.f, 0.f};
+    {
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const int g = threadIdx.x + j * blockDim.x;
+        if (g < groups) {
+          float u[W];
+          rx[j].unpack(v[j]);
+          if (OP != kRowQuant && has2) ru[j].unpack(u);
+          float gv[W];
+          if (OP == kRowNorm && p.gate) load_w<W>(gate + g * W, gv);
+          row8_combine<OP, W>(v[j], u, has2, p.gate != nullptr, gv);
+          if constexpr (OP == kRowNorm) {
+            if (p.total) store_w<W>(static_cast<T*>(p.total) + row * p.h + g * W, v[j]);
+#pragma unroll
+            for (int i = 0; i < W; ++i) ss[i & 1] = fmaf(v[j][i], v[j][i], ss[i & 1]);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < W; ++i) v[j][i] = 0.f;
+        }
+      }
+    }
+    if (row + 1 < end) fetch(row + 1);
+    if constexpr (OP == kRowNorm) {
+      const float rstd = rsqrtf(block_sum(ss[0] + ss[1], red_sum) / static_cast<float>(p.h) + p.eps);
+      const float* gain = p.gain + obs * p.gain_stride;
+      const float* shift = p.shift + obs * p.shift_stride;
+#pragma unroll
+      for (int j = 0; j < VPT; ++j) {
+        const int g = threadIdx.x + j * blockDim.x;
+        if (g < groups) {
+          float gn[W], sh[W], r[W];
+          load_w<W>(gain + g * W, gn);
+#pragma unroll
+          for (int i = 0; i < W; ++i) r[i] = rstd, sh[i] = 0.f;
+          if (p.shift) load_w<W>(shift + g * W, sh);
+          mul_w<W>(v[j], r);
+          fma_w<W>(v[j], gn, sh);
+        }
+      }
+    }
+    float amax = 0.f;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j)
+#pragma unroll
+      for (int i = 0; i < W; ++i) amax = max_abs(amax, v[j][i]);
+    const float scale = __uint_as_float(block_max(abs_key(amax), red_max[turn])) * kInv127;
+    const Coder code(scale);
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      const int g = threadIdx.x + j * blockDim.x;
+      if (g < groups) store_codes<W>(p.codes + row * p.ldc + g * W, v[j], code);
+    }
+    if (threadIdx.x == 0) p.scale[row] = scale;
   }
-  uint32_t key = 0;
-#pragma unroll
-  for (int j = 0; j < VPT; ++j)
-#pragma unroll
-    for (int i = 0; i < W; ++i) key = max(key, abs_key(v[j][i]));
-  const float scale = __uint_as_float(block_max(key, red_max)) * kInv127;
-  const Coder code(scale);
-#pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    const int g = threadIdx.x + j * blockDim.x;
-    if (g < groups) store_codes<W>(p.codes + row * p.ldc + g * W, v[j], code);
-  }
-  if (threadIdx.x == 0) p.scale[row] = scale;
 }
 
 // Rows too long for registers: each pass reads the row again (from L2).
@@ -296,61 +396,61 @@ __global__ void __launch_bounds__(1024) row8_long_kernel(const __grid_constant__
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* x2 = p.x2 ? static_cast<const T*>(p.x2) + row * p.ld2 : nullptr;
   const T* gate = p.gate ? static_cast<const T*>(p.gate) + obs * p.gate_stride : nullptr;
-  const float* gain = nullptr;
-  const float* shift = nullptr;
+  const float* gain = OP == kRowNorm ? p.gain + obs * p.gain_stride : nullptr;
+  const float* shift = OP == kRowNorm && p.shift ? p.shift + obs * p.shift_stride : nullptr;
   float rstd = 0.f;
+  const auto value = [&](int e, bool normed) {
+    float v[1] = {to_float(x[e])}, u[1] = {x2 ? to_float(x2[e]) : 0.f};
+    const float gv[1] = {gate ? to_float(gate[e]) : 1.f};
+    row8_combine<OP, 1>(v, u, x2 != nullptr, gate != nullptr, gv);
+    return OP == kRowNorm && normed ? fmaf(gain[e], v[0] * rstd, shift ? shift[e] : 0.f) : v[0];
+  };
   if constexpr (OP == kRowNorm) {
-    gain = p.gain + obs * p.gain_stride;
-    shift = p.shift ? p.shift + obs * p.shift_stride : nullptr;
     float ss = 0.f;
     for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-      float v[1];
-      row8_load<OP, 1, T>(p, x, x2, gate, e, v);
-      if (p.total) store_w<1>(static_cast<T*>(p.total) + row * p.h + e, v);
-      ss = fmaf(v[0], v[0], ss);
+      const float v = value(e, false);
+      if (p.total) static_cast<T*>(p.total)[row * p.h + e] = from_float<T>(v);
+      ss = fmaf(v, v, ss);
     }
     rstd = rsqrtf(block_sum(ss, red_sum) / static_cast<float>(p.h) + p.eps);
   }
-  uint32_t key = 0;
-  for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-    float v[1];
-    row8_load<OP, 1, T>(p, x, x2, gate, e, v);
-    if constexpr (OP == kRowNorm) row8_norm<1>(gain, shift, e, rstd, v);
-    key = max(key, abs_key(v[0]));
-  }
-  const float scale = __uint_as_float(block_max(key, red_max)) * kInv127;
+  float amax = 0.f;
+  for (int e = threadIdx.x; e < p.h; e += blockDim.x) amax = max_abs(amax, value(e, true));
+  const float scale = __uint_as_float(block_max(abs_key(amax), red_max)) * kInv127;
   const Coder code(scale);
   for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-    float v[1];
-    row8_load<OP, 1, T>(p, x, x2, gate, e, v);
-    if constexpr (OP == kRowNorm) row8_norm<1>(gain, shift, e, rstd, v);
+    const float v[1] = {value(e, true)};
     store_codes<1>(p.codes + row * p.ldc + e, v, code);
   }
   if (threadIdx.x == 0) p.scale[row] = scale;
 }
 
-// out[r, :] = codes[r, :] * scale[r], rounded once; grid (column groups of
-// 256 x W, rows).
+// out[r, :] = codes[r, :] * scale[r], rounded once.  W = 16 or 1 codes a
+// thread, `per` threads to a row.
 template <typename T, int W>
 __global__ void __launch_bounds__(256) dequant8_kernel(const int8_t* __restrict__ codes, long long ldc,
                                                        const float* __restrict__ scale, T* __restrict__ out,
-                                                       long long rows, int h) {
+                                                       long long total, int per, int h) {
   pdl_launch_dependents();
   pdl_wait();
-  const int e = (blockIdx.x * 256 + threadIdx.x) * W;
-  if (e >= h) return;
-  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float s = scale[row];
-    float v[W];
-    if constexpr (W == 8) {
-      const uint2 raw = *reinterpret_cast<const uint2*>(codes + row * ldc + e);
+  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  const long long row = i / per;
+  const int e = static_cast<int>(i - row * per) * W;
+  const float s = __ldg(scale + row);
+  if constexpr (W == 16) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * ldc + e));
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = static_cast<float>(static_cast<int8_t>((i < 4 ? raw.x : raw.y) >> (8 * (i & 3)))) * s;
-    } else {
-      v[0] = static_cast<float>(codes[row * ldc + e]) * s;
+    for (int half = 0; half < 2; ++half) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[j] = static_cast<float>(static_cast<int8_t>(w[2 * half + (j >> 2)] >> (8 * (j & 3)))) * s;
+      store8(out + row * h + e + 8 * half, v);
     }
-    store_w<W>(out + row * h + e, v);
+  } else {
+    out[row * h + e] = from_float<T>(static_cast<float>(codes[row * ldc + e]) * s);
   }
 }
 

@@ -59,22 +59,31 @@ int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* wh
   if (p.gain) vec = vec && rows_aligned(p.gain, p.gain_stride, 4, 16);
   if (p.shift) vec = vec && rows_aligned(p.shift, p.shift_stride, 4, 16);
   if (p.total) vec = vec && aligned(p.total, 16);
+  int dev, sms;
+  if (int e = current_device(&dev)) return e;
+  if (int e = sm_count(dev, &sms)) return e;
   return by_dtype(dtype, true, what, [&](auto tag) {
     using T = decltype(tag);
-    const dim3 grid(static_cast<unsigned>(p.rows));
-    const auto go = [&](void (*kernel)(const Row8Params), int groups, int vpt) {
+    // as many CTAs as run at once (2,048 threads and 64 K registers of an SM), each with its share of the rows
+    const auto go = [&](void (*kernel)(const Row8Params), int groups, int vpt, int regs) {
       const int threads = (((groups + vpt - 1) / vpt) + 31) / 32 * 32;
+      const int ctas = std::max(1, std::min({2048 / threads, 65536 / (threads * regs), 32}));
+      const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p.rows, static_cast<int64_t>(sms) * ctas)));
       return cuda_status(launch_kernel(kernel, grid, dim3(threads), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
     };
     if (vec && p.h <= kRow8MaxVec) {
       const int groups = p.h / 8;
-      if (groups <= 256) return go(row8_kernel<T, OP, 8, 1>, groups, 1);
-      if (groups <= 1024) return go(row8_kernel<T, OP, 8, 2>, groups, 2);
-      return go(row8_kernel<T, OP, 8, 4>, groups, 4);
+      // few rows: as many threads as a row has vectors, for the latency; many: four vectors a thread, so that the
+      // reductions' instructions are shared by more elements
+      if (groups <= 256 && p.rows <= 8 * sms) return go(row8_kernel<T, OP, 8, 1, 256, 4>, groups, 1, 64);
+      if (groups <= 64) return go(row8_kernel<T, OP, 8, 2, 512, 1>, groups, 2, 128);
+      if (groups <= 2048) return go(row8_kernel<T, OP, 8, 4, 512, 1>, groups, 4, 128);
+      return go(row8_kernel<T, OP, 8, 4, 1024, 1>, groups, 4, 64);
     }
-    if (p.h <= 1024) return go(row8_kernel<T, OP, 1, 4>, p.h, 4);
-    if (p.h <= kRow8MaxScalar) return go(row8_kernel<T, OP, 1, 16>, p.h, 16);
-    return go(row8_long_kernel<T, OP>, 1024, 1);
+    if (p.h <= 1024) return go(row8_kernel<T, OP, 1, 4, 256, 4>, p.h, 4, 64);
+    if (p.h <= kRow8MaxScalar) return go(row8_kernel<T, OP, 1, 16, 1024, 1>, p.h, 16, 64);
+    const dim3 grid(static_cast<unsigned>(p.rows));
+    return cuda_status(launch_kernel(row8_long_kernel<T, OP>, grid, dim3(1024), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
   });
 }
 
@@ -362,14 +371,15 @@ int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t 
                   void* out, void* stream) {
   if (int e = check_rows8(rows, h, out, h, codes, ldc, scale, "dequant8")) return e;
   if (rows == 0) return ok();
-  const bool vec = h % 8 == 0 && rows_aligned(codes, ldc, 1, 8) && aligned(out, 16);
+  const bool vec = h % 16 == 0 && rows_aligned(codes, ldc, 1, 16) && aligned(out, 16);
   return by_dtype(dtype, true, "dequant8", [&](auto tag) {
     using T = decltype(tag);
-    const int per = vec ? 2048 : 256;
-    const dim3 grid((h + per - 1) / per, static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
-    const auto kernel = vec ? dequant8_kernel<T, 8> : dequant8_kernel<T, 1>;
-    return cuda_status(launch_kernel(kernel, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), 1, codes, ldc, scale,
-                                     static_cast<T*>(out), rows, h))
+    const int per = vec ? h / 16 : h;
+    const int64_t total = rows * per, blocks = (total + 255) / 256;
+    if (blocks > 0x7fffffffLL) return fail(W4A4_ERR_UNSUPPORTED, "dequant8: too many values");
+    const auto kernel = vec ? dequant8_kernel<T, 16> : dequant8_kernel<T, 1>;
+    return cuda_status(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream),
+                                     1, codes, ldc, scale, static_cast<T*>(out), total, per, h))
                ? W4A4_ERR_CUDA
                : ok();
   });
