@@ -45,7 +45,7 @@ struct Attn8Params {
   const float* ks;
   const float* vs;
   const int32_t* lengths;
-  float* part_o;           // [batch * heads][splits][rows][width]
+  float* part_o;           // [batch * heads][splits][rows][width], 16-byte chunk c of row r at c ^ (r & 7)
   float2* part_ml;         // [batch * heads][splits][rows]
   long long qb, qt, qh;    // query strides (elements)
   long long cb, ct, ch;    // cache strides
@@ -98,7 +98,8 @@ __device__ __forceinline__ float move_vref(float vsc, float& vref) {
 }
 __device__ __forceinline__ float vscale_ratio(float vsc, float vref) {
   if (vsc == 0.f) return 0.f;
-  return vsc <= 3.4028234e38f ? __fdividef(vsc, vref) : __uint_as_float(0x7fc00000u);
+  if (!(vsc <= 3.4028234e38f)) return __uint_as_float(0x7fc00000u);
+  return vref >= 1e-30f ? __fdividef(vsc, vref) : vsc / vref;  // the quick division wants a normal divisor
 }
 // p times the ratio; keys that are not seen (p = 0) add nothing whatever it is.
 __device__ __forceinline__ float weigh(float p, float rv) { return p == 0.f ? 0.f : p * rv; }
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
       if (e == 0) warp_ml[C::kWarps * C::kRowsMax + r] = make_float2(mm, sum);
     } else {
       const long long at = (static_cast<long long>(unit) * p.splits + split) * p.rows + r;
-      *reinterpret_cast<float4*>(p.part_o + at * D + e) = acc;
+      *reinterpret_cast<float4*>(p.part_o + at * D + ((e / 4) ^ (r & 7)) * 4) = acc;
       if (e == 0) p.part_ml[at] = make_float2(mm, sum);
     }
   }
@@ -550,32 +551,44 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
 
 // ------------------------------------------------------ many rows (> 16)
 // tcgen05: a CTA takes 128 rows (t, g) of one key/value head and a range of
-// its keys, in tiles of 64.  The codes become fp16 in shared memory once per
-// tile and CTA, by eight warps of their own:
-//   warps 0-3   softmax (thread = row = TMEM lane) and the epilogue
-//   warp 4      issues S = Q K^T (M 128, N 64) and O += P V (M 128, N D)
-//   warps 5-8   keys:   16 codes a load -> K-major rows, 128-byte swizzle
-//   warps 9-12  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
-//               permutes), as the second product wants its B operand K-major
-// K and V^T tiles, scores and P are double buffered; O stays in TMEM.  Each
-// converter loads its part of the next tile into registers before it waits
-// for the buffer that the current one goes to.
-// At D = 256 a tile costs the tensor pipe 1024 cycles, the exponentials (16 a
-// cycle) 512, and the conversion about 400 issue slots on each SM
-// sub-partition, so the products bound it.
+// its keys, in tiles of 64.  Q lies in TMEM, as the A operand of S = Q K^T (from
+// shared memory its reads alone would take the products' time again).  The
+// codes become fp16 in shared memory once per tile and CTA, by eight warps of
+// their own:
+//   warps 0-7    softmax and epilogue: two warps to a quarter of the TMEM lanes
+//                (thread = row), each with half of a tile's keys; they agree on
+//                the row maximum through shared memory
+//   warp 8       issues S = Q K^T (M 128, N 64) and O += P V (M 128, N D)
+//   warps 9-12   keys:   16 codes a load -> K-major rows, 128-byte swizzle
+//   warps 13-16  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
+//                permutes), as the second product wants its B operand K-major
+// K and V^T tiles and scores are double buffered; P(i) takes the place of S(i)
+// in TMEM (the MMAs run in the order they are issued, and S(i + 2) is issued
+// after P(i) V); O stays in TMEM.  Each converter loads its part of the next
+// tile into registers before it waits for the buffer that the current one goes
+// to.  At D = 256 a tile costs the tensor pipe 1024 cycles, the exponentials
+// (16 a cycle) 512, and each SM sub-partition about 1100 issue slots
+// (conversion 700, softmax 400), which bounds it.
 template <int D>
 struct Attn8Many {
   static constexpr int kRows = 128, kKeys = 64;
   static constexpr int kSlices = D / 64;
   static constexpr int kQBytes = kRows * D * 2;
   static constexpr int kKBytes = kKeys * D * 2, kVBytes = D * kKeys * 2;
-  static constexpr int kThreads = 13 * 32;
-  static constexpr int kNumBars = 17;
-  static constexpr int kNeed = kQBytes + 2 * (kKBytes + kVBytes) + kRows * 8 + kNumBars * 8 + 16 + 1024;
+  static constexpr int kSoftWarps = 8, kThreads = 17 * 32;
+  static constexpr int kNumBars = 20;
+  // Q as it comes (the partial O of a split later begins there too), K and V^T
+  // rings, row data: score factor, keys seen; maxima and sums of both halves
+  static constexpr int kRing = kQBytes + 2 * (kKBytes + kVBytes);
+  static constexpr int kNeed = kRing + kRows * 8 + 2 * 2 * kRows * 4 + kNumBars * 8 + 16 + 1024;
   static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
   static constexpr int kSmem = kNeed > kOneCtaSmem ? kNeed : kOneCtaSmem;
-  static constexpr uint32_t kOCol = 0, kSCol = D, kPCol = D + 128;
+  static constexpr uint32_t kOCol = 0, kQCol = D, kSCol = D == 64 ? 128 : D + D / 2;
 };
+
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(const __grid_constant__ Attn8Params p) {
@@ -583,11 +596,12 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   extern __shared__ uint8_t many_smem[];
   uint8_t* base =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* q_smem = base;                       // [slices][128 rows][128 B]
+  uint8_t* q_smem = base;                       // [128 rows][2 D B], 16-byte chunk c of row r at c ^ (r & 7)
   uint8_t* k_ring = base + C::kQBytes;          // [2][slices][64 rows][128 B]
   uint8_t* v_ring = k_ring + 2 * C::kKBytes;    // [2][D rows][128 B]
-  float2* row_info = reinterpret_cast<float2*>(v_ring + 2 * C::kVBytes);  // score factor, keys seen
-  uint64_t* bars = reinterpret_cast<uint64_t*>(row_info + C::kRows);
+  float2* row_info = reinterpret_cast<float2*>(v_ring + 2 * C::kVBytes);  // amax of Q's halves; score factor, keys seen
+  float* row_x = reinterpret_cast<float*>(row_info + C::kRows);           // [2 tiles][2 halves][128 rows]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_x + 2 * 2 * C::kRows);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const auto bar_kfull = [&](int s) { return smem_addr(bars + s); };
@@ -595,10 +609,10 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   const auto bar_vfull = [&](int s) { return smem_addr(bars + 4 + s); };
   const auto bar_vempty = [&](int s) { return smem_addr(bars + 6 + s); };
   const auto bar_sfull = [&](int s) { return smem_addr(bars + 8 + s); };
-  const auto bar_sfree = [&](int s) { return smem_addr(bars + 10 + s); };
-  const auto bar_pfull = [&](int s) { return smem_addr(bars + 12 + s); };
-  const auto bar_pfree = [&](int s) { return smem_addr(bars + 14 + s); };
-  const uint32_t bar_o = smem_addr(bars + 16);
+  const auto bar_pfull = [&](int s) { return smem_addr(bars + 10 + s); };
+  const auto bar_pfree = [&](int s) { return smem_addr(bars + 12 + s); };
+  const auto bar_pair = [&](int q) { return smem_addr(bars + 14 + q); };  // the two warps of a quarter
+  const uint32_t bar_o = smem_addr(bars + 18), bar_q = smem_addr(bars + 19);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.y, unit = blockIdx.z;
@@ -615,19 +629,24 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
       mbar_init(bar_vfull(s), 4);
       mbar_init(bar_vempty(s), 1);
       mbar_init(bar_sfull(s), 1);
-      mbar_init(bar_sfree(s), 4);
-      mbar_init(bar_pfull(s), 4);
+      mbar_init(bar_pfull(s), C::kSoftWarps);
       mbar_init(bar_pfree(s), 1);
     }
+    for (int q = 0; q < 4; ++q) mbar_init(bar_pair(q), 2);
     mbar_init(bar_o, 1);
+    mbar_init(bar_q, C::kSoftWarps);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 4) {
+  if (warp == 8) {
     tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
     tmem_relinquish();
   }
   pdl_wait();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
   const int n = min(max(p.lengths[b], 0), p.capacity);
   // the tile's keys: those its last row sees (an earlier row never sees more)
   const int last = min(p.rows, r0 + C::kRows) - 1;
@@ -637,81 +656,22 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   const int tile0 = min(ntiles, split * per), nt = min(ntiles, tile0 + per) - tile0;
   const int nblocks = (n + kKvBlock - 1) / kKvBlock;  // blocks with a scale
 
-  // ---- Q: a row per warp and step, fp16, 128-byte swizzle
-  {
-    constexpr int E = D / 32;  // elements of a lane: 2, 4 or 8
-    constexpr int kSteps = (C::kRows + 12) / 13;
-    uint32_t raw[kSteps][E / 2];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int r = r0 + warp + 13 * i;
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) raw[i][e] = 0u;
-      if (warp + 13 * i < C::kRows && r < p.rows) {
-        const T* src = static_cast<const T*>(p.q) + b * p.qb + (r / p.group) * p.qt +
-                       (h * p.group + r % p.group) * p.qh + lane * E;
-        if constexpr (E == 8) *reinterpret_cast<uint4*>(raw[i]) = *reinterpret_cast<const uint4*>(src);
-        else if constexpr (E == 4) *reinterpret_cast<uint2*>(raw[i]) = *reinterpret_cast<const uint2*>(src);
-        else raw[i][0] = *reinterpret_cast<const uint32_t*>(src);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int row = warp + 13 * i;
-      if (row >= C::kRows) break;
-      float v[E];
-      uint32_t key = 0;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        v[e] = to_float(reinterpret_cast<const T*>(raw[i])[e]);
-        key = max(key, abs_key(v[e]));
-      }
-      key = __reduce_max_sync(0xffffffffu, key);
-      const float shift = query_shift(__uint_as_float(key));
-      const float up = p.scale < 0.f ? -shift : shift;
-      uint32_t w[E / 2];
-#pragma unroll
-      for (int e = 0; e < E; e += 2) w[e / 2] = pack_half2_bits(v[e] * up, v[e + 1] * up);
-      const int byte = lane * E * 2;  // in the row of D fp16
-      uint8_t* dst = q_smem + (byte >> 7) * (C::kRows * 128) + row * 128 + (((((byte >> 4) & 7) ^ (row & 7)) << 4) | (byte & 15));
-      if constexpr (E == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w);
-      else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w);
-      else *reinterpret_cast<uint32_t*>(dst) = w[0];
-      if (lane == 0) {
-        const int r = r0 + row;
-        row_info[row] =
-            make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, r / p.group) : 0));
-      }
-    }
-  }
-  fence_proxy_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-
-  if (warp == 4) {
+  if (warp == 8) {
     // ------------------------------------------------ MMA issuer (one elected lane)
     const bool issuer = elect_one();
     const uint32_t idesc_s = idesc_f16(C::kRows, C::kKeys);
     const uint32_t idesc_o = idesc_f16(C::kRows, D);
-    const uint64_t qdesc = smem_desc_sw128(smem_addr(q_smem));
     const auto issue_s = [&](int i) -> bool {
       const int slot = i & 1;
-      bool ok = mbar_wait_spin(bar_kfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit);
-      if (ok && i >= 2)
-        ok = mbar_wait_spin(bar_sfree(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit);
-      if (!warp_all(ok)) return false;
+      if (!warp_all(mbar_wait_spin(bar_kfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit))) return false;
       tc_fence_after();
       const uint64_t kdesc = smem_desc_sw128(smem_addr(k_ring + slot * C::kKBytes));
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint64_t off = static_cast<uint64_t>((kk & 3) * 2);
+      for (int kk = 0; kk < D / 16; ++kk)
         if (issuer)
-          umma_f16_ss(tmem_base + C::kSCol + slot * C::kKeys,
-                      qdesc + static_cast<uint64_t>((kk >> 2) * (C::kRows * 128) >> 4) + off,
-                      kdesc + static_cast<uint64_t>((kk >> 2) * (C::kKeys * 128) >> 4) + off, idesc_s, kk > 0);
-      }
+          umma_f16_ts(tmem_base + C::kSCol + slot * C::kKeys, tmem_base + C::kQCol + 8 * kk,
+                      kdesc + static_cast<uint64_t>((kk >> 2) * (C::kKeys * 128) >> 4) + static_cast<uint64_t>((kk & 3) * 2),
+                      idesc_s, kk > 0);
       if (issuer) {
         umma_commit(bar_kempty(slot));
         umma_commit(bar_sfull(slot));
@@ -719,7 +679,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
       __syncwarp();
       return true;
     };
-    bool alive = nt > 0 && issue_s(0);
+    bool alive = nt > 0 && warp_all(mbar_wait_spin(bar_q, 0, abort_flag, err, kErrWaitUnpack, limit)) && issue_s(0);
     for (int i = 0; alive && i < nt; ++i) {
       if (i + 1 < nt && !(alive = issue_s(i + 1))) break;
       const int slot = i & 1;
@@ -734,7 +694,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
 #pragma unroll
       for (int kk = 0; kk < C::kKeys / 16; ++kk)
         if (issuer)
-          umma_f16_ts(tmem_base + C::kOCol, tmem_base + C::kPCol + slot * 32 + 8 * kk,
+          umma_f16_ts(tmem_base + C::kOCol, tmem_base + C::kSCol + slot * C::kKeys + 8 * kk,
                       vdesc + static_cast<uint64_t>(kk * 2), idesc_o, (i | kk) != 0);
       if (issuer) {
         umma_commit(bar_vempty(slot));
@@ -746,24 +706,24 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
     __syncwarp();
     volatile int no_abort = 0;
     mbar_wait_bounded(bar_o, 0, &no_abort, err, kErrWaitDrain, limit);
-  } else if (warp >= 9) {
+  } else if (warp >= 13) {
     // ------------------------------------------------ values -> V^T (fp16)
     constexpr int W = D / 64;  // words of a lane's run of dims: 1, 2 or 4
     const int kc = lane & 7;   // keys 8 kc .. 8 kc + 7 of a tile
-    const int dim0 = (warp - 9) * (D / 4) + (lane >> 3) * (D / 16);
+    const int dim0 = (warp - 13) * (D / 4) + (lane >> 3) * (D / 16);
     const int8_t* src = p.v + b * p.cb + h * p.ch + dim0;
     uint32_t w[8][W];
     const auto load = [&](int i) {
       const int j0 = (tile0 + i) * C::kKeys + 8 * kc;
+      const int8_t* a = src + static_cast<long long>(j0) * p.ct;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
 #pragma unroll
         for (int x = 0; x < W; ++x) w[k][x] = 0u;
         if (j0 + k < n) {
-          const int8_t* a = src + static_cast<long long>(j0 + k) * p.ct;
-          if constexpr (W == 4) *reinterpret_cast<uint4*>(w[k]) = __ldg(reinterpret_cast<const uint4*>(a));
-          else if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = __ldg(reinterpret_cast<const uint2*>(a));
-          else w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(a));
+          if constexpr (W == 4) *reinterpret_cast<uint4*>(w[k]) = __ldg(reinterpret_cast<const uint4*>(a + k * p.ct));
+          else if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = __ldg(reinterpret_cast<const uint2*>(a + k * p.ct));
+          else w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(a + k * p.ct));
         }
       }
     };
@@ -799,20 +759,19 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_vfull(slot));
     }
-  } else if (warp >= 5) {
+  } else if (warp >= 9) {
     // ------------------------------------------------ keys -> K (fp16)
     constexpr int U = 2 * C::kSlices;  // (8 keys x 64 dims) units of a warp
     const int kr = lane >> 2, c4 = lane & 3;
-    const int8_t* src = p.k + b * p.cb + h * p.ch;
+    const int8_t* src = p.k + b * p.cb + h * p.ch + 16 * c4;
     uint4 w[U];
     const auto load = [&](int i) {
       const int j0 = (tile0 + i) * C::kKeys + kr;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int id = warp - 5 + 4 * u, j = j0 + 8 * (id / C::kSlices);
+        const int id = warp - 9 + 4 * u, j = j0 + 8 * (id / C::kSlices);
         w[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < n)
-          w[u] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(j) * p.ct + 64 * (id % C::kSlices) + 16 * c4));
+        if (j < n) w[u] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(j) * p.ct + 64 * (id % C::kSlices)));
       }
     };
     if (nt > 0) load(0);
@@ -822,7 +781,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
         break;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int id = warp - 5 + 4 * u, row = 8 * (id / C::kSlices) + kr;
+        const int id = warp - 9 + 4 * u, row = 8 * (id / C::kSlices) + kr;
         uint8_t* dst = k_ring + slot * C::kKBytes + (id % C::kSlices) * (C::kKeys * 128) + row * 128;
         const uint32_t x[4] = {w[u].x ^ 0x80808080u, w[u].y ^ 0x80808080u, w[u].z ^ 0x80808080u, w[u].w ^ 0x80808080u};
 #pragma unroll
@@ -837,61 +796,100 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
       if (lane == 0) mbar_arrive(bar_kfull(slot));
     }
   } else {
-    // ------------------------------------------------ softmax + epilogue (warps 0-3)
-    const int row = warp * 32 + lane;
-    const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+    // ------------------------------------------------ softmax + epilogue (warps 0-7)
+    const int quarter = warp & 3, half = warp >> 2;
+    const int row = quarter * 32 + lane, r = r0 + row;
+    const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
+    // ---- Q: raw rows to shared memory, then (thread = row and half of its dims) to TMEM as fp16
+    {
+      constexpr int QC = D * 2 / 16;  // chunks of a row
+      for (int i = warp; i < C::kRows; i += C::kSoftWarps) {
+        const int tok = (r0 + i) / p.group, g = (r0 + i) - tok * p.group;
+        const T* src = static_cast<const T*>(p.q) + b * p.qb + tok * p.qt + (h * p.group + g) * p.qh + lane * 8;
+        const uint32_t dst = smem_addr(q_smem) + i * 2 * D + ((lane ^ (i & 7)) << 4);
+        if (lane < QC) {
+          if (r0 + i < p.rows) cp_async16(dst, src);
+          else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
+        }
+      }
+      cp_async_commit();
+      cp_async_wait<0>();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the 8 softmax warps (nothing has given up yet)
+      const uint8_t* mine = q_smem + row * 2 * D;
+      uint32_t key = 0;
+#pragma unroll 4
+      for (int c = half * (QC / 2); c < (half + 1) * (QC / 2); ++c) {
+        float v[8];
+        load8(reinterpret_cast<const T*>(mine + ((c ^ (row & 7)) << 4)), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) key = max(key, abs_key(v[e]));
+      }
+      row_x[half * C::kRows + row] = __uint_as_float(key);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const uint32_t amax = max(abs_key(row_x[row]), abs_key(row_x[C::kRows + row]));
+      const float shift = query_shift(__uint_as_float(amax));
+      const float up = p.scale < 0.f ? -shift : shift;
+      if (half == 0)
+        row_info[row] = make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, r / p.group) : 0));
+#pragma unroll 1
+      for (int c = half * (QC / 2); c < (half + 1) * (QC / 2); c += 4) {
+        uint32_t w[16];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          float v[8];
+          load8(reinterpret_cast<const T*>(mine + (((c + x) ^ (row & 7)) << 4)), v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[4 * x + e] = pack_half2_bits(v[2 * e] * up, v[2 * e + 1] * up);
+        }
+        tmem_st_32x32b_x16(tmem_base + lane_addr + C::kQCol + 4 * c, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_info, and row_x may be written again
+      if (lane == 0) mbar_arrive(bar_q);
+    }
     const float2 info = row_info[row];
     const float factor = info.x;
     const int seen = __float_as_int(info.y);
     const float* ks = p.ks + static_cast<long long>(unit) * (p.capacity / kKvBlock);
     const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
-    float m = -INFINITY, l = 0.f, vref = 0.f;
+    float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;
     bool alive = true;
-    for (int i = 0; alive && i < nt; ++i) {
+    for (int i = 0; i < nt; ++i) {
       const int slot = i & 1, j0 = (tile0 + i) * C::kKeys, blk = j0 / kKvBlock;
-      float ksc[4], vsc[4];
+      float ksc[2], vsc[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const bool has = blk + q < nblocks;
-        ksc[q] = has ? __ldg(ks + blk + q) : 0.f;
-        vsc[q] = has ? __ldg(vs + blk + q) : 0.f;
-      }
+      for (int q = 0; q < 4; ++q) vsc[q] = blk + q < nblocks ? __ldg(vs + blk + q) : 0.f;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) ksc[q] = blk + 2 * half + q < nblocks ? __ldg(ks + blk + 2 * half + q) : 0.f;
       if (!warp_all(mbar_wait_spin(bar_sfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
         alive = false;
         break;
       }
       tc_fence_after();
-      uint32_t raw[64];
+      uint32_t raw[32];
       {
-        const uint32_t t = tmem_base + lane_addr + C::kSCol + slot * C::kKeys;
+        const uint32_t t = tmem_base + lane_addr + C::kSCol + slot * C::kKeys + 32 * half;
         tmem_ld_32x32b_x16(t, *reinterpret_cast<uint32_t(*)[16]>(&raw[0]));
         tmem_ld_32x32b_x16(t + 16, *reinterpret_cast<uint32_t(*)[16]>(&raw[16]));
-        tmem_ld_32x32b_x16(t + 32, *reinterpret_cast<uint32_t(*)[16]>(&raw[32]));
-        tmem_ld_32x32b_x16(t + 48, *reinterpret_cast<uint32_t(*)[16]>(&raw[48]));
         tmem_ld_wait();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_sfree(slot));
       // unseen keys of a row's last tiles: -inf, whatever their block's scale is
       float bmax = -INFINITY;
-      const int left = seen - j0;
-      if (left >= C::kKeys) {
+      const int left = seen - j0 - 32 * half;
+      const bool whole = __all_sync(0xffffffffu, left >= 32);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < 2; ++q) {
+        ksc[q] *= factor;
+        if (whole) {
           float x = -INFINITY, y = -INFINITY;
 #pragma unroll
           for (int c = 0; c < 16; c += 2) {
             x = fmaxf(x, __uint_as_float(raw[16 * q + c]));
             y = fmaxf(y, __uint_as_float(raw[16 * q + c + 1]));
           }
-          ksc[q] *= factor;
           bmax = fmaxf(bmax, fmaxf(x, y) * ksc[q]);  // the factor is not negative
-        }
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          ksc[q] *= factor;
+        } else {
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
             const float v = 16 * q + c < left ? __uint_as_float(raw[16 * q + c]) * ksc[q] : -INFINITY;
@@ -901,24 +899,37 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
           ksc[q] = 1.f;
         }
       }
+      // the row's maximum over both halves (both warps have read their scores: P may take their place)
+      row_x[(slot * 2 + half) * C::kRows + row] = bmax;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_pair(quarter));
+      if (!warp_all(mbar_wait_spin(bar_pair(quarter), i & 1, abort_flag, err, kErrWaitAccum, limit))) {
+        alive = false;
+        break;
+      }
+      bmax = fmaxf(bmax, row_x[(slot * 2 + (half ^ 1)) * C::kRows + row]);
       float f = 1.f;
-      const bool grow = bmax > m + kAttn8Grow;
-      if (grow) {
+      if (bmax > m + kAttn8Grow) {
         f = m == -INFINITY ? 0.f : ex2_approx(m - bmax);
         m = bmax;
         l *= f;
       }
+      const float vmax = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));  // passes NaN by
+      if (vmax > kAttn8VGrow * vref) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) f *= move_vref(vsc[q], vref);
+        for (int q = 0; q < 4; ++q) f *= move_vref(vsc[q], vref);
+        vinv = vref >= 1e-30f ? __fdividef(1.f, vref) : 0.f;
+      }
       if (i >= 1 && __any_sync(0xffffffffu, f != 1.f)) {
-        // O holds the earlier tiles: wait for the last of them, rescale this warp's rows
+        // O holds the earlier tiles: wait for the last of them, rescale this warp's rows and half of the columns
         if (!warp_all(mbar_wait_spin(bar_pfree((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
           alive = false;
           break;
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = 0; c0 < D; c0 += 16) {
+        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
           uint32_t o[16];
           const uint32_t t = tmem_base + lane_addr + C::kOCol + c0;
           tmem_ld_32x32b_x16(t, o);
@@ -930,129 +941,154 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
         tmem_st_wait();
       }
       const float nm = m == -INFINITY ? 0.f : -m;
-      uint32_t pw[32];
+      uint32_t pw[16];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float rv = vscale_ratio(vsc[q], vref);
-        float s2[2] = {0.f, 0.f};
+      for (int q = 0; q < 2; ++q) {
+        const float v = vsc[2 * half + q];
+        const float rv = vinv > 0.f ? v * vinv : vscale_ratio(v, vref);
+        float2 sum = make_float2(0.f, 0.f);
+        const float2 kk = make_float2(ksc[q], ksc[q]), mm = make_float2(nm, nm), rr = make_float2(rv, rv);
+        if (v <= 3.4028234e38f) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float p0 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c]), ksc[q], nm));
-          const float p1 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c + 1]), ksc[q], nm));
-          s2[0] += p0;
-          s2[1] += p1;
-          pw[8 * q + c] = pack_half2_bits(weigh(p0, rv), weigh(p1, rv));
+          for (int c = 0; c < 8; ++c) {
+            const float2 x = __ffma2_rn(
+                make_float2(__uint_as_float(raw[16 * q + 2 * c]), __uint_as_float(raw[16 * q + 2 * c + 1])), kk, mm);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum = __fadd2_rn(sum, e);
+            const float2 w = __fmul2_rn(e, rr);
+            pw[8 * q + c] = pack_half2_bits(w.x, w.y);
+          }
+        } else {  // a block with an infinity or NaN: rows that see it become NaN, others stay clean
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const float e0 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c]), ksc[q], nm));
+            const float e1 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c + 1]), ksc[q], nm));
+            sum.x += e0;
+            sum.y += e1;
+            const float nan = __uint_as_float(0x7fc00000u);
+            pw[8 * q + c] = pack_half2_bits(weigh(e0, nan), weigh(e1, nan));
+          }
         }
-        l += s2[0] + s2[1];
-      }
-      if (i >= 2 && !warp_all(mbar_wait_spin(bar_pfree(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
-        alive = false;
-        break;
+        l += sum.x + sum.y;
       }
       tc_fence_after();
-      tmem_st_32x32b_x32(tmem_base + lane_addr + C::kPCol + slot * 32, pw);
+      tmem_st_32x32b_x16(tmem_base + lane_addr + C::kSCol + slot * C::kKeys + 16 * half, pw);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_pfull(slot));
     }
-    // ---- epilogue: O vref / l, or the unnormalised O with (m, l)
-    const bool ok = alive && warp_all(mbar_wait_bounded(bar_o, 0, abort_flag, err, kErrWaitAccum, limit));
+    // ---- epilogue: O vref / l as T, or the unnormalised O vref and (m, l) of this split, to shared memory (the
+    // Q buffer and the idle rings)
+    alive = alive && warp_all(mbar_wait_bounded(bar_o, 0, abort_flag, err, kErrWaitAccum, limit));
     tc_fence_after();
-    const int r = r0 + row;
+    row_x[half * C::kRows + row] = l;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_pair(quarter));
+    alive = warp_all(mbar_wait_spin(bar_pair(quarter), nt & 1, abort_flag, err, kErrWaitAccum, limit)) && alive;
+    l += row_x[(half ^ 1) * C::kRows + row];
     const bool part = p.splits > 1;
     const float f = part ? vref : l == 0.f ? 0.f : vref / l;
-    const long long at = (static_cast<long long>(unit) * p.splits + split) * p.rows + r;
-    const int head = h * p.group + r % p.group;
-    T* dst = static_cast<T*>(p.out) +
-             ((static_cast<long long>(b) * p.tokens + r / p.group) * (p.heads * p.group) + head) * D;
-    if (ok && part && r < p.rows) p.part_ml[at] = make_float2(m, l);
+    if (part && half == 0 && r < p.rows)
+      p.part_ml[(static_cast<long long>(unit) * p.splits + split) * p.rows + r] = make_float2(m, alive ? l : __uint_as_float(0x7fc00000u));
 #pragma unroll 1
-    for (int c0 = 0; c0 < D; c0 += 16) {
+    for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
       uint32_t o[16];
-      if (ok && nt > 0) {
+      if (nt > 0) {
         tmem_ld_32x32b_x16(tmem_base + lane_addr + C::kOCol + c0, o);
         tmem_ld_wait();
       } else {
 #pragma unroll
         for (int c = 0; c < 16; ++c) o[c] = 0u;
       }
-      if (!ok || r >= p.rows) continue;
-      // a row that saw nothing (l = 0) has P = 0 for every key
       float v[2][8];
 #pragma unroll
       for (int c = 0; c < 16; ++c) v[c >> 3][c & 7] = f == 0.f ? 0.f : __uint_as_float(o[c]) * f;
+      if (part) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        if (part) store8(p.part_o + at * D + c0 + 8 * c, v[c]);
-        else store8(dst + c0 + 8 * c, v[c]);
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<float4*>(base + row * 4 * D + (((c0 / 4 + c) ^ (row & 7)) << 4)) =
+              make_float4(v[c >> 1][4 * (c & 1)], v[c >> 1][4 * (c & 1) + 1], v[c >> 1][4 * (c & 1) + 2], v[c >> 1][4 * (c & 1) + 3]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          store8(reinterpret_cast<T*>(base + row * 2 * D + (((c0 / 8 + c) ^ (row & 7)) << 4)), v[c]);
       }
     }
+    fence_proxy_async_smem();
   }
   // every MMA has completed (the issuer waited for bar_o) before TMEM is freed
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
+  const int rows = min(C::kRows, p.rows - r0);
+  if (p.splits > 1) {
+    // the rows lie in the workspace as in shared memory (chunk c of row r at c ^ (r & 7)): one copy
+    if (threadIdx.x == 0) {
+      bulk_store(p.part_o + ((static_cast<long long>(unit) * p.splits + split) * p.rows + r0) * D, smem_addr(base),
+                 static_cast<uint32_t>(rows) * 4 * D);
+      bulk_commit_group();
+      bulk_wait_group0();
+    }
+  } else {
+    constexpr int QC = D * 2 / 16;
+    for (int i = warp; i < rows; i += C::kThreads / 32)
+      if (lane < QC)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row(p, b, h, r0 + i) * D + lane * 8) =
+            *reinterpret_cast<const uint4*>(base + i * 2 * D + ((lane ^ (i & 7)) << 4));
+  }
 }
 
-// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one CTA of 4 warps
-// per row, each warp every fourth part; the parts' O and (m, l) are loaded
-// together (at most 256 parts: 64 a warp).
+// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one CTA of 128
+// threads per row, a thread with one 16-byte chunk of every (512 / D)-th part
+// (chunk c of row r lies at c ^ (r & 7)).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn8_join_kernel(const __grid_constant__ Attn8Params p) {
-  __shared__ float red[4][D];
-  __shared__ float2 red_ml[4];
+  constexpr int NC = D / 4, G = 128 / NC;
+  __shared__ float4 red[G][NC];
+  __shared__ float2 red_ml[G];
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = threadIdx.x % NC, g = threadIdx.x / NC;
   const int r = blockIdx.x, unit = blockIdx.y;
-  constexpr int V = D / 32;  // elements of a lane: 2, 4 or 8
   const long long first = static_cast<long long>(unit) * p.splits * p.rows + r;
-  float acc[V] = {};
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   float m = -INFINITY, sum = 0.f;
 #pragma unroll 4
-  for (int s = warp; s < p.splits; s += 4) {
-    const float2 ml = p.part_ml[first + static_cast<long long>(s) * p.rows];
-    const float* src = p.part_o + (first + static_cast<long long>(s) * p.rows) * D + lane * V;
-    float v[V];
-    if constexpr (V == 2) *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-    else {
-#pragma unroll
-      for (int j = 0; j < V; j += 4) *reinterpret_cast<float4*>(&v[j]) = *reinterpret_cast<const float4*>(src + j);
-    }
+  for (int s = g; s < p.splits; s += G) {
+    const long long at = first + static_cast<long long>(s) * p.rows;
+    const float2 ml = p.part_ml[at];
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + (c ^ (r & 7)) * 4);
     if (ml.y == 0.f) continue;  // saw nothing (a NaN stays)
     const float mn = fmaxf(m, ml.x);
     const float fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fn = ex2_approx(ml.x - mn);
     m = mn;
     sum = sum * fo + ml.y * fn;
-#pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = acc[j] * fo + v[j] * fn;
+    acc = make_float4(acc.x * fo + v.x * fn, acc.y * fo + v.y * fn, acc.z * fo + v.z * fn, acc.w * fo + v.w * fn);
   }
-#pragma unroll
-  for (int j = 0; j < V; ++j) red[warp][lane * V + j] = acc[j];
-  if (lane == 0) red_ml[warp] = make_float2(m, sum);
+  red[g][c] = acc;
+  if (c == 0) red_ml[g] = make_float2(m, sum);
   __syncthreads();
-  if (threadIdx.x >= D / 4) return;
-  const int e = threadIdx.x * 4;
+  if (g > 0) return;
   float mm = -INFINITY, total = 0.f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) mm = fmaxf(mm, red_ml[w].x);
+  for (int w = 0; w < G; ++w) mm = fmaxf(mm, red_ml[w].x);
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < G; ++w) {
     const float2 ml = red_ml[w];
     if (ml.y == 0.f) continue;
     const float f = ex2_approx(ml.x - mm);
-    x.x = fmaf(red[w][e], f, x.x), x.y = fmaf(red[w][e + 1], f, x.y);
-    x.z = fmaf(red[w][e + 2], f, x.z), x.w = fmaf(red[w][e + 3], f, x.w);
+    const float4 v = red[w][c];
+    x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
     total = fmaf(ml.y, f, total);
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int b = unit / p.heads, h = unit - b * p.heads;
-  store4(static_cast<T*>(p.out) + out_row(p, b, h, r) * D + e, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+  store4(static_cast<T*>(p.out) + out_row(p, b, h, r) * D + 4 * c, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
 }  // namespace w4a4
