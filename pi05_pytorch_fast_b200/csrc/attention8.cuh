@@ -13,13 +13,14 @@
 //  * Q in fp16 times a power of two for each row (bf16 queries keep their 8
 //    bits wherever an element is within 2^28 of the row's largest);
 //  * scores, row maxima, row sums and O in fp32, softmax in base 2;
-//  * the running maximum m of a row moves only when a block exceeds it by more
-//    than 2^8, so that O is rarely rescaled; p = 2^(s - m) <= 2^8;
+//  * the reference m of a row is set 2^4 above the maximum so far and moves only
+//    when a block exceeds it by more than 2^11, so that O is rarely rescaled (a
+//    rescale of 128 x 256 takes as long as two tiles): p = 2^(s - m) <= 2^11;
 //  * p vs / vref is rounded to fp16 for the P V product (11 bits, as the
 //    scores' own error after exp2 is not much smaller).  vref, a running
 //    reference for the value scales, moves (and O is rescaled) when a scale
-//    exceeds it by more than 2^4: p vs / vref <= 2^12 fits fp16, and what
-//    falls below its range is below 2^-24 of the row's largest term.
+//    exceeds it by more than 2^4: p vs / vref <= 2^15 fits fp16, and what
+//    falls below its range is below 2^-20 of the row's largest term.
 // When the keys of a head are split over CTAs, each writes its unnormalised O
 // with (m, l) and attn8_join_kernel adds them up.
 #pragma once
@@ -34,7 +35,8 @@ namespace w4a4 {
 // cluster's CTA holds could wait for good, each cluster's other half being
 // blocked by the other.
 constexpr int kOneCtaSmem = 117 * 1024;
-constexpr float kAttn8Grow = 8.f;      // log2 by which a block may exceed m
+constexpr float kAttn8Margin = 4.f;    // log2 by which m is set above a row's maximum
+constexpr float kAttn8Grow = 11.f;     // log2 by which a block may exceed m
 constexpr float kAttn8VGrow = 16.f;    // factor by which a value scale may exceed vref
 
 struct Attn8Params {
@@ -375,6 +377,7 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
       bm[i] = fmaxf(bm[i], __shfl_xor_sync(0xffffffffu, bm[i], 2));
       f[i] = 1.f;
       if (bm[i] > m[i] + kAttn8Grow) {
+        bm[i] += kAttn8Margin;
         f[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm[i]);
         m[i] = bm[i];
         l[i] *= f[i];
@@ -553,37 +556,49 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
 // tcgen05: a CTA takes 128 rows (t, g) of one key/value head and a range of
 // its keys, in tiles of 64.  Q lies in TMEM, as the A operand of S = Q K^T (from
 // shared memory its reads alone would take the products' time again).  The
-// codes become fp16 in shared memory once per tile and CTA, by eight warps of
-// their own:
-//   warps 0-7    softmax and epilogue: two warps to a quarter of the TMEM lanes
-//                (thread = row), each with half of a tile's keys; they agree on
-//                the row maximum through shared memory
-//   warp 8       issues S = Q K^T (M 128, N 64) and O += P V (M 128, N D)
-//   warps 9-12   keys:   16 codes a load -> K-major rows, 128-byte swizzle
-//   warps 13-16  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
+// codes come by TMA and become fp16 in shared memory once per tile and CTA, by
+// eight warps of their own:
+//   warps 0-7    softmax and epilogue (thread = row = TMEM lane): warps 0-3 take
+//                the even tiles, 4-7 the odd ones, so that one group's
+//                exponentials run beside the other's maxima; the running maximum
+//                passes from tile to tile through shared memory
+//   warps 8-11   keys: 16 codes a load -> K-major rows, 128-byte swizzle
+//   warps 12-15  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
 //                permutes), as the second product wants its B operand K-major
-// K and V^T tiles and scores are double buffered; P(i) takes the place of S(i)
-// in TMEM (the MMAs run in the order they are issued, and S(i + 2) is issued
-// after P(i) V); O stays in TMEM.  Each converter loads its part of the next
-// tile into registers before it waits for the buffer that the current one goes
-// to.  At D = 256 a tile costs the tensor pipe 1024 cycles, the exponentials
-// (16 a cycle) 512, and each SM sub-partition about 1100 issue slots
-// (conversion 700, softmax 400), which bounds it.
+//   warp 16      issues S = Q K^T (M 128, N 64) and O += P V (M 128, N D)
+//   warp 17      asks for the codes (TMA, two tiles ahead)
+// Codes, K and V^T tiles and P are double buffered; the one score buffer is
+// free again as soon as its readers have it in registers, so S(i + 2) is under
+// way before P(i) V; O stays in TMEM.  Keys sit in a tile in the order rho =
+// 8 (j % 8) + j / 8: an eighth of the tile's keys lies 8 rows apart in the codes,
+// where the swizzle spreads them over all banks.
+// setmaxnreg moves registers to the softmax warps (of 640 x 96: 256 x 128 for
+// them, 256 x 80 for the converters, 128 x 56 for the rest).
+// At D = 256 a tile costs the tensor pipe 1024 cycles and the exponentials (16 a
+// cycle) 512.
 template <int D>
 struct Attn8Many {
   static constexpr int kRows = 128, kKeys = 64;
   static constexpr int kSlices = D / 64;
   static constexpr int kQBytes = kRows * D * 2;
-  static constexpr int kKBytes = kKeys * D * 2, kVBytes = D * kKeys * 2;
-  static constexpr int kSoftWarps = 8, kThreads = 17 * 32;
-  static constexpr int kNumBars = 20;
-  // Q as it comes (the partial O of a split later begins there too), K and V^T
-  // rings, row data: score factor, keys seen; maxima and sums of both halves
-  static constexpr int kRing = kQBytes + 2 * (kKBytes + kVBytes);
-  static constexpr int kNeed = kRing + kRows * 8 + 2 * 2 * kRows * 4 + kNumBars * 8 + 16 + 1024;
+  static constexpr int kKBytes = kKeys * D * 2, kVBytes = D * kKeys * 2, kRaw = kKeys * D;
+  static constexpr int kSoftWarps = 8, kThreads = 20 * 32;
+  static constexpr int kSoftRegs = 128, kConvRegs = 80, kRestRegs = 56;
+  static constexpr int kPoolRegs = 256 * kSoftRegs + 256 * kConvRegs + 128 * kRestRegs;
+  static constexpr int kNumBars = 33;
+  // K and V^T rings (the raw Q before, and O after the tiles, use them), rings of codes, row data: score factor, keys
+  // seen; sums of both groups; running maxima; the last vref
+  static constexpr int kRing = 2 * (kKBytes + kVBytes);
+  static constexpr int kNeed = kRing + 4 * kRaw + kRows * 8 + 4 * kRows * 4 + kNumBars * 8 + 32 + 1024;
   static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
   static constexpr int kSmem = kNeed > kOneCtaSmem ? kNeed : kOneCtaSmem;
-  static constexpr uint32_t kOCol = 0, kQCol = D, kSCol = D == 64 ? 128 : D + D / 2;
+  static constexpr uint32_t kOCol = 0, kQCol = D, kSCol = D == 64 ? 128 : D + D / 2, kPCol = kSCol + kKeys;
+  static_assert(2 * kKBytes >= kQBytes && kRing >= kRows * D * 4, "Q and O must fit the rings");
+};
+
+struct alignas(64) Attn8ManyParams {
+  CUtensorMap tmap_k, tmap_v;  // int8 {width, heads, capacity, batch}, box {min(width, 128), 1, 64, 1}, swizzle = its width
+  Attn8Params p;
 };
 
 __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
@@ -591,28 +606,41 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(const __grid_constant__ Attn8Params p) {
+__global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
+    attn8_many_kernel(const __grid_constant__ Attn8ManyParams params) {
   using C = Attn8Many<D>;
+  const Attn8Params& p = params.p;
   extern __shared__ uint8_t many_smem[];
   uint8_t* base =
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_smem) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t* q_smem = base;                       // [128 rows][2 D B], 16-byte chunk c of row r at c ^ (r & 7)
-  uint8_t* k_ring = base + C::kQBytes;          // [2][slices][64 rows][128 B]
+  uint8_t* k_ring = base;                       // [2][slices][64 rows][128 B]
+  uint8_t* q_smem = base;                       // (before) [128 rows][2 D B], 16-byte chunk c of row r at c ^ (r & 7)
   uint8_t* v_ring = k_ring + 2 * C::kKBytes;    // [2][D rows][128 B]
-  float2* row_info = reinterpret_cast<float2*>(v_ring + 2 * C::kVBytes);  // amax of Q's halves; score factor, keys seen
-  float* row_x = reinterpret_cast<float*>(row_info + C::kRows);           // [2 tiles][2 halves][128 rows]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(row_x + 2 * 2 * C::kRows);
+  uint8_t* k_raw = v_ring + 2 * C::kVBytes;     // [2][D / 128 (at least 1) boxes][64 keys][128 or 64 B]
+  uint8_t* v_raw = k_raw + 2 * C::kRaw;
+  float2* row_info = reinterpret_cast<float2*>(v_raw + 2 * C::kRaw);      // score factor, keys seen
+  float* row_x = reinterpret_cast<float*>(row_info + C::kRows);           // [2 groups][128 rows]: amax of half of Q, later l
+  float* row_m = row_x + 2 * C::kRows;                                    // running maxima
+  float* row_v = row_m + C::kRows;                                        // the last tile's vref
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_v + C::kRows);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const auto bar_kfull = [&](int s) { return smem_addr(bars + s); };
-  const auto bar_kempty = [&](int s) { return smem_addr(bars + 2 + s); };
-  const auto bar_vfull = [&](int s) { return smem_addr(bars + 4 + s); };
-  const auto bar_vempty = [&](int s) { return smem_addr(bars + 6 + s); };
-  const auto bar_sfull = [&](int s) { return smem_addr(bars + 8 + s); };
-  const auto bar_pfull = [&](int s) { return smem_addr(bars + 10 + s); };
-  const auto bar_pfree = [&](int s) { return smem_addr(bars + 12 + s); };
-  const auto bar_pair = [&](int q) { return smem_addr(bars + 14 + q); };  // the two warps of a quarter
-  const uint32_t bar_o = smem_addr(bars + 18), bar_q = smem_addr(bars + 19);
+  int* plan = reinterpret_cast<int*>(tmem_slot + 2);  // length, first tile, tiles
+  const auto bar_kraw = [&](int s) { return smem_addr(bars + s); };        // codes landed
+  const auto bar_vraw = [&](int s) { return smem_addr(bars + 2 + s); };
+  const auto bar_kread = [&](int s) { return smem_addr(bars + 4 + s); };   // codes read
+  const auto bar_vread = [&](int s) { return smem_addr(bars + 6 + s); };
+  const auto bar_kfull = [&](int s) { return smem_addr(bars + 8 + s); };
+  const auto bar_kempty = [&](int s) { return smem_addr(bars + 10 + s); };
+  const auto bar_vfull = [&](int s) { return smem_addr(bars + 12 + s); };
+  const auto bar_vempty = [&](int s) { return smem_addr(bars + 14 + s); };
+  const auto bar_pfull = [&](int s) { return smem_addr(bars + 16 + s); };
+  const auto bar_pfree = [&](int s) { return smem_addr(bars + 18 + s); };  // P V of that parity's last tile is done
+  const auto bar_m = [&](int q) { return smem_addr(bars + 20 + q); };      // a quarter's maxima of a tile are decided
+  const auto bar_l = [&](int q) { return smem_addr(bars + 24 + q); };      // both groups' sums of a quarter are there
+  // one for each group, as a wait for a phase must not begin before the phase before it has passed
+  const auto bar_sfull = [&](int s) { return smem_addr(bars + 28 + s); };
+  const uint32_t bar_sread = smem_addr(bars + 30), bar_o = smem_addr(bars + 31), bar_q = smem_addr(bars + 32);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.y, unit = blockIdx.z;
@@ -624,114 +652,187 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   pdl_launch_dependents();
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
+      mbar_init(bar_kraw(s), 1);
+      mbar_init(bar_vraw(s), 1);
+      mbar_init(bar_kread(s), 4);
+      mbar_init(bar_vread(s), 4);
       mbar_init(bar_kfull(s), 4);
       mbar_init(bar_kempty(s), 1);
       mbar_init(bar_vfull(s), 4);
       mbar_init(bar_vempty(s), 1);
-      mbar_init(bar_sfull(s), 1);
-      mbar_init(bar_pfull(s), C::kSoftWarps);
+      mbar_init(bar_pfull(s), 4);
       mbar_init(bar_pfree(s), 1);
+      mbar_init(bar_sfull(s), 1);
     }
-    for (int q = 0; q < 4; ++q) mbar_init(bar_pair(q), 2);
+    for (int q = 0; q < 4; ++q) {
+      mbar_init(bar_m(q), 1);
+      mbar_init(bar_l(q), 2);
+    }
+    mbar_init(bar_sread, 4);
     mbar_init(bar_o, 1);
     mbar_init(bar_q, C::kSoftWarps);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 16) {
     tmem_alloc(smem_addr(tmem_slot), C::kTmemCols);
     tmem_relinquish();
   }
   pdl_wait();
+  constexpr int QC = D * 2 / 16;  // 16-byte chunks of a row of Q
+  if (warp < C::kSoftWarps) {
+    // Q as it comes to shared memory; a lane works out where one of the warp's 16 rows is
+    const int ri = r0 + warp + C::kSoftWarps * (lane & 15);
+    const int tok = ri / p.group, g = ri - tok * p.group;
+    const long long off = b * p.qb + tok * p.qt + (h * p.group + g) * p.qh;
+#pragma unroll 2
+    for (int i = 0; i < 16; ++i) {
+      const int x = warp + C::kSoftWarps * i;
+      const long long o = __shfl_sync(0xffffffffu, off, i);
+      const uint32_t dst = smem_addr(q_smem) + x * 2 * D + ((lane ^ (x & 7)) << 4);
+      if (lane < QC) {
+        if (r0 + x < p.rows) cp_async16(dst, static_cast<const T*>(p.q) + o + lane * 8);
+        else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
+      }
+    }
+    cp_async_commit();
+  } else if (threadIdx.x == 17 * 32) {
+    // which tiles: the keys that the last row sees (an earlier row never sees more), this split's share
+    const int len = min(max(p.lengths[b], 0), p.capacity);
+    const int last = min(p.rows, r0 + C::kRows) - 1;
+    const int tiles = (keys_seen(p, len, p.causal ? last / p.group : 0) + C::kKeys - 1) / C::kKeys;
+    const int per = (tiles + p.splits - 1) / p.splits;
+    const int first = min(tiles, split * per);
+    plan[0] = len;
+    plan[1] = first;
+    plan[2] = min(tiles, first + per) - first;
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  const int n = min(max(p.lengths[b], 0), p.capacity);
-  // the tile's keys: those its last row sees (an earlier row never sees more)
-  const int last = min(p.rows, r0 + C::kRows) - 1;
-  const int kend = keys_seen(p, n, last / p.group);
-  const int ntiles = (kend + C::kKeys - 1) / C::kKeys;
-  const int per = (ntiles + p.splits - 1) / p.splits;
-  const int tile0 = min(ntiles, split * per), nt = min(ntiles, tile0 + per) - tile0;
+  const int n = plan[0], tile0 = plan[1], nt = plan[2];
   const int nblocks = (n + kKvBlock - 1) / kKvBlock;  // blocks with a scale
 
-  if (warp == 8) {
-    // ------------------------------------------------ MMA issuer (one elected lane)
-    const bool issuer = elect_one();
-    const uint32_t idesc_s = idesc_f16(C::kRows, C::kKeys);
-    const uint32_t idesc_o = idesc_f16(C::kRows, D);
-    const auto issue_s = [&](int i) -> bool {
-      const int slot = i & 1;
-      if (!warp_all(mbar_wait_spin(bar_kfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit))) return false;
-      tc_fence_after();
-      const uint64_t kdesc = smem_desc_sw128(smem_addr(k_ring + slot * C::kKBytes));
-#pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
-        if (issuer)
-          umma_f16_ts(tmem_base + C::kSCol + slot * C::kKeys, tmem_base + C::kQCol + 8 * kk,
-                      kdesc + static_cast<uint64_t>((kk >> 2) * (C::kKeys * 128) >> 4) + static_cast<uint64_t>((kk & 3) * 2),
-                      idesc_s, kk > 0);
-      if (issuer) {
-        umma_commit(bar_kempty(slot));
-        umma_commit(bar_sfull(slot));
-      }
-      __syncwarp();
-      return true;
-    };
-    bool alive = nt > 0 && warp_all(mbar_wait_spin(bar_q, 0, abort_flag, err, kErrWaitUnpack, limit)) && issue_s(0);
-    for (int i = 0; alive && i < nt; ++i) {
-      if (i + 1 < nt && !(alive = issue_s(i + 1))) break;
-      const int slot = i & 1;
-      bool ok = mbar_wait_spin(bar_vfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitUnpack, limit);
-      if (ok) ok = mbar_wait_spin(bar_pfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit);
-      if (!warp_all(ok)) {
-        alive = false;
-        break;
-      }
-      tc_fence_after();
-      const uint64_t vdesc = smem_desc_sw128(smem_addr(v_ring + slot * C::kVBytes));
-#pragma unroll
-      for (int kk = 0; kk < C::kKeys / 16; ++kk)
-        if (issuer)
-          umma_f16_ts(tmem_base + C::kOCol, tmem_base + C::kSCol + slot * C::kKeys + 8 * kk,
-                      vdesc + static_cast<uint64_t>(kk * 2), idesc_o, (i | kk) != 0);
-      if (issuer) {
-        umma_commit(bar_vempty(slot));
-        umma_commit(bar_pfree(slot));
-      }
-      __syncwarp();
-    }
-    if (issuer) umma_commit(bar_o);  // arrives once every MMA of this CTA has completed
-    __syncwarp();
-    volatile int no_abort = 0;
-    mbar_wait_bounded(bar_o, 0, &no_abort, err, kErrWaitDrain, limit);
-  } else if (warp >= 13) {
-    // ------------------------------------------------ values -> V^T (fp16)
-    constexpr int W = D / 64;  // words of a lane's run of dims: 1, 2 or 4
-    const int kc = lane & 7;   // keys 8 kc .. 8 kc + 7 of a tile
-    const int dim0 = (warp - 13) * (D / 4) + (lane >> 3) * (D / 16);
-    const int8_t* src = p.v + b * p.cb + h * p.ch + dim0;
-    uint32_t w[8][W];
-    const auto load = [&](int i) {
-      const int j0 = (tile0 + i) * C::kKeys + 8 * kc;
-      const int8_t* a = src + static_cast<long long>(j0) * p.ct;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-#pragma unroll
-        for (int x = 0; x < W; ++x) w[k][x] = 0u;
-        if (j0 + k < n) {
-          if constexpr (W == 4) *reinterpret_cast<uint4*>(w[k]) = __ldg(reinterpret_cast<const uint4*>(a + k * p.ct));
-          else if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = __ldg(reinterpret_cast<const uint2*>(a + k * p.ct));
-          else w[k][0] = __ldg(reinterpret_cast<const uint32_t*>(a + k * p.ct));
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRestRegs));
+    if (warp == 17) {
+      // ---------------------------------------------- codes (lane 0)
+      if (lane == 0) {
+        constexpr int kBoxes = D > 128 ? D / 128 : 1, kBox = C::kRaw / kBoxes;
+        int issued = 0;
+        for (int i = 0; i < nt; ++i, ++issued) {
+          const int slot = i & 1, j0 = (tile0 + i) * C::kKeys;
+          if (i >= 2 && !mbar_wait_spin(bar_kread(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)) break;
+          mbar_arrive_expect_tx(bar_kraw(slot), C::kRaw);
+          for (int x = 0; x < kBoxes; ++x)
+            tma_load_4d(smem_addr(k_raw + slot * C::kRaw + x * kBox), &params.tmap_k, 128 * x, h, j0, b, bar_kraw(slot));
+          if (i >= 2 && !mbar_wait_spin(bar_vread(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)) {
+            volatile int no_abort = 0;
+            mbar_wait_bounded(bar_kraw(slot), (i >> 1) & 1, &no_abort, err, kErrWaitDrain, limit);
+            break;
+          }
+          mbar_arrive_expect_tx(bar_vraw(slot), C::kRaw);
+          for (int x = 0; x < kBoxes; ++x)
+            tma_load_4d(smem_addr(v_raw + slot * C::kRaw + x * kBox), &params.tmap_v, 128 * x, h, j0, b, bar_vraw(slot));
+        }
+        // no copy may still be in flight at exit
+        volatile int no_abort = 0;
+        for (int i = max(0, issued - 2); i < issued; ++i) {
+          mbar_wait_bounded(bar_kraw(i & 1), (i >> 1) & 1, &no_abort, err, kErrWaitDrain, limit);
+          mbar_wait_bounded(bar_vraw(i & 1), (i >> 1) & 1, &no_abort, err, kErrWaitDrain, limit);
         }
       }
-    };
-    if (nt > 0) load(0);
+      __syncwarp();
+    } else if (warp == 16) {
+      // ---------------------------------------------- MMA issuer (one elected lane)
+      const bool issuer = elect_one();
+      const uint32_t idesc_s = idesc_f16(C::kRows, C::kKeys);
+      const uint32_t idesc_o = idesc_f16(C::kRows, D);
+      bool alive = nt == 0 || warp_all(mbar_wait_spin(bar_q, 0, abort_flag, err, kErrWaitUnpack, limit));
+      // whichever product is ready next: S(si) (its keys are there and S(si - 1) has been read) or P(pi) V
+      int si = 0, pi = 0, idle = 0;
+      uint64_t since = 0;
+      while (alive && pi < nt) {
+        const int ss = si & 1, ps = pi & 1;
+        const bool s_ready = si < nt && mbar_test_wait(bar_kfull(ss), (si >> 1) & 1) &&
+                             (si == 0 || mbar_test_wait(bar_sread, (si - 1) & 1));
+        if (__any_sync(0xffffffffu, s_ready)) {
+          tc_fence_after();
+          const uint64_t kdesc = smem_desc_sw128(smem_addr(k_ring + ss * C::kKBytes));
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            if (issuer)
+              umma_f16_ts(tmem_base + C::kSCol, tmem_base + C::kQCol + 8 * kk,
+                          kdesc + static_cast<uint64_t>((kk >> 2) * (C::kKeys * 128) >> 4) + static_cast<uint64_t>((kk & 3) * 2),
+                          idesc_s, kk > 0);
+          if (issuer) {
+            umma_commit(bar_sfull(ss));
+            umma_commit(bar_kempty(ss));
+          }
+          __syncwarp();
+          ++si;
+          idle = 0;
+          continue;
+        }
+        const bool p_ready = mbar_test_wait(bar_vfull(ps), (pi >> 1) & 1) && mbar_test_wait(bar_pfull(ps), (pi >> 1) & 1);
+        if (__any_sync(0xffffffffu, p_ready)) {
+          tc_fence_after();
+          const uint64_t vdesc = smem_desc_sw128(smem_addr(v_ring + ps * C::kVBytes));
+#pragma unroll
+          for (int kk = 0; kk < C::kKeys / 16; ++kk)
+            if (issuer)
+              umma_f16_ts(tmem_base + C::kOCol, tmem_base + C::kPCol + ps * 32 + 8 * kk,
+                          vdesc + static_cast<uint64_t>(kk * 2), idesc_o, (pi | kk) != 0);
+          if (issuer) {
+            umma_commit(bar_pfree(ps));
+            umma_commit(bar_vempty(ps));
+          }
+          __syncwarp();
+          ++pi;
+          idle = 0;
+          continue;
+        }
+        if ((++idle & 63) == 0) {
+          const uint64_t now = global_timer_ns();
+          if (idle == 64) since = now;
+          bool stop = *abort_flag != 0;
+          if (!stop && now - since > limit) {
+            stop = true;
+            *abort_flag = 1;
+            if (lane == 0) atomicOr(err, kErrWaitUnpack);
+          }
+          alive = !__any_sync(0xffffffffu, stop);
+        }
+      }
+      if (issuer) umma_commit(bar_o);  // arrives once every MMA of this CTA has completed
+      __syncwarp();
+      volatile int no_abort = 0;
+      mbar_wait_bounded(bar_o, 0, &no_abort, err, kErrWaitDrain, limit);
+    }
+  } else if (warp >= 12) {
+    // ------------------------------------------------ values -> V^T (fp16)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvRegs));
+    constexpr int W = D / 64;  // words of a lane's run of dims: 1, 2 or 4
+    const int kc = lane & 7;   // positions 8 kc .. 8 kc + 7 of a tile: keys kc, kc + 8, ...
+    const int dim0 = (warp - 12) * (D / 4) + (lane >> 3) * (D / 16);
+    // keys kc + 8 k lie 8 rows apart, with the same swizzle
+    const uint8_t* src = v_raw + (D >= 128 ? (dim0 >> 7) * (C::kKeys * 128) + kc * 128 + ((((dim0 >> 4) & 7) ^ kc) << 4)
+                                           : kc * 64 + (((dim0 >> 4) ^ ((kc >> 1) & 3)) << 4)) + (dim0 & 15);
+    constexpr int kStep = 8 * (D >= 128 ? 128 : 64);
     for (int i = 0; i < nt; ++i) {
       const int slot = i & 1;
-      if (i >= 2 && !warp_all(mbar_wait_spin(bar_vempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)))
-        break;
+      bool ok = mbar_wait_spin(bar_vraw(slot), (i >> 1) & 1, abort_flag, err, kErrWaitTma, limit);
+      if (ok && i >= 2) ok = mbar_wait_spin(bar_vempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit);
+      if (!warp_all(ok)) break;
+      uint32_t w[8][W];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint8_t* a = src + slot * C::kRaw + k * kStep;
+        if constexpr (W == 4) *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(a);
+        else if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(a);
+        else w[k][0] = *reinterpret_cast<const uint32_t*>(a);
+      }
       uint8_t* dst = v_ring + slot * C::kVBytes;
 #pragma unroll
       for (int x = 0; x < W; ++x) {
@@ -754,98 +855,113 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
           *reinterpret_cast<uint4*>(dst + dim * 128 + ((kc ^ (dim & 7)) << 4)) = o;
         }
       }
-      if (i + 1 < nt) load(i + 1);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_vfull(slot));
-    }
-  } else if (warp >= 9) {
-    // ------------------------------------------------ keys -> K (fp16)
-    constexpr int U = 2 * C::kSlices;  // (8 keys x 64 dims) units of a warp
-    const int kr = lane >> 2, c4 = lane & 3;
-    const int8_t* src = p.k + b * p.cb + h * p.ch + 16 * c4;
-    uint4 w[U];
-    const auto load = [&](int i) {
-      const int j0 = (tile0 + i) * C::kKeys + kr;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int id = warp - 9 + 4 * u, j = j0 + 8 * (id / C::kSlices);
-        w[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (j < n) w[u] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(j) * p.ct + 64 * (id % C::kSlices)));
+      if (lane == 0) {
+        mbar_arrive(bar_vread(slot));
+        mbar_arrive(bar_vfull(slot));
       }
-    };
-    if (nt > 0) load(0);
-    for (int i = 0; i < nt; ++i) {
+    }
+  } else if (warp >= 8) {
+    // ------------------------------------------------ keys -> K (fp16)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvRegs));
+    constexpr int J = D / 16;          // 16-byte chunks of a key
+    constexpr int kPass = 128 / J;     // keys of a pass of the 128 threads
+    constexpr int U = C::kKeys / kPass;
+    const int t = threadIdx.x - 256, j = t % J, s0 = t / J, sel = (lane >> 2) & 1;
+    bool alive = nt == 0 || warp_all(mbar_wait_spin(bar_q, 0, abort_flag, err, kErrWaitUnpack, limit));  // Q has left the ring
+    for (int i = 0; alive && i < nt; ++i) {
       const int slot = i & 1;
-      if (i >= 2 && !warp_all(mbar_wait_spin(bar_kempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit)))
-        break;
+      bool ok = mbar_wait_spin(bar_kraw(slot), (i >> 1) & 1, abort_flag, err, kErrWaitTma, limit);
+      if (ok && i >= 2) ok = mbar_wait_spin(bar_kempty(slot), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitEmpty, limit);
+      if (!warp_all(ok)) break;
+      uint4 w[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int id = warp - 9 + 4 * u, row = 8 * (id / C::kSlices) + kr;
-        uint8_t* dst = k_ring + slot * C::kKBytes + (id % C::kSlices) * (C::kKeys * 128) + row * 128;
+        const int s = s0 + kPass * u;  // key of the tile
+        w[u] = *reinterpret_cast<const uint4*>(
+            k_raw + slot * C::kRaw + (D >= 128 ? (j >> 3) * (C::kKeys * 128) + s * 128 + (((j & 7) ^ (s & 7)) << 4)
+                                               : s * 64 + ((j ^ ((s >> 1) & 3)) << 4)));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = s0 + kPass * u, row = 8 * (s & 7) + (s >> 3);
+        uint8_t* dst = k_ring + slot * C::kKBytes + (j >> 2) * (C::kKeys * 128) + row * 128;
         const uint32_t x[4] = {w[u].x ^ 0x80808080u, w[u].y ^ 0x80808080u, w[u].z ^ 0x80808080u, w[u].w ^ 0x80808080u};
+        uint4 o[2];
 #pragma unroll
         for (int y = 0; y < 2; ++y)
-          *reinterpret_cast<uint4*>(dst + (((2 * c4 + y) ^ (row & 7)) << 4)) =
-              make_uint4(codes_to_half2<0>(x[2 * y]), codes_to_half2<1>(x[2 * y]), codes_to_half2<0>(x[2 * y + 1]),
-                         codes_to_half2<1>(x[2 * y + 1]));
+          o[y] = make_uint4(codes_to_half2<0>(x[2 * y]), codes_to_half2<1>(x[2 * y]), codes_to_half2<0>(x[2 * y + 1]),
+                            codes_to_half2<1>(x[2 * y + 1]));
+        // the two halves in turn, so that 8 lanes meet all banks
+        const int c = 2 * (j & 3);
+        *reinterpret_cast<uint4*>(dst + (((c + sel) ^ (row & 7)) << 4)) = sel ? o[1] : o[0];
+        *reinterpret_cast<uint4*>(dst + (((c + 1 - sel) ^ (row & 7)) << 4)) = sel ? o[0] : o[1];
       }
-      if (i + 1 < nt) load(i + 1);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_kfull(slot));
+      if (lane == 0) {
+        mbar_arrive(bar_kread(slot));
+        mbar_arrive(bar_kfull(slot));
+      }
     }
   } else {
     // ------------------------------------------------ softmax + epilogue (warps 0-7)
-    const int quarter = warp & 3, half = warp >> 2;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+    const int quarter = warp & 3, group = warp >> 2;
     const int row = quarter * 32 + lane, r = r0 + row;
     const uint32_t lane_addr = static_cast<uint32_t>(quarter * 32) << 16;
     // ---- Q: raw rows to shared memory, then (thread = row and half of its dims) to TMEM as fp16
     {
-      constexpr int QC = D * 2 / 16;  // chunks of a row
-      for (int i = warp; i < C::kRows; i += C::kSoftWarps) {
-        const int tok = (r0 + i) / p.group, g = (r0 + i) - tok * p.group;
-        const T* src = static_cast<const T*>(p.q) + b * p.qb + tok * p.qt + (h * p.group + g) * p.qh + lane * 8;
-        const uint32_t dst = smem_addr(q_smem) + i * 2 * D + ((lane ^ (i & 7)) << 4);
-        if (lane < QC) {
-          if (r0 + i < p.rows) cp_async16(dst, src);
-          else asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(0u) : "memory");
-        }
-      }
-      cp_async_commit();
       cp_async_wait<0>();
       asm volatile("bar.sync 1, 256;" ::: "memory");  // the 8 softmax warps (nothing has given up yet)
       const uint8_t* mine = q_smem + row * 2 * D;
-      uint32_t key = 0;
+      float shift = 1.f;
+      if constexpr (!std::is_same_v<T, __half>) {
+        // bf16: the row's largest element decides the power of two that brings it into fp16
+        __nv_bfloat162 top = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll 4
-      for (int c = half * (QC / 2); c < (half + 1) * (QC / 2); ++c) {
-        float v[8];
-        load8(reinterpret_cast<const T*>(mine + ((c ^ (row & 7)) << 4)), v);
+        for (int c = group * (QC / 2); c < (group + 1) * (QC / 2); ++c) {
+          const uint4 raw = *reinterpret_cast<const uint4*>(mine + ((c ^ (row & 7)) << 4));
+          const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&raw);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) key = max(key, abs_key(v[e]));
+          for (int e = 0; e < 4; ++e) top = __hmax2(top, __habs2(x[e]));
+        }
+        row_x[group * C::kRows + row] = fmaxf(__low2float(top), __high2float(top));
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        shift = query_shift(fmaxf(row_x[row], row_x[C::kRows + row]));
       }
-      row_x[half * C::kRows + row] = __uint_as_float(key);
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      const uint32_t amax = max(abs_key(row_x[row]), abs_key(row_x[C::kRows + row]));
-      const float shift = query_shift(__uint_as_float(amax));
       const float up = p.scale < 0.f ? -shift : shift;
-      if (half == 0)
-        row_info[row] = make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, r / p.group) : 0));
+      if (group == 0) {
+        row_info[row] = make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, p.causal ? r / p.group : 0) : 0));
+        row_m[row] = -INFINITY;
+        row_v[row] = 0.f;
+      }
 #pragma unroll 1
-      for (int c = half * (QC / 2); c < (half + 1) * (QC / 2); c += 4) {
+      for (int c = group * (QC / 2); c < (group + 1) * (QC / 2); c += 4) {
         uint32_t w[16];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          float v[8];
-          load8(reinterpret_cast<const T*>(mine + (((c + x) ^ (row & 7)) << 4)), v);
+          const uint8_t* src = mine + (((c + x) ^ (row & 7)) << 4);
+          if constexpr (std::is_same_v<T, __half>) {
+            const uint4 raw = *reinterpret_cast<const uint4*>(src);
+            const uint32_t flip = p.scale < 0.f ? 0x80008000u : 0u;
+            w[4 * x] = raw.x ^ flip, w[4 * x + 1] = raw.y ^ flip, w[4 * x + 2] = raw.z ^ flip, w[4 * x + 3] = raw.w ^ flip;
+          } else {
+            float v[8];
+            load8(reinterpret_cast<const T*>(src), v);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[4 * x + e] = pack_half2_bits(v[2 * e] * up, v[2 * e + 1] * up);
+            for (int e = 0; e < 4; ++e) {
+              const float2 y = __fmul2_rn(make_float2(v[2 * e], v[2 * e + 1]), make_float2(up, up));
+              w[4 * x + e] = pack_half2_bits(y.x, y.y);
+            }
+          }
         }
         tmem_st_32x32b_x16(tmem_base + lane_addr + C::kQCol + 4 * c, w);
       }
       tmem_st_wait();
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_info, and row_x may be written again
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_info, row_m; row_x may be written again
       if (lane == 0) mbar_arrive(bar_q);
     }
     const float2 info = row_info[row];
@@ -855,144 +971,187 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
     const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
     float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;
     bool alive = true;
-    for (int i = 0; i < nt; ++i) {
-      const int slot = i & 1, j0 = (tile0 + i) * C::kKeys, blk = j0 / kKvBlock;
-      float ksc[2], vsc[4];
+    // a tile's scales, one to a lane, a turn ahead: keys' (lanes 0-3), values' (4-7), the tile before's values' (8-11);
+    // zero past the length
+    const float* scale_src = (lane < 4 ? ks : vs) + (lane & 3);
+    const auto fetch_scale = [&](int i) {
+      const int blk = (tile0 + i - (lane >= 8)) * (C::kKeys / kKvBlock);
+      return lane < 12 && i < nt && blk >= 0 && blk + (lane & 3) < nblocks ? __ldg(scale_src + blk) : 0.f;
+    };
+    float scales = fetch_scale(group);
+    const auto largest = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };  // passes NaN by
+    for (int i = group; i < nt; i += 2) {
+      const int j0 = (tile0 + i) * C::kKeys;
+      float ksc[4], vsc[4], vbefore[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) vsc[q] = blk + q < nblocks ? __ldg(vs + blk + q) : 0.f;
-#pragma unroll
-      for (int q = 0; q < 2; ++q) ksc[q] = blk + 2 * half + q < nblocks ? __ldg(ks + blk + 2 * half + q) : 0.f;
-      if (!warp_all(mbar_wait_spin(bar_sfull(slot), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+      for (int q = 0; q < 4; ++q) {
+        ksc[q] = __shfl_sync(0xffffffffu, scales, q) * factor;
+        vsc[q] = __shfl_sync(0xffffffffu, scales, 4 + q);
+        vbefore[q] = __shfl_sync(0xffffffffu, scales, 8 + q);
+      }
+      scales = fetch_scale(i + 2);
+      if (!warp_all(mbar_wait_spin(bar_sfull(group), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
         alive = false;
         break;
       }
       tc_fence_after();
-      uint32_t raw[32];
-      {
-        const uint32_t t = tmem_base + lane_addr + C::kSCol + slot * C::kKeys + 32 * half;
-        tmem_ld_32x32b_x16(t, *reinterpret_cast<uint32_t(*)[16]>(&raw[0]));
-        tmem_ld_32x32b_x16(t + 16, *reinterpret_cast<uint32_t(*)[16]>(&raw[16]));
-        tmem_ld_wait();
-      }
-      // unseen keys of a row's last tiles: -inf, whatever their block's scale is
-      float bmax = -INFINITY;
-      const int left = seen - j0 - 32 * half;
-      const bool whole = __all_sync(0xffffffffu, left >= 32);
+      uint32_t raw[64];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        ksc[q] *= factor;
-        if (whole) {
-          float x = -INFINITY, y = -INFINITY;
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) {
-            x = fmaxf(x, __uint_as_float(raw[16 * q + c]));
-            y = fmaxf(y, __uint_as_float(raw[16 * q + c + 1]));
-          }
-          bmax = fmaxf(bmax, fmaxf(x, y) * ksc[q]);  // the factor is not negative
-        } else {
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float v = 16 * q + c < left ? __uint_as_float(raw[16 * q + c]) * ksc[q] : -INFINITY;
-            raw[16 * q + c] = __float_as_uint(v);
-            bmax = fmaxf(bmax, v);
-          }
-          ksc[q] = 1.f;
-        }
-      }
-      // the row's maximum over both halves (both warps have read their scores: P may take their place)
-      row_x[(slot * 2 + half) * C::kRows + row] = bmax;
+      for (int c = 0; c < 64; c += 16)
+        tmem_ld_32x32b_x16(tmem_base + lane_addr + C::kSCol + c, *reinterpret_cast<uint32_t(*)[16]>(&raw[c]));
+      tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_pair(quarter));
-      if (!warp_all(mbar_wait_spin(bar_pair(quarter), i & 1, abort_flag, err, kErrWaitAccum, limit))) {
-        alive = false;
-        break;
+      if (lane == 0) mbar_arrive(bar_sread);
+      // ---- the tile's maximum of the row; column c is key 8 (c % 8) + c / 8, whose scale is number (c % 8) / 2.  Keys
+      // that the row does not see are left out, whatever their block's scale
+      float bmax = -INFINITY;
+      const int left = seen - j0;
+      const bool whole = __all_sync(0xffffffffu, left >= C::kKeys);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float x0 = -INFINITY, x1 = -INFINITY;
+        if (whole) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            x0 = fmaxf(x0, __uint_as_float(raw[8 * c + 2 * q]));
+            x1 = fmaxf(x1, __uint_as_float(raw[8 * c + 2 * q + 1]));
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (16 * q + c < left) x0 = fmaxf(x0, __uint_as_float(raw[8 * c + 2 * q]));
+            if (16 * q + 8 + c < left) x1 = fmaxf(x1, __uint_as_float(raw[8 * c + 2 * q + 1]));
+          }
+        }
+        x0 = fmaxf(x0, x1);
+        if (x0 > -INFINITY) bmax = fmaxf(bmax, x0 * ksc[q]);  // the factor is not negative
       }
-      bmax = fmaxf(bmax, row_x[(slot * 2 + (half ^ 1)) * C::kRows + row]);
+      // ---- m as the tile before left it, then this tile's
+      if (i > 0) {
+        if (!warp_all(mbar_wait_spin(bar_m(quarter), (i - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+          alive = false;
+          break;
+        }
+        const float mb = row_m[row];
+        if (mb != m) {
+          l *= m == -INFINITY ? 0.f : ex2_approx(m - mb);
+          m = mb;
+        }
+        if (largest(vbefore) > kAttn8VGrow * vref) {  // O has been rescaled for it
+#pragma unroll
+          for (int q = 0; q < 4; ++q) move_vref(vbefore[q], vref);
+          vinv = vref >= 1e-30f ? __fdividef(1.f, vref) : 0.f;
+        }
+      }
       float f = 1.f;
       if (bmax > m + kAttn8Grow) {
+        bmax += kAttn8Margin;
         f = m == -INFINITY ? 0.f : ex2_approx(m - bmax);
         m = bmax;
         l *= f;
       }
-      const float vmax = fmaxf(fmaxf(vsc[0], vsc[1]), fmaxf(vsc[2], vsc[3]));  // passes NaN by
-      if (vmax > kAttn8VGrow * vref) {
+      if (largest(vsc) > kAttn8VGrow * vref) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) f *= move_vref(vsc[q], vref);
         vinv = vref >= 1e-30f ? __fdividef(1.f, vref) : 0.f;
       }
       if (i >= 1 && __any_sync(0xffffffffu, f != 1.f)) {
-        // O holds the earlier tiles: wait for the last of them, rescale this warp's rows and half of the columns
+        // O holds the earlier tiles: wait for the last of them, rescale this warp's rows
         if (!warp_all(mbar_wait_spin(bar_pfree((i - 1) & 1), ((i - 1) >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
           alive = false;
           break;
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
-          uint32_t o[16];
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t o[32];
           const uint32_t t = tmem_base + lane_addr + C::kOCol + c0;
-          tmem_ld_32x32b_x16(t, o);
+          tmem_ld_32x32b_x16(t, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
+          tmem_ld_32x32b_x16(t + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
-          tmem_st_32x32b_x16(t, o);
+          for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * f);
+          tmem_st_32x32b_x32(t, o);
         }
         tmem_st_wait();
+        tc_fence_before();
       }
+      row_m[row] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_m(quarter));
+      // ---- P = 2^(s - m), times vs / vref
       const float nm = m == -INFINITY ? 0.f : -m;
-      uint32_t pw[16];
+      const bool plain = whole && vsc[0] + vsc[1] + vsc[2] + vsc[3] <= 3.4028234e38f;  // false for NaN
+      float rv[4];
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const float v = vsc[2 * half + q];
-        const float rv = vinv > 0.f ? v * vinv : vscale_ratio(v, vref);
-        float2 sum = make_float2(0.f, 0.f);
-        const float2 kk = make_float2(ksc[q], ksc[q]), mm = make_float2(nm, nm), rr = make_float2(rv, rv);
-        if (v <= 3.4028234e38f) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float2 x = __ffma2_rn(
-                make_float2(__uint_as_float(raw[16 * q + 2 * c]), __uint_as_float(raw[16 * q + 2 * c + 1])), kk, mm);
-            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
-            sum = __fadd2_rn(sum, e);
-            const float2 w = __fmul2_rn(e, rr);
-            pw[8 * q + c] = pack_half2_bits(w.x, w.y);
-          }
-        } else {  // a block with an infinity or NaN: rows that see it become NaN, others stay clean
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const float e0 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c]), ksc[q], nm));
-            const float e1 = ex2_approx(__fmaf_rn(__uint_as_float(raw[16 * q + 2 * c + 1]), ksc[q], nm));
-            sum.x += e0;
-            sum.y += e1;
-            const float nan = __uint_as_float(0x7fc00000u);
-            pw[8 * q + c] = pack_half2_bits(weigh(e0, nan), weigh(e1, nan));
-          }
-        }
-        l += sum.x + sum.y;
+      for (int q = 0; q < 4; ++q) rv[q] = vinv > 0.f && plain ? vsc[q] * vinv : vscale_ratio(vsc[q], vref);
+      if (i >= 2 && !warp_all(mbar_wait_spin(bar_pfree(group), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+        alive = false;
+        break;
       }
       tc_fence_after();
-      tmem_st_32x32b_x16(tmem_base + lane_addr + C::kSCol + slot * C::kKeys + 16 * half, pw);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        uint32_t pw[16];
+        if (plain) {
+          const float2 mm = make_float2(nm, nm);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {  // columns 32 hf + 2c, + 1: scale c % 4
+            const int q = c & 3;
+            const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[32 * hf + 2 * c]), __uint_as_float(raw[32 * hf + 2 * c + 1])),
+                                        make_float2(ksc[q], ksc[q]), mm);
+            const float2 e = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum[c & 1] = __fadd2_rn(sum[c & 1], e);
+            const float2 w = __fmul2_rn(e, make_float2(rv[q], rv[q]));
+            pw[c] = pack_half2_bits(w.x, w.y);
+          }
+        } else {
+          // a row's last keys, or a block with an infinity or NaN: a key that is not seen counts nothing, whatever its
+          // block's scales are
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const int q = c & 3, key = 16 * q + 4 * hf + (c >> 2);
+            float e[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+              e[z] = key + 8 * z < left ? ex2_approx(__fmaf_rn(__uint_as_float(raw[32 * hf + 2 * c + z]), ksc[q], nm)) : 0.f;
+            sum[0].x += e[0];
+            sum[0].y += e[1];
+            pw[c] = pack_half2_bits(weigh(e[0], rv[q]), weigh(e[1], rv[q]));
+          }
+        }
+        tmem_st_32x32b_x16(tmem_base + lane_addr + C::kPCol + 32 * group + 16 * hf, pw);
+      }
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_pfull(slot));
+      if (lane == 0) mbar_arrive(bar_pfull(group));
     }
     // ---- epilogue: O vref / l as T, or the unnormalised O vref and (m, l) of this split, to shared memory (the
-    // Q buffer and the idle rings)
+    // idle rings)
     alive = alive && warp_all(mbar_wait_bounded(bar_o, 0, abort_flag, err, kErrWaitAccum, limit));
     tc_fence_after();
-    row_x[half * C::kRows + row] = l;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(bar_pair(quarter));
-    alive = warp_all(mbar_wait_spin(bar_pair(quarter), nt & 1, abort_flag, err, kErrWaitAccum, limit)) && alive;
-    l += row_x[(half ^ 1) * C::kRows + row];
+    {
+      // the groups' sums, each at its own last maximum; the last tile's group has the final vref
+      const float mb = row_m[row];
+      row_x[group * C::kRows + row] = m == -INFINITY ? l : l * ex2_approx(m - mb);
+      if (nt > 0 && group == ((nt - 1) & 1)) row_v[row] = vref;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_l(quarter));
+      alive = warp_all(mbar_wait_spin(bar_l(quarter), 0, abort_flag, err, kErrWaitAccum, limit)) && alive;
+      m = mb;
+      l = row_x[row] + row_x[C::kRows + row];
+      vref = row_v[row];
+    }
     const bool part = p.splits > 1;
     const float f = part ? vref : l == 0.f ? 0.f : vref / l;
-    if (part && half == 0 && r < p.rows)
+    if (part && group == 0 && r < p.rows)
       p.part_ml[(static_cast<long long>(unit) * p.splits + split) * p.rows + r] = make_float2(m, alive ? l : __uint_as_float(0x7fc00000u));
 #pragma unroll 1
-    for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
+    for (int c0 = group * (D / 2); c0 < (group + 1) * (D / 2); c0 += 16) {
       uint32_t o[16];
       if (nt > 0) {
         tmem_ld_32x32b_x16(tmem_base + lane_addr + C::kOCol + c0, o);
@@ -1020,7 +1179,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
   // every MMA has completed (the issuer waited for bar_o) before TMEM is freed
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 16) {
     tc_fence_after();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
@@ -1034,7 +1193,6 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1) attn8_many_kernel(c
       bulk_wait_group0();
     }
   } else {
-    constexpr int QC = D * 2 / 16;
     for (int i = warp; i < rows; i += C::kThreads / 32)
       if (lane < QC)
         *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + out_row(p, b, h, r0 + i) * D + lane * 8) =

@@ -40,6 +40,27 @@ int ensure_smem_attr8(int dev, int bit, Kernel kernel, int bytes) {
   return W4A4_OK;
 }
 
+// Tiled map of rank 2 to 4, zeros outside, encoded for each call: dims[0]
+// innermost (elements), strides_bytes[i] the byte stride of dims[i + 1].
+int encode_map(CUtensorMap* out, const void* ptr, CUtensorMapDataType type, int rank, const uint64_t* dims,
+               const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
+  cuuint64_t d[4], st[3];
+  cuuint32_t bx[4], one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < rank; ++i) {
+    d[i] = dims[i], bx[i] = box[i];
+    if (i + 1 < rank) st[i] = strides_bytes[i];
+  }
+  const CUresult r = fn(out, type, static_cast<cuuint32_t>(rank), const_cast<void*>(ptr), d, st, bx, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? W4A4_OK
+                           : fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): rank %d, inner %llu, rows %llu, stride %llu",
+                                  static_cast<int>(r), rank, (unsigned long long)d[0], (unsigned long long)d[1],
+                                  (unsigned long long)st[0]);
+}
+
 // Whether rows of `stride` elements of `size` bytes from p all begin at a
 // multiple of `bytes`.
 bool rows_aligned(const void* p, int64_t stride, int size, int bytes) {
@@ -172,23 +193,10 @@ int gemm8_fit(int dev, int sms, int (&fit)[4]) {
   return W4A4_OK;
 }
 
-// Tiled map of rows of `k` elements of `size` bytes with boxes of bx elements x
-// by rows, zeros outside.  Encoded for each call.
-int gemm8_map(CUtensorMap* out, const void* ptr, CUtensorMapDataType type, int64_t k, int64_t rows, int64_t stride_bytes,
-              int bx, int by, CUtensorMapSwizzle swizzle) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable from the driver");
-  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
-  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(stride_bytes)};
-  const cuuint32_t boxes[2] = {static_cast<cuuint32_t>(bx), static_cast<cuuint32_t>(by)}, estr[2] = {1, 1};
-  const CUresult r = fn(out, type, 2, const_cast<void*>(ptr), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? W4A4_OK
-                           : fail(W4A4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for [%lld, %lld], row stride %lld bytes",
-                                  static_cast<int>(r), (long long)rows, (long long)k, (long long)stride_bytes);
-}
 int gemm8_codes_map(CUtensorMap* out, const int8_t* ptr, int k, int64_t rows, int64_t ld, int box) {
-  return gemm8_map(out, ptr, CU_TENSOR_MAP_DATA_TYPE_UINT8, k, rows, ld, 128, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)}, stride = static_cast<uint64_t>(ld);
+  const uint32_t boxes[2] = {128, static_cast<uint32_t>(box)};
+  return encode_map(out, ptr, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, dims, &stride, boxes, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
@@ -227,13 +235,14 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     const int bit = 24 + 2 * (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 1 : 2);
     if (plan.pair) {
       p.tma_store = n * sizeof(T) % 16 == 0;
-      if (p.tma_store)
-        if (int e = gemm8_map(&p.tmap_y, y,
-                              std::is_same_v<T, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                              : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                              n, m, static_cast<int64_t>(n) * sizeof(T), 64 / sizeof(T), 32, CU_TENSOR_MAP_SWIZZLE_64B))
-          return e;
+      if (p.tma_store) {
+        const auto type = std::is_same_v<T, float>    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                          : std::is_same_v<T, __half> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const uint64_t dims[2] = {static_cast<uint64_t>(n), static_cast<uint64_t>(m)}, stride = n * sizeof(T);
+        const uint32_t box[2] = {64 / sizeof(T), 32};
+        if (int e = encode_map(&p.tmap_y, y, type, 2, dims, &stride, box, CU_TENSOR_MAP_SWIZZLE_64B)) return e;
+      }
       if (int e = ensure_smem_attr8(dev, bit, gemm8_pair_kernel<T>, kG8PairSmem)) return e;
       const int pairs = std::min(sms / 2, plan.n_tok_tiles * plan.n_w_tiles);
       W4A4_CUDA_TRY(launch_kernel(gemm8_pair_kernel<T>, dim3(2 * pairs), dim3(kG8PairThreads), kG8PairSmem, stream, 2, p));
@@ -262,7 +271,7 @@ int check_cache8(const void* k, const void* v, const void* ks, const void* vs, c
   if (!k || !v || !ks || !vs) return fail(W4A4_ERR_INVALID, "%s: null pointer argument", what);
   if (!aligned(k, 16) || !aligned(v, 16) || stride[0] % 16 || stride[1] % 16 || stride[2] % 16)
     return fail(W4A4_ERR_INVALID, "%s: cache rows must begin at multiples of 16 bytes", what);
-  if (stride[0] < 0 || stride[1] < width || stride[2] < width)
+  if (stride[0] < width || stride[1] < width || stride[2] < width)
     return fail(W4A4_ERR_INVALID, "%s: cache strides must be at least the head width", what);
   return W4A4_OK;
 }
@@ -282,7 +291,7 @@ Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, int sms) {
   plan.tiles = static_cast<int>((rows + 127) / 128);
   const int64_t work = units * (plan.few ? 1 : plan.tiles);
   // keys that make a split worth its part of the join
-  const int64_t most = plan.few ? (capacity + 127) / 128 : (capacity + 255) / 256;
+  const int64_t most = plan.few ? (capacity + 127) / 128 : (capacity + 191) / 192;
   plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, sms / std::max<int64_t>(work, 1), 256})));
   return plan;
 }
@@ -303,10 +312,27 @@ int launch_attention8_d(const Attn8Params& p, const Attn8Plan& plan, int64_t uni
     };
     if (int e = p.rows <= 8 ? go(std::true_type{}, bit) : go(std::false_type{}, bit + 1)) return e;
   } else {
+    using C = Attn8Many<D>;
     const auto kernel = attn8_many_kernel<T, D>;
-    if (int e = ensure_smem_attr8(dev, bit + 2, kernel, Attn8Many<D>::kSmem)) return e;
-    W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.tiles, p.splits, static_cast<unsigned>(units)),
-                                dim3(Attn8Many<D>::kThreads), Attn8Many<D>::kSmem, stream, 1, p));
+    // the register split draws on what the CTA is launched with: more than that would wait for good
+    static const int regs = [&] {
+      cudaFuncAttributes fa;
+      return cudaFuncGetAttributes(&fa, kernel) == cudaSuccess ? (fa.numRegs + 7) / 8 * 8 : 0;
+    }();
+    if (regs * C::kThreads < C::kPoolRegs)
+      return fail(W4A4_ERR_UNSUPPORTED, "attention8: built with %d registers a thread, too few for its register split", regs);
+    if (int e = ensure_smem_attr8(dev, bit + 2, kernel, C::kSmem)) return e;
+    Attn8ManyParams mp;
+    mp.p = p;
+    const uint64_t dims[4] = {D, static_cast<uint64_t>(p.heads), static_cast<uint64_t>(p.capacity),
+                              static_cast<uint64_t>(units / p.heads)};
+    const uint64_t strides[3] = {static_cast<uint64_t>(p.ch), static_cast<uint64_t>(p.ct), static_cast<uint64_t>(p.cb)};
+    const uint32_t box[4] = {D < 128 ? D : 128, 1, C::kKeys, 1};
+    const CUtensorMapSwizzle sw = D < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    if (int e = encode_map(&mp.tmap_k, p.k, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, dims, strides, box, sw)) return e;
+    if (int e = encode_map(&mp.tmap_v, p.v, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, dims, strides, box, sw)) return e;
+    W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.tiles, p.splits, static_cast<unsigned>(units)), dim3(C::kThreads), C::kSmem,
+                                stream, 1, mp));
   }
   if (p.splits > (plan.few ? 8 : 1))
     W4A4_CUDA_TRY(launch_kernel(attn8_join_kernel<T, D>, dim3(static_cast<unsigned>(p.rows), static_cast<unsigned>(units)),
