@@ -346,8 +346,8 @@ int w4a4_layer_norm_bf16(const void* x, void* y, int64_t rows, int32_t h, const 
  * x, delta and gate of type `dtype`, gain and shift fp32; gate, gain and shift
  * rows of h for each observation of rows_per_batch rows, `*_stride` elements
  * apart (0: one row for all).  total (NULL: not stored) is [rows, h]
- * contiguous; codes have row stride ldc.  Any h > 0 and alignment; rows that
- * begin at multiples of 16 bytes (codes: 8) with h % 8 == 0 run vectorised. */
+ * contiguous; codes have row stride ldc.  Any alignment, h up to 49152; rows
+ * that begin at multiples of 16 bytes (codes: 8) with h % 8 == 0 run fastest. */
 int w4a4_rms_norm_quant8(const void* x, int64_t ldx, const void* delta, int64_t ldd, const void* gate,
                          int64_t gate_stride, const float* gain, int64_t gain_stride, const float* shift,
                          int64_t shift_stride, float eps, int32_t dtype, int64_t rows, int32_t rows_per_batch,

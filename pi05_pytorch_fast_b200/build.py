@@ -109,7 +109,7 @@ def build_ops(force: bool = False, verbose: bool = False) -> str:
             "-o", OPS_OUT + ".tmp", *OPS_SOURCES]
     for libdir in cpp_extension.library_paths():
         cmd += ["-L", libdir]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-L", PKG_DIR, "-lw4a4_sm100",
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-L", PKG_DIR, "-lw4a4_sm100",
             "-Wl,-rpath,$ORIGIN"]
     _run(cmd, OPS_OUT, verbose)
     return OPS_OUT

@@ -634,12 +634,24 @@ __global__ void __launch_bounds__(kG8PairThreads, 1) gemm8_pair_kernel(const __g
             bulk_commit_group();
           }
         } else {
-          // rows that do not begin at multiples of 16 bytes: a row of the box at a time
+          // rows that do not begin at multiples of 16 bytes: 8, 4 or 2 bytes a lane
           __syncwarp();
-          for (int q = 0; q < 32; ++q)
-            if (m0 + q < p.m && lane < W && n + lane < p.n)
-              static_cast<T*>(p.y)[(m0 + q) * p.n + n + lane] = *reinterpret_cast<const T*>(
-                  box + q * 64 + (((lane / V) ^ ((q >> 1) & 3)) << 4) + (lane % V) * sizeof(T));
+          const auto by = [&](auto word) {
+            using X = decltype(word);
+            constexpr int E = sizeof(X) / sizeof(T);       // values of a lane
+            constexpr int L = 64 / sizeof(X);              // lanes of a row
+            constexpr int RR = L < 32 ? 32 / L : 1;        // rows of an instruction
+            const int c = (lane % L) * E;
+#pragma unroll 4
+            for (int q = L < 32 ? lane / L : 0; q < 32; q += RR)
+              if (m0 + q < p.m && n + c < p.n)
+                *reinterpret_cast<X*>(static_cast<T*>(p.y) + (m0 + q) * p.n + n + c) = *reinterpret_cast<const X*>(
+                    box + q * 64 + (((c / V) ^ ((q >> 1) & 3)) << 4) + (c % V) * sizeof(T));
+          };
+          const int step = p.n * static_cast<int>(sizeof(T));
+          if (step % 8 == 0) by(uint2{});
+          else if (sizeof(T) == 4 || step % 4 == 0) by(uint32_t{});
+          else if constexpr (sizeof(T) == 2) by(uint16_t{});
           __syncwarp();
         }
       }

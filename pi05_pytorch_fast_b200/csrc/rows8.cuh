@@ -29,10 +29,8 @@ namespace w4a4 {
 
 enum RowOp : int { kRowQuant = 0, kRowGeglu = 1, kRowNorm = 2 };
 
-// Longest rows held in registers: 8-element vectors (aligned rows), single
-// elements (any row); longer ones are read again for each pass.
+// Longest rows held in registers (aligned rows of 8-element vectors).
 constexpr int kRow8MaxVec = 32768;
-constexpr int kRow8MaxScalar = 16384;
 
 constexpr float kInv127 = 1.0f / 127.0f;
 
@@ -384,73 +382,128 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
   }
 }
 
-// Rows too long for registers: each pass reads the row again (from L2).
-template <typename T, int OP>
-__global__ void __launch_bounds__(1024) row8_long_kernel(const __grid_constant__ Row8Params p) {
+// Any row: one, two or four elements at a time, the row's fp32 values in shared
+// memory between the passes.  For rows that do not begin at multiples of 16
+// bytes (a length that is not a multiple of 8), and for long ones.
+constexpr int kRow8AnyThreads = 256;
+constexpr int kRow8AnyMax = 49152;  // elements: 192 KB of shared memory
+
+// W = 4, 2 or 1 elements, aligned to their size.
+template <int W, typename T>
+__device__ __forceinline__ void load_few(const T* p, float (&v)[W]) {
+  struct alignas(W * sizeof(T)) Pack { T x[W]; };
+  const Pack a = *reinterpret_cast<const Pack*>(p);
+#pragma unroll
+  for (int i = 0; i < W; ++i) v[i] = to_float(a.x[i]);
+}
+template <int W, typename T>
+__device__ __forceinline__ void store_few(T* p, const float (&v)[W]) {
+  struct alignas(W * sizeof(T)) Pack { T x[W]; };
+  Pack a;
+#pragma unroll
+  for (int i = 0; i < W; ++i) a.x[i] = from_float<T>(v[i]);
+  *reinterpret_cast<Pack*>(p) = a;
+}
+
+template <typename T, int OP, int W>
+__global__ void __launch_bounds__(kRow8AnyThreads) row8_any_kernel(const __grid_constant__ Row8Params p) {
+  extern __shared__ __align__(16) float row8_smem[];
   __shared__ float red_sum[32];
   __shared__ uint32_t red_max[32];
   pdl_launch_dependents();
   pdl_wait();
   const long long row = blockIdx.x;
-  const long long obs = row / p.rows_per_batch;
+  const long long obs = OP == kRowNorm ? row / p.rows_per_batch : 0;
   const T* x = static_cast<const T*>(p.x) + row * p.ldx;
   const T* x2 = p.x2 ? static_cast<const T*>(p.x2) + row * p.ld2 : nullptr;
   const T* gate = p.gate ? static_cast<const T*>(p.gate) + obs * p.gate_stride : nullptr;
-  const float* gain = OP == kRowNorm ? p.gain + obs * p.gain_stride : nullptr;
-  const float* shift = OP == kRowNorm && p.shift ? p.shift + obs * p.shift_stride : nullptr;
-  float rstd = 0.f;
-  const auto value = [&](int e, bool normed) {
-    float v[1] = {to_float(x[e])}, u[1] = {x2 ? to_float(x2[e]) : 0.f};
-    const float gv[1] = {gate ? to_float(gate[e]) : 1.f};
-    row8_combine<OP, 1>(v, u, x2 != nullptr, gate != nullptr, gv);
-    return OP == kRowNorm && normed ? fmaf(gain[e], v[0] * rstd, shift ? shift[e] : 0.f) : v[0];
-  };
-  if constexpr (OP == kRowNorm) {
-    float ss = 0.f;
-    for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-      const float v = value(e, false);
-      if (p.total) static_cast<T*>(p.total)[row * p.h + e] = from_float<T>(v);
-      ss = fmaf(v, v, ss);
+  float ss = 0.f, amax = 0.f;
+#pragma unroll 4
+  for (int e = W * threadIdx.x; e < p.h; e += W * blockDim.x) {
+    float v[W], u[W], g[W];
+    load_few<W>(x + e, v);
+    if (OP != kRowQuant && x2) load_few<W>(x2 + e, u);
+    if (OP == kRowNorm && gate) load_few<W>(gate + e, g);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (OP == kRowGeglu) v[i] = gelu_tanh_f32x2(make_float2(v[i], 0.f)).x * u[i];
+      if constexpr (OP == kRowNorm) {
+        if (x2) v[i] = gate ? fmaf(g[i], u[i], v[i]) : v[i] + u[i];
+        ss = fmaf(v[i], v[i], ss);
+      } else {
+        amax = max_abs(amax, v[i]);
+      }
     }
-    rstd = rsqrtf(block_sum(ss, red_sum) / static_cast<float>(p.h) + p.eps);
+    if (OP == kRowNorm && p.total) store_few<W>(static_cast<T*>(p.total) + row * p.h + e, v);
+    store_few<W>(row8_smem + e, v);
   }
-  float amax = 0.f;
-  for (int e = threadIdx.x; e < p.h; e += blockDim.x) amax = max_abs(amax, value(e, true));
+  if constexpr (OP == kRowNorm) {
+    const float rstd = rsqrtf(block_sum(ss, red_sum) / static_cast<float>(p.h) + p.eps);
+    const float* gain = p.gain + obs * p.gain_stride;
+    const float* shift = p.shift ? p.shift + obs * p.shift_stride : nullptr;
+#pragma unroll 4
+    for (int e = W * threadIdx.x; e < p.h; e += W * blockDim.x) {
+      float v[W], g[W], b[W];
+      load_few<W>(row8_smem + e, v);
+      load_few<W>(gain + e, g);
+#pragma unroll
+      for (int i = 0; i < W; ++i) b[i] = 0.f;
+      if (shift) load_few<W>(shift + e, b);
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        v[i] = fmaf(v[i] * rstd, g[i], b[i]);
+        amax = max_abs(amax, v[i]);
+      }
+      store_few<W>(row8_smem + e, v);
+    }
+  }
   const float scale = __uint_as_float(block_max(abs_key(amax), red_max)) * kInv127;
   const Coder code(scale);
-  for (int e = threadIdx.x; e < p.h; e += blockDim.x) {
-    const float v[1] = {value(e, true)};
-    store_codes<1>(p.codes + row * p.ldc + e, v, code);
+#pragma unroll 4
+  for (int e = W * threadIdx.x; e < p.h; e += W * blockDim.x) {
+    struct alignas(W) Bytes { int8_t x[W]; } c;
+    float v[W];
+    load_few<W>(row8_smem + e, v);
+#pragma unroll
+    for (int i = 0; i < W; ++i) c.x[i] = static_cast<int8_t>(code.fast ? code.quick(v[i]) : code.slow(v[i]));
+    *reinterpret_cast<Bytes*>(p.codes + row * p.ldc + e) = c;
   }
   if (threadIdx.x == 0) p.scale[row] = scale;
 }
 
-// out[r, :] = codes[r, :] * scale[r], rounded once.  W = 16 or 1 codes a
-// thread, `per` threads to a row.
+// out[r, :] = codes[r, :] * scale[r], rounded once.  W = 16, 4 or 1 codes a
+// thread; grid (column groups, rows).
 template <typename T, int W>
 __global__ void __launch_bounds__(256) dequant8_kernel(const int8_t* __restrict__ codes, long long ldc,
                                                        const float* __restrict__ scale, T* __restrict__ out,
-                                                       long long total, int per, int h) {
+                                                       long long rows, int h) {
   pdl_launch_dependents();
   pdl_wait();
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
-  const long long row = i / per;
-  const int e = static_cast<int>(i - row * per) * W;
-  const float s = __ldg(scale + row);
-  if constexpr (W == 16) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * ldc + e));
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  const int e = (blockIdx.x * blockDim.x + threadIdx.x) * W;
+  if (e >= h) return;
+  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float s = __ldg(scale + row);
+    const int8_t* src = codes + row * ldc + e;
+    T* dst = out + row * h + e;
+    if constexpr (W == 16) {
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      float v[8];
+      for (int half = 0; half < 2; ++half) {
+        float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        v[j] = static_cast<float>(static_cast<int8_t>(w[2 * half + (j >> 2)] >> (8 * (j & 3)))) * s;
-      store8(out + row * h + e + 8 * half, v);
+        for (int j = 0; j < 8; ++j)
+          v[j] = static_cast<float>(static_cast<int8_t>(w[2 * half + (j >> 2)] >> (8 * (j & 3)))) * s;
+        store8(dst + 8 * half, v);
+      }
+    } else {
+      struct alignas(W) Bytes { int8_t x[W]; };
+      const Bytes c = *reinterpret_cast<const Bytes*>(src);
+      float v[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) v[i] = static_cast<float>(c.x[i]) * s;
+      store_few<W>(dst, v);
     }
-  } else {
-    out[row * h + e] = from_float<T>(static_cast<float>(codes[row * ldc + e]) * s);
   }
 }
 

@@ -6,7 +6,7 @@
 #include <torch/library.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/util/Exception.h>
@@ -54,6 +54,11 @@ int32_t as_i32(int64_t v, const char* what) {
 
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// A contiguous tensor on x's device, without the dispatcher's way to the same function.
+Tensor empty_on(const Tensor& x, at::IntArrayRef size, at::ScalarType type) {
+  return at::detail::empty_cuda(size, type, x.device(), std::nullopt);
+}
+
 // x [..., h] as rows: [m, h] with unit inner stride (a view where x's strides allow one).
 struct Rows {
   Tensor t;
@@ -74,15 +79,14 @@ Rows rows_of(const Tensor& x) {
 Tensor empty_codes(const Tensor& x, int64_t m, int64_t* ld) {
   const int64_t h = x.size(-1);
   *ld = h <= 128 ? (h + 15) / 16 * 16 : (h + 127) / 128 * 128;
-  const auto opts = x.options().dtype(at::kChar);
-  if (*ld == h) return at::empty(x.sizes(), opts);
+  if (*ld == h) return empty_on(x, x.sizes(), at::kChar);
   std::vector<int64_t> stride(x.dim(), 1);
   int64_t step = *ld;
   for (int64_t i = x.dim() - 2; i >= 0; --i) {
     stride[i] = step;
     step *= x.size(i);
   }
-  return at::empty({m * *ld}, opts).as_strided(x.sizes(), stride);
+  return empty_on(x, {m * *ld}, at::kChar).as_strided(x.sizes(), stride);
 }
 
 void check_rows(const Tensor& x, const char* what) {
@@ -130,8 +134,8 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_quant(const Tensor& x, const Tensor&
   const Rows dr = delta.has_value() ? rows_of(*delta) : Rows{Tensor(), 0, 0};
   int64_t ldc;
   Tensor codes = empty_codes(x, xr.m, &ldc);
-  Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
-  Tensor total = delta.has_value() ? at::empty(x.sizes(), x.options()) : at::empty({0}, x.options());
+  Tensor scale = empty_on(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
+  Tensor total = empty_on(x, delta.has_value() ? x.sizes() : at::IntArrayRef({0}), x.scalar_type());
   if (xr.m == 0) return {codes, scale, total};
   const int64_t per_batch = x.dim() >= 2 ? xr.m / x.size(0) : 1;
   check_status(w4a4_rms_norm_quant8(
@@ -156,7 +160,7 @@ std::tuple<Tensor, Tensor> quantize(const Tensor& x, const OptTensor& up) {
   const Rows ur = up.has_value() ? rows_of(*up) : Rows{Tensor(), 0, 0};
   int64_t ldc;
   Tensor codes = empty_codes(x, xr.m, &ldc);
-  Tensor scale = at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat));
+  Tensor scale = empty_on(x, x.sizes().slice(0, x.dim() - 1), at::kFloat);
   if (xr.m == 0) return {codes, scale};
   check_status(w4a4_quant8(xr.data(), xr.ld, up.has_value() ? ur.data() : nullptr, ur.ld, dt, xr.m,
                            as_i32(x.size(-1), "the row length"), codes.data_ptr<int8_t>(), ldc,
@@ -180,7 +184,7 @@ Tensor dequantize(const Tensor& codes, const Tensor& scale, at::ScalarType dtype
   const int32_t dt = dtype_code(dtype, true, "dtype");
   const Rows r = check_codes(codes, scale, "codes", "scale");
   c10::cuda::CUDAGuard guard(codes.device());
-  Tensor out = at::empty(codes.sizes(), codes.options().dtype(dtype));
+  Tensor out = empty_on(codes, codes.sizes(), dtype);
   check_status(w4a4_dequant8(static_cast<const int8_t*>(r.data()), r.ld, scale.const_data_ptr<float>(), dt, r.m,
                              as_i32(codes.size(-1), "the row length"), out.data_ptr(), stream_of(codes)));
   return out;
@@ -198,7 +202,7 @@ Rows tma_rows(Rows r, const char* what) {
                   " do not begin at multiples of 16 bytes; copying them on every call. quantize, rms_norm_quant and "
                   "pack_weight lay them out.");
   const int64_t ld = (k + 127) / 128 * 128;
-  Tensor t = at::empty({r.m, ld}, r.t.options()).narrow(1, 0, k);
+  Tensor t = empty_on(r.t, {r.m, ld}, at::kChar).narrow(1, 0, k);
   t.copy_(r.t);
   return {t, r.m, ld};
 }
@@ -226,7 +230,7 @@ Tensor linear(const Tensor& codes, const Tensor& scale, const Tensor& weight, co
   }
   std::vector<int64_t> shape(codes.sizes().begin(), codes.sizes().end());
   shape.back() = n;
-  Tensor y = at::empty(shape, codes.options().dtype(dtype));
+  Tensor y = empty_on(codes, shape, dtype);
   if (a.m == 0) return y;
   a = tma_rows(a, "codes");
   w = tma_rows(w, "weight");
@@ -304,7 +308,7 @@ Tensor kv_append(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_s
   c10::cuda::CUDAGuard guard(k_cache.device());
   if (valid.has_value()) mask = valid->stride(1) == 1 || tokens <= 1 ? *valid : valid->contiguous();
   const Tensor kr = with_rows(k, 1), vr = with_rows(v, 1);
-  Tensor lengths = at::empty({c.batch}, start.options());
+  Tensor lengths = empty_on(start, {c.batch}, at::kInt);
   if (c.batch == 0) return lengths;
   const int64_t ks[3] = {kr.stride(0), kr.stride(1), kr.stride(2)}, vs[3] = {vr.stride(0), vr.stride(1), vr.stride(2)};
   check_status(w4a4_kv8_append(
@@ -323,8 +327,8 @@ std::tuple<Tensor, Tensor> kv_values(const Tensor& k_cache, const Tensor& v_cach
   const int32_t dt = dtype_code(dtype, true, "dtype");
   const int32_t* len = check_lengths(lengths, k_cache, "lengths");
   c10::cuda::CUDAGuard guard(k_cache.device());
-  Tensor k = at::empty(k_cache.sizes(), k_cache.options().dtype(dtype));
-  Tensor v = at::empty(k_cache.sizes(), k_cache.options().dtype(dtype));
+  Tensor k = empty_on(k_cache, k_cache.sizes(), dtype);
+  Tensor v = empty_on(k_cache, k_cache.sizes(), dtype);
   if (c.batch == 0) return {k, v};
   check_status(w4a4_kv8_values(k_cache.const_data_ptr<int8_t>(), v_cache.const_data_ptr<int8_t>(),
                                k_scale.const_data_ptr<float>(), v_scale.const_data_ptr<float>(), c.stride,
@@ -344,7 +348,7 @@ Tensor kv_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
   const int32_t* len = check_lengths(lengths, k_cache, "lengths");
   c10::cuda::CUDAGuard guard(k_cache.device());
   const Tensor qr = with_rows(q, 8);
-  Tensor out = at::empty(q.sizes(), q.options());
+  Tensor out = empty_on(q, q.sizes(), q.scalar_type());
   if (q.numel() == 0) return out;
   const int64_t qs[3] = {qr.stride(0), qr.stride(1), qr.stride(2)};
   int64_t bytes = 0;
@@ -352,7 +356,7 @@ Tensor kv_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
                                          as_i32(q.size(2), "the query head count"), as_i32(c.heads, "the head count"),
                                          as_i32(c.width, "the head width"), as_i32(c.capacity, "the capacity"), &bytes));
   Tensor workspace;
-  if (bytes > 0) workspace = at::empty({bytes}, q.options().dtype(at::kByte));
+  if (bytes > 0) workspace = empty_on(q, {bytes}, at::kByte);
   check_status(w4a4_attention8(qr.const_data_ptr(), qs, k_cache.const_data_ptr<int8_t>(),
                                v_cache.const_data_ptr<int8_t>(), k_scale.const_data_ptr<float>(),
                                v_scale.const_data_ptr<float>(), c.stride, as_i32(c.capacity, "the capacity"), len, dt,

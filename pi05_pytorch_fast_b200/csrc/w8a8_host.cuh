@@ -73,18 +73,18 @@ int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* wh
   if (p.rows > 0x7fffffffLL) return fail(W4A4_ERR_UNSUPPORTED, "%s: too many rows: %lld", what, (long long)p.rows);
   const int size = elem_size(dtype);
   // The 8-element path wants 16-byte vectors of every operand and 8-byte
-  // vectors of codes; anything else goes one element at a time.
+  // vectors of codes.
   bool vec = p.h % 8 == 0 && rows_aligned(p.x, p.ldx, size, 16) && rows_aligned(p.codes, p.ldc, 1, 8);
   if (p.x2) vec = vec && rows_aligned(p.x2, p.ld2, size, 16);
   if (p.gate) vec = vec && rows_aligned(p.gate, p.gate_stride, size, 16);
   if (p.gain) vec = vec && rows_aligned(p.gain, p.gain_stride, 4, 16);
   if (p.shift) vec = vec && rows_aligned(p.shift, p.shift_stride, 4, 16);
   if (p.total) vec = vec && aligned(p.total, 16);
-  int dev, sms;
-  if (int e = current_device(&dev)) return e;
-  if (int e = sm_count(dev, &sms)) return e;
   return by_dtype(dtype, true, what, [&](auto tag) {
     using T = decltype(tag);
+    int dev, sms;
+    if (int e = current_device(&dev)) return e;
+    if (int e = sm_count(dev, &sms)) return e;
     // as many CTAs as run at once (2,048 threads and 64 K registers of an SM), each with its share of the rows
     const auto go = [&](void (*kernel)(const Row8Params), int groups, int vpt, int regs) {
       const int threads = (((groups + vpt - 1) / vpt) + 31) / 32 * 32;
@@ -101,10 +101,30 @@ int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* wh
       if (groups <= 2048) return go(row8_kernel<T, OP, 8, 4, 512, 1>, groups, 4, 128);
       return go(row8_kernel<T, OP, 8, 4, 1024, 1>, groups, 4, 64);
     }
-    if (p.h <= 1024) return go(row8_kernel<T, OP, 1, 4, 256, 4>, p.h, 4, 64);
-    if (p.h <= kRow8MaxScalar) return go(row8_kernel<T, OP, 1, 16, 1024, 1>, p.h, 16, 64);
-    const dim3 grid(static_cast<unsigned>(p.rows));
-    return cuda_status(launch_kernel(row8_long_kernel<T, OP>, grid, dim3(1024), 0, stream, 1, p)) ? W4A4_ERR_CUDA : ok();
+    if (p.h > kRow8AnyMax)
+      return fail(W4A4_ERR_UNSUPPORTED, "%s: rows of more than %d elements are not supported", what, kRow8AnyMax);
+    // elements at a time: what the length and every operand's rows allow
+    const auto together = [&](int w) {
+      bool fits = p.h % w == 0 && rows_aligned(p.x, p.ldx, size, w * size) && rows_aligned(p.codes, p.ldc, 1, w);
+      if (p.x2) fits = fits && rows_aligned(p.x2, p.ld2, size, w * size);
+      if (p.gate) fits = fits && rows_aligned(p.gate, p.gate_stride, size, w * size);
+      if (p.gain) fits = fits && rows_aligned(p.gain, p.gain_stride, 4, w * 4);
+      if (p.shift) fits = fits && rows_aligned(p.shift, p.shift_stride, 4, w * 4);
+      if (p.total) fits = fits && aligned(p.total, w * size);
+      return fits;
+    };
+    const int w = together(4) ? 2 : together(2) ? 1 : 0;
+    const auto kernel = w == 2 ? row8_any_kernel<T, OP, 4> : w == 1 ? row8_any_kernel<T, OP, 2> : row8_any_kernel<T, OP, 1>;
+    const int bytes = p.h * 4;
+    if (bytes > 40 * 1024) {
+      const int bit = 32 + w + 3 * OP + 9 * (std::is_same_v<T, float> ? 0 : std::is_same_v<T, __half> ? 1 : 2);
+      if (int e = ensure_smem_attr8(dev, bit, kernel, kRow8AnyMax * 4)) return e;
+    }
+    // four steps of a row a thread, up to 256 threads
+    const int each = 4 << w, threads = std::min(kRow8AnyThreads, ((p.h + each - 1) / each + 31) / 32 * 32);
+    return cuda_status(launch_kernel(kernel, dim3(static_cast<unsigned>(p.rows)), dim3(threads), bytes, stream, 1, p))
+               ? W4A4_ERR_CUDA
+               : ok();
   });
 }
 
@@ -167,11 +187,13 @@ Gemm8Plan gemm8_plan(int64_t m, int n, int k, const int (&fit)[4]) {
   return best;
 }
 
-// Clusters of 1, 2, 4 and 8 CTAs of the tile kernel that the device runs at once.
-int g_gemm8_fit[kMaxDevices][4];
-int gemm8_fit(int dev, int sms, int (&fit)[4]) {
+// Clusters of 1, 2, 4 and 8 CTAs that the device runs at once with one CTA to an SM.
+int g_cluster_fit[kMaxDevices][4];
+int cluster_fit(int dev, int (&fit)[4]) {
+  int sms;
+  if (int e = sm_count(dev, &sms)) return e;
   std::lock_guard<std::mutex> lk(g_dev_mu);
-  int(&f)[4] = g_gemm8_fit[dev];
+  int(&f)[4] = g_cluster_fit[dev];
   if (f[0] == 0) {
     W4A4_CUDA_TRY(cudaFuncSetAttribute(gemm8_tile_kernel<__half>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit));
     for (int i = 1; i < 4; ++i) {
@@ -222,7 +244,7 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     });
   }
   int fit[4];
-  if (int e = gemm8_fit(dev, sms, fit)) return e;
+  if (int e = cluster_fit(dev, fit)) return e;
   const Gemm8Plan plan = gemm8_plan(m, n, k, fit);
   Gemm8Params p;
   if (int e = gemm8_codes_map(&p.tmap_a, a, k, m, lda, plan.pair ? 128 : plan.tok_tile)) return e;
@@ -278,21 +300,29 @@ int check_cache8(const void* k, const void* v, const void* ks, const void* vs, c
 
 // How many CTAs the keys of one key/value head are split over, from the
 // cache's capacity (the lengths are on the device; a split without keys writes
-// an empty part).
+// an empty part).  Up to 8 CTAs of the few-rows form are a cluster, as long as
+// all clusters run at once: `fit[i]` of 1 << i CTAs.
 constexpr int kAttn8FewRows = 16;
 struct Attn8Plan {
   bool few;
   int tiles;   // row tiles of the many-rows form
   int splits;
 };
-Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, int sms) {
+Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, const int (&fit)[4]) {
   Attn8Plan plan{};
   plan.few = rows <= kAttn8FewRows;
   plan.tiles = static_cast<int>((rows + 127) / 128);
   const int64_t work = units * (plan.few ? 1 : plan.tiles);
-  // keys that make a split worth its part of the join
+  // splits that the keys are worth (a CTA's warps and three tiles of 64 keys take that many at a time), and that the
+  // SMs have room for
   const int64_t most = plan.few ? (capacity + 127) / 128 : (capacity + 191) / 192;
-  plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, sms / std::max<int64_t>(work, 1), 256})));
+  const int64_t room = fit[0] / std::max<int64_t>(work, 1);
+  plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, room, 256})));
+  if (plan.few && plan.splits <= 8) {
+    int i = 3;
+    while (i > 0 && ((1 << i) > plan.splits || units > fit[i])) --i;
+    plan.splits = 1 << i;
+  }
   return plan;
 }
 
@@ -397,15 +427,17 @@ int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t 
                   void* out, void* stream) {
   if (int e = check_rows8(rows, h, out, h, codes, ldc, scale, "dequant8")) return e;
   if (rows == 0) return ok();
-  const bool vec = h % 16 == 0 && rows_aligned(codes, ldc, 1, 16) && aligned(out, 16);
+  const int size = elem_size(dtype);
+  const int w = h % 16 == 0 && rows_aligned(codes, ldc, 1, 16) && aligned(out, 16)        ? 16
+                : h % 4 == 0 && rows_aligned(codes, ldc, 1, 4) && aligned(out, 4 * size) ? 4
+                                                                                         : 1;
   return by_dtype(dtype, true, "dequant8", [&](auto tag) {
     using T = decltype(tag);
-    const int per = vec ? h / 16 : h;
-    const int64_t total = rows * per, blocks = (total + 255) / 256;
-    if (blocks > 0x7fffffffLL) return fail(W4A4_ERR_UNSUPPORTED, "dequant8: too many values");
-    const auto kernel = vec ? dequant8_kernel<T, 16> : dequant8_kernel<T, 1>;
-    return cuda_status(launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream),
-                                     1, codes, ldc, scale, static_cast<T*>(out), total, per, h))
+    const int groups = (h + w - 1) / w, threads = std::min(256, (groups + 31) / 32 * 32);
+    const dim3 grid((groups + threads - 1) / threads, static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
+    const auto kernel = w == 16 ? dequant8_kernel<T, 16> : w == 4 ? dequant8_kernel<T, 4> : dequant8_kernel<T, 1>;
+    return cuda_status(launch_kernel(kernel, grid, dim3(threads), 0, static_cast<cudaStream_t>(stream), 1, codes, ldc, scale,
+                                     static_cast<T*>(out), rows, h))
                ? W4A4_ERR_CUDA
                : ok();
   });
@@ -494,11 +526,11 @@ int w4a4_attention8_workspace(int32_t batch, int32_t tokens, int32_t q_heads, in
     return fail(W4A4_ERR_INVALID, "attention8: invalid shape");
   *bytes = 0;
   if (batch == 0 || tokens == 0) return ok();
-  int dev, sms;
+  int dev, fit[4];
   if (int e = current_device(&dev)) return e;
-  if (int e = sm_count(dev, &sms)) return e;
+  if (int e = cluster_fit(dev, fit)) return e;
   const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
-  const Attn8Plan plan = attn8_plan(units, rows, capacity, sms);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, fit);
   if (plan.splits > 1) *bytes = units * plan.splits * rows * (static_cast<int64_t>(width) * 4 + 8);
   return ok();
 }
@@ -520,11 +552,11 @@ int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_code
     return fail(W4A4_ERR_INVALID, "attention8: query rows must begin at multiples of 16 bytes");
   if (static_cast<int64_t>(batch) * tokens * q_heads > 0x7fffffffLL)
     return fail(W4A4_ERR_UNSUPPORTED, "attention8: too many query rows");
-  int dev, sms;
+  int dev, fit[4];
   if (int e = current_device(&dev)) return e;
-  if (int e = sm_count(dev, &sms)) return e;
+  if (int e = cluster_fit(dev, fit)) return e;
   const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
-  const Attn8Plan plan = attn8_plan(units, rows, capacity, sms);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, fit);
   Attn8Params p{};
   p.q = q, p.out = out, p.k = k_codes, p.v = v_codes, p.ks = k_scale, p.vs = v_scale, p.lengths = lengths;
   p.qb = q_stride[0], p.qt = q_stride[1], p.qh = q_stride[2];
