@@ -81,6 +81,9 @@ def parse_args():
     ap.add_argument("--snapflow", action="store_true",
                     help="config 4: the SnapFlow 1-NFE action chunk (SigLIP + the W4A4 prefix LM + the "
                          "action expert); --batch observations per GPU (config 4: 64 over 8 GPUs)")
+    ap.add_argument("--expert-bits", type=int, choices=(8, 16), default=16,
+                    help="with --snapflow: the action expert's layers in bf16 (16, the default) or on the "
+                         "8-bit operators (8)")
     ap.add_argument("--case", choices=("qkv", "o", "gateup", "down", "quant2k", "quant16k",
                                        "normquant", "geglu", "attn", "forward", "snapflow"),
                     default=None, help="run one op (or one forward) 3 times at the bench shape and "
@@ -657,7 +660,8 @@ def run_snapflow(args, rank, world, local_rank, dist_on) -> dict:
     ext.preload()
     cfg = sf.SnapFlowConfig()
     lm = plm.W4A4PrefixLM.random(cfg.lm, device, seed=1234)
-    policy = sf.SnapFlowPolicy(cfg, lm, device, seed=4321)
+    policy = sf.SnapFlowPolicy(cfg, lm, device, seed=4321, expert_bits=args.expert_bits)
+    own_expert = args.expert_bits == 8
     b = args.batch
     obs = sf.synthetic_observation(cfg, b, seed=300 + rank, device=device)
     with torch.no_grad():
@@ -700,8 +704,9 @@ def run_snapflow(args, rank, world, local_rank, dist_on) -> dict:
         "higher_is_better": True,
         "scaling": "weak",
         "vs_baseline": None,
-        "dtype": "bf16 SigLIP-So400m and action expert (cuBLAS / SDPA); the prefix LM W4A4 (int4 x int4 "
-                 "-> int32 on tcgen05, fp16 activations)",
+        "dtype": ("bf16 SigLIP-So400m (cuBLAS / SDPA); the action expert's layers int8 weights, activations and "
+                  "KV cache" if own_expert else "bf16 SigLIP-So400m and action expert (cuBLAS / SDPA)")
+                 + "; the prefix LM W4A4 (int4 x int4 -> int32 on tcgen05, fp16 activations)",
         "data": "synthetic: random-init weights (N(0, 0.02)); 2 real cameras of 224 x 224 pixels ~ U[-1, 1], "
                 "the empty camera cached and pooled 4:1, 200 language tokens (52 real ids), noise ~ N(0, 1)",
         "config": {
@@ -714,9 +719,12 @@ def run_snapflow(args, rank, world, local_rank, dist_on) -> dict:
             "l2": "weights ~2.9 GB per step >> 126 MB L2 (no flush needed)",
         },
         "stages_ms": stages,
-        "gpu_launches": lm.launches_per_forward() * args.steps,
-        "gpu_launches_note": "kernels of libw4a4_sm100.so per timed region (the prefix LM); SigLIP and "
-                             "the expert run cuBLAS / PyTorch kernels",
+        "gpu_launches": (lm.launches_per_forward() + (policy.expert.launches_per_forward() if own_expert else 0))
+                        * args.steps,
+        "gpu_launches_note": ("kernels of libw4a4_sm100.so per timed region (the prefix LM and the expert's layers); "
+                              "SigLIP runs cuBLAS / PyTorch kernels" if own_expert else
+                              "kernels of libw4a4_sm100.so per timed region (the prefix LM); SigLIP and "
+                              "the expert run cuBLAS / PyTorch kernels"),
         "clocks": clocks.summary(),
         "e2e": {
             "value": job_throughput(ms_e2e, b, world),

@@ -41,6 +41,10 @@ The exact lerobot module layout (and so a checkpoint's tensor names) is not
 reproduced; shapes, dtypes, masks, positions and the order of operations
 are.  ``GraphedSnapFlow`` captures the whole step (SigLIP, the prefix
 assembly, the W4A4 prefix LM, the expert) in one CUDA graph.
+
+``SnapFlowPolicy(..., expert_bits=8)`` runs the expert's layers on the 8-bit
+operators instead (``ActionExpert8``): weights, activations and the key/value
+cache as int8 codes with fp32 scales.
 """
 
 from __future__ import annotations
@@ -54,6 +58,7 @@ from torch import nn
 
 from . import _native as nat
 from . import prefix_lm as plm
+from . import w8a8
 
 
 @dataclass(frozen=True)
@@ -264,10 +269,10 @@ class ActionExpert(nn.Module):
             emb = emb + self.target_time_mlp(tt.to(dt))
         return F.silu(self.time_mlp_out(F.silu(self.time_mlp_in(emb))))
 
-    def forward(self, x_t, t, target_t, prefix_pad, keys, values) -> torch.Tensor:
-        """x_t [B, chunk, action_dim] in the expert's dtype; prefix_pad bool
-        [B, L]; keys / values: per layer [B, L, kv_heads * hd] (any float
-        dtype).  Returns v_t [B, chunk, action_dim] in the expert's dtype."""
+    def prepare(self, x_t, t, target_t, prefix_pad):
+        """What the layers start from: x [B, chunk, h]; mod, each norm's (1 +
+        scale, shift) in fp32 and gate, all [B, h]; rope, the rotary tables in
+        the form that ``ExpertLayer`` takes."""
         cfg = self.cfg
         dt = self.action_in_proj.weight.dtype
         b, s, h = x_t.shape[0], cfg.chunk, cfg.expert_hidden
@@ -285,6 +290,16 @@ class ActionExpert(nn.Module):
                     sin[:, 0].reshape(b * s, cfg.head_dim).contiguous())
         else:
             rope = (cos.transpose(1, 2), signed_sin(sin.transpose(1, 2)))
+        return x, mod, rope
+
+    def forward(self, x_t, t, target_t, prefix_pad, keys, values) -> torch.Tensor:
+        """x_t [B, chunk, action_dim] in the expert's dtype; prefix_pad bool
+        [B, L]; keys / values: per layer [B, L, kv_heads * hd] (any float
+        dtype).  Returns v_t [B, chunk, action_dim] in the expert's dtype."""
+        cfg = self.cfg
+        dt = self.action_in_proj.weight.dtype
+        b, s = x_t.shape[0], cfg.chunk
+        x, mod, rope = self.prepare(x_t, t, target_t, prefix_pad)
         # the prefix's real tokens and every suffix token are visible
         visible = torch.cat((prefix_pad, torch.ones((b, s), dtype=torch.bool, device=x.device)), dim=1)
         mask_add = torch.zeros(visible.shape, dtype=dt, device=x.device).masked_fill_(
@@ -296,6 +311,86 @@ class ActionExpert(nn.Module):
             x = layer(x, mod[2 * i], mod[2 * i + 1], rope, pk, pv, mask_add)
         x, _ = ada_rms_norm(x, mod[-1], cfg.rms_eps)
         return self.action_out_proj(x[:, -s:])
+
+
+class ExpertLayer8:
+    """An ``ExpertLayer``'s weights in 8 bits (q, k and v as one matrix, gate
+    and up as another) and its forward on the 8-bit operators.  The residual
+    sum, the two norms and their codes are one kernel each; the attention reads
+    the 8-bit cache, so no mask and no copy of the prefix's keys is made."""
+
+    def __init__(self, layer: ExpertLayer):
+        self.heads, self.kv_heads, self.hd, self.eps = layer.heads, layer.kv_heads, layer.hd, layer.eps
+        self.qkv = w8a8.pack_weight(torch.cat((layer.q.weight, layer.k.weight, layer.v.weight)))
+        self.o = w8a8.pack_weight(layer.o.weight)
+        self.gate_up = w8a8.pack_weight(torch.cat((layer.gate.weight, layer.up.weight)))
+        self.down = w8a8.pack_weight(layer.down.weight)
+
+    def forward(self, x, delta, gate, mod_in, mod_post, rope, cache, prefix_k, prefix_v, prefix_pad, empty):
+        """x [B, S, h], the residual before the previous layer's last sublayer
+        ``delta`` [B, S, h] and its ``gate`` [B, h] are added (None in the first
+        layer); prefix_k / prefix_v [B, L, kv_heads, hd] (keys after RoPE), of
+        which the tokens of prefix_pad [B, L] are kept; cache for L + S tokens;
+        empty int32 zeros [B].  Returns (x, delta, gate) for the next layer."""
+        b, s, _ = x.shape
+        qh, kvh, hd = self.heads, self.kv_heads, self.hd
+        codes, scale, x = w8a8.rms_norm_quant(x, mod_in[0], self.eps, delta=delta, gate=gate, shift=mod_in[1])
+        qkv = w8a8.linear(codes, scale, self.qkv).view(b, s, qh + 2 * kvh, hd)
+        q, k, v = qkv.split((qh, kvh, kvh), dim=2)
+        row = (qh + 2 * kvh) * hd
+        nat.check(nat.lib().w4a4_rope_qk_bf16(q.data_ptr(), row, qh, k.data_ptr(), row, kvh, rope[0].data_ptr(),
+                                              rope[1].data_ptr(), b * s, hd, _stream()))
+        lengths = w8a8.kv_append(cache, prefix_k, prefix_v, empty, valid=prefix_pad)
+        lengths = w8a8.kv_append(cache, k, v, lengths)
+        a = w8a8.kv_attention(q, cache, lengths).view(b, s, qh * hd)
+        delta = w8a8.linear(*w8a8.quantize(a), self.o)
+        codes, scale, x = w8a8.rms_norm_quant(x, mod_post[0], self.eps, delta=delta, gate=mod_in[2], shift=mod_post[1])
+        gate, up = w8a8.linear(codes, scale, self.gate_up).chunk(2, dim=-1)
+        return x, w8a8.linear(*w8a8.quantize(gate, up), self.down), mod_post[2]
+
+
+class ActionExpert8(ActionExpert):
+    """An ``ActionExpert`` (bf16, on the GPU) with its layers in 8 bits.  The
+    condition, the action projections and the final norm are the given
+    expert's; its layers are read once, for their weights."""
+
+    def __init__(self, expert: ActionExpert):
+        nn.Module.__init__(self)
+        if not _on_kernels(expert.modulation.weight):
+            raise ValueError("the 8-bit action expert is made from a bf16 expert on a CUDA device")
+        self.cfg, self.n_norms = expert.cfg, expert.n_norms
+        for name, module in expert.named_children():
+            if name != "layers":
+                setattr(self, name, module)
+        with torch.no_grad():
+            self.layers = [ExpertLayer8(layer) for layer in expert.layers]
+        self._caches: dict = {}
+
+    def _cache(self, b: int, tokens: int, device) -> tuple[w8a8.KVCache8, torch.Tensor]:
+        # one cache for all layers: each fills it from its first slot again
+        key = (b, tokens)
+        if key not in self._caches:
+            self._caches[key] = (w8a8.KVCache8.allocate(b, tokens, self.cfg.expert_kv_heads, self.cfg.head_dim, device),
+                                 torch.zeros(b, dtype=torch.int32, device=device))
+        return self._caches[key]
+
+    def launches_per_forward(self) -> int:
+        """Kernels of the layers (the attention counted as one)."""
+        return 12 * len(self.layers)
+
+    def forward(self, x_t, t, target_t, prefix_pad, keys, values) -> torch.Tensor:
+        """As ``ActionExpert.forward``; keys and values fp16 or bf16."""
+        cfg = self.cfg
+        b = x_t.shape[0]
+        x, mod, rope = self.prepare(x_t, t, target_t, prefix_pad)
+        cache, empty = self._cache(b, prefix_pad.shape[1] + cfg.chunk, x.device)
+        delta = gate = None
+        for i, (layer, k, v) in enumerate(zip(self.layers, keys, values)):
+            pk, pv = (a.view(b, -1, cfg.expert_kv_heads, cfg.head_dim) for a in (k, v))
+            x, delta, gate = layer.forward(x, delta, gate, mod[2 * i], mod[2 * i + 1], rope, cache, pk, pv,
+                                           prefix_pad, empty)
+        x, _ = ada_rms_norm(torch.addcmul(x, gate[:, None], delta), mod[-1], cfg.rms_eps)
+        return self.action_out_proj(x)
 
 
 class SiglipTower(nn.Module):
@@ -398,10 +493,13 @@ class SnapFlowPolicy:
     """The config-4 step on one GPU: ``sample_actions(images, lang_ids,
     lang_mask, noise)`` -> actions [B, chunk, action_dim] = x_t - v_t, x_t the
     noise in the expert's dtype and v_t the expert's velocity at t = target
-    t = 1, in the noise's dtype (snapflow_pi05.py:170-195)."""
+    t = 1, in the noise's dtype (snapflow_pi05.py:170-195).  ``expert_bits``:
+    16 (the expert's layers in ``dtype``) or 8 (``ActionExpert8``)."""
 
     def __init__(self, cfg: SnapFlowConfig, lm: plm.W4A4PrefixLM, device, seed: int = 0,
-                 dtype=torch.bfloat16, std: float = 0.02):
+                 dtype=torch.bfloat16, std: float = 0.02, expert_bits: int = 16):
+        if expert_bits not in (8, 16):
+            raise ValueError(f"expert_bits is 8 or 16, not {expert_bits}")
         self.cfg, self.lm, self.device, self.dtype = cfg, lm, torch.device(device), dtype
         torch.manual_seed(seed)
         with torch.device(self.device):
@@ -412,6 +510,8 @@ class SnapFlowPolicy:
                 if p.dim() >= 2 and "embeddings" not in name:
                     nn.init.normal_(p, std=std)
             mod.to(dtype).eval()
+        if expert_bits == 8:
+            self.expert = ActionExpert8(self.expert)
         gen = torch.Generator(device=self.device).manual_seed(seed + 1)
         self.lang_table = torch.randn(cfg.vocab, cfg.lm.hidden, device=self.device, generator=gen,
                                       dtype=torch.float16)

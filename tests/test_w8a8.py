@@ -14,6 +14,7 @@ import pytest
 import torch
 
 from pi05_pytorch_fast_b200 import _native as nat
+from pi05_pytorch_fast_b200 import snapflow as sf
 from pi05_pytorch_fast_b200 import w8a8
 
 DEV = "cuda:0"
@@ -740,3 +741,89 @@ def test_ops_refuse_bad_arguments():
     refuses("cache scales must be", lambda: w8a8.kv_values(cache._replace(key_scale=cache.key_scale[..., :1]), n))
     wide = w8a8.KVCache8.allocate(2, 32, 2, 72, DEV)
     refuses("64, 128 or 256", lambda: w8a8.kv_values(wide, n))
+
+
+# --- the operators together: the SnapFlow action expert in 8 bits -----------
+
+
+def _expert(layers=2, seed=3):
+    """A bf16 expert of the published width, an 8-bit one of its weights, and
+    inputs of two observations with different prefix lengths (40 slots)."""
+    dev = torch.device("cuda:0")
+    cfg = sf.SnapFlowConfig(expert_layers=layers)
+    torch.manual_seed(seed)
+    with torch.device(dev):
+        expert = sf.ActionExpert(cfg)
+    for p in expert.parameters():
+        if p.dim() >= 2:
+            torch.nn.init.normal_(p, std=0.02)
+    expert = expert.bfloat16().eval()
+    g = torch.Generator(device=dev).manual_seed(seed + 1)
+    pad = torch.zeros(2, 40, dtype=torch.bool, device=dev)
+    pad[0, :33] = True
+    pad[1, 5:40:3] = True
+    kv = [[torch.randn(2, 40, 256, device=dev, generator=g).half() for _ in range(layers)] for _ in range(2)]
+    x_t = torch.randn(2, cfg.chunk, cfg.action_dim, device=dev, generator=g).bfloat16()
+    return expert, (x_t, torch.ones(2, device=dev), torch.ones(2, device=dev), pad, *kv)
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_against_fp64():
+    """Relative error of the velocity.  A rounding to 127 steps of a row's
+    largest value, r times the row's RMS, has a relative error r / (127
+    sqrt(12)): 0.8 % for normal rows of 1,024 to 2,048 (r = 3.5), and at most
+    2.3 % for the GeGLU product (r = 10).  Along the attention branch: norm
+    codes and weights 1.1 %, keys and values 0.8 %, codes and weights of the
+    output product 1.1 %, together under 2 %; along the MLP: 1.1 % on each
+    factor, 2.3 % on their product, 0.8 % weights, together under 3 %.  The
+    branches of two layers are summed, so their relative error is no more than
+    one's plus what a layer passes on from the one before it (under 3 % again):
+    6 %, and 1 % for bf16."""
+    expert, inputs = _expert()
+    expert8 = sf.ActionExpert8(expert)
+    expert64 = sf.ActionExpert(expert.cfg).to("cuda:0").double()
+    expert64.load_state_dict(expert.state_dict())
+    with torch.no_grad():
+        v = expert8(*inputs)
+        ref = expert64(inputs[0].double(), *inputs[1:])
+    assert v.shape == ref.shape and v.dtype == torch.bfloat16
+    rel = (v.double() - ref).norm() / ref.norm()
+    assert rel < 0.07, float(rel)
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_masked_prefix_and_reuse():
+    """What stands in masked prefix slots does not matter, neither does what an
+    earlier call left in the cache; a call of another batch in between neither."""
+    expert, inputs = _expert(layers=1)
+    expert8 = sf.ActionExpert8(expert)
+    x_t, t, target, pad, keys, values = inputs
+    with torch.no_grad():
+        v = expert8(*inputs)
+        other = expert8(x_t[:1], t[:1], target[:1], ~pad[:1], [k[:1] for k in keys], [k[:1] * 7 for k in values])
+        junk = [[torch.where(pad[..., None], k, torch.tensor(bad, dtype=k.dtype, device=k.device)) for k in kv]
+                for kv, bad in ((keys, math.nan), (values, math.inf))]
+        expert8(x_t * 5, t, target, ~pad, [k * 9 for k in keys], [k * 9 for k in values])
+        again = expert8(x_t, t, target, pad, *junk)
+    assert torch.equal(v, again) and torch.isfinite(other).all()
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_in_a_graph():
+    expert, inputs = _expert(layers=1)
+    expert8 = sf.ActionExpert8(expert)
+    with torch.no_grad():
+        eager = expert8(*inputs)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = expert8(*inputs)
+        graph.replay()
+    assert torch.equal(out, eager)
+
+
+def test_snapflow_expert_in_8_bits_refusals():
+    cfg = sf.SnapFlowConfig(expert_layers=1, expert_hidden=32, expert_intermediate=32, head_dim=64)
+    with pytest.raises(ValueError, match="bf16 expert on a CUDA device"):
+        sf.ActionExpert8(sf.ActionExpert(cfg))
+    with pytest.raises(ValueError, match="expert_bits is 8 or 16"):
+        sf.SnapFlowPolicy(cfg, None, "cpu", expert_bits=4)
