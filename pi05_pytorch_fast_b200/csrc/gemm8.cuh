@@ -72,12 +72,6 @@ struct G8Channels {
   }
 };
 
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-
 // Shared memory: the ring of `stages` (16 KB of weights, T rows of tokens),
 // which the sums [T][128] and what the other CTAs of the cluster send take
 // over once the products are done; token scales; barriers.
@@ -99,7 +93,7 @@ __global__ void __launch_bounds__(kG8TileThreads) gemm8_tile_kernel(const __grid
   extern __shared__ uint8_t g8_smem[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(g8_smem) + 1023) & ~static_cast<uintptr_t>(1023));
   const int S = p.stages, tok_bytes = p.tok_tile * kG8StepBytes;
-  const int ranks = static_cast<int>(cluster_size()), rank = static_cast<int>(cluster_ctarank());
+  const int ranks = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
   uint8_t* w_ring = base;                    // [S][16 KB]
   uint8_t* t_ring = base + S * kG8ABytes;    // [S][T x 128]
   int* sums = reinterpret_cast<int*>(base);  // [T][128], after the products

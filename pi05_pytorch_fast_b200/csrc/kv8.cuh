@@ -13,8 +13,12 @@
 // anew (its first slot is >= start[b]) forgets its old scale.  An infinity or
 // NaN among x makes the block's scale non-finite and its codes zero.
 //
-// Bound: HBM, or the launch for a few tokens (2 bytes read and 1 written per
-// value).  One CTA per block, head and {keys, values}.
+// Bound: HBM (2 bytes read and 1 written per value), or for short appends the
+// chain of loads flags -> tokens -> codes.  One CTA per block and head for keys
+// and values together, a thread to 8 elements of one slot of each, which stay in
+// registers between the maximum and the rounding.  Every warp counts the valid
+// tokens for itself, 1,024 flags at a time, and finds those of its own slots: no
+// earlier kernel, no barrier, no list in memory.
 #pragma once
 
 #include "rows8.cuh"
@@ -22,7 +26,6 @@
 namespace w4a4 {
 
 constexpr int kKvBlock = 16;  // tokens that share a scale
-constexpr int kKvThreads = 256;
 
 struct Kv8Params {
   int8_t* codes[2];        // keys, values
@@ -37,115 +40,141 @@ struct Kv8Params {
   int batch, tokens, heads, width, capacity;
 };
 
-// Source tokens of ranks [r0, r0 + 16) among the valid tokens of one
-// observation, into src[16] (-1: none), and the number of valid tokens.  All
-// 256 threads; `red` has 8 words.
-__device__ __forceinline__ int find_valid_tokens(const uint8_t* valid, int tokens, long long r0, int* src, int* red) {
-  if (threadIdx.x < kKvBlock) {
-    const long long r = r0 + threadIdx.x;
-    src[threadIdx.x] = !valid && r >= 0 && r < tokens ? static_cast<int>(r) : -1;
+// The token whose rank among an observation's valid tokens is r0 + (the calling
+// thread's slot), or -1, and the number of valid tokens.  A warp has 256 / width
+// slots, the first of them `slot0`, and calls as a whole.
+__device__ __forceinline__ int find_token(const uint8_t* valid, int tokens, long long r0, int slot0, int slot, int width,
+                                          int& count) {
+  if (!valid) {
+    const long long r = r0 + slot;
+    count = tokens;
+    return r >= 0 && r < tokens ? static_cast<int>(r) : -1;
   }
-  __syncthreads();
-  if (!valid) return tokens;
-  int base = 0;
-  for (int t0 = 0; t0 < tokens; t0 += 4 * kKvThreads) {
-    const int t = t0 + 4 * threadIdx.x;
-    int f[4], n = 0;
+  // words of four flags from the last address before the row that is a multiple of 4 on; the row's ends go by bytes
+  const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(valid) & 3);
+  const int lane = threadIdx.x & 31;
+  int found = -1;
+  count = 0;
+  for (int t0 = -lead; t0 < tokens; t0 += 1024) {
+    const int t = t0 + 32 * lane;
+    uint32_t f = 0;  // 32 flags
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[i] = t + i < tokens && valid[t + i] != 0;
-      n += f[i];
+    for (int i = 0; i < 8; ++i) {
+      const int u = t + 4 * i;
+      uint32_t w = 0;
+      if (u >= 0 && u + 4 <= tokens) {
+        w = __vcmpne4(*reinterpret_cast<const uint32_t*>(valid + u), 0u) & 0x01010101u;
+      } else if (u < tokens) {
+        for (int j = max(0, -u); j < 4 && u + j < tokens; ++j) w |= static_cast<uint32_t>(valid[u + j] != 0) << (8 * j);
+      }
+      f |= (w * 0x01020408u >> 24) << (4 * i);  // the four bytes' lowest bits, side by side
     }
+    const int n = __popc(f);
     int incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, incl, o);
-      if ((threadIdx.x & 31) >= o) incl += u;
+      if (lane >= o) incl += u;
     }
-    if ((threadIdx.x & 31) == 31) red[threadIdx.x >> 5] = incl;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kKvThreads / 32; ++w) {
-      if (w < static_cast<int>(threadIdx.x >> 5)) before += red[w];
-      all += red[w];
+    const int all = __shfl_sync(0xffffffffu, incl, 31);
+    for (int k = 0; k < 256 / width; ++k) {
+      const long long want = r0 + slot0 + k - count;  // its rank among these 1,024
+      if (want < 0 || want >= all) continue;
+      const int left = static_cast<int>(want) - (incl - n);
+      int token = -1;
+      if (left >= 0 && left < n) {
+        uint32_t rest = f;
+        for (int i = 0; i < left; ++i) rest &= rest - 1;
+        token = t + __ffs(rest) - 1;
+      }
+      token = __reduce_max_sync(0xffffffffu, token);
+      if (slot == slot0 + k) found = token;
     }
-    long long r = static_cast<long long>(base) + before + incl - n - r0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (f[i] && r >= 0 && r < kKvBlock) src[r] = t + i;
-      r += f[i];
-    }
-    base += all;
-    __syncthreads();
+    count += all;
   }
-  return base;
+  return found;
 }
 
-// grid (ceil((tokens + 14) / 16) + ..., batch * heads, 2); W = 8 or 1 elements.
-template <typename T, int W>
-__global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const __grid_constant__ Kv8Params p) {
-  __shared__ int src[kKvBlock];
-  __shared__ int red[kKvThreads / 32];
-  __shared__ uint32_t red_max[32];
+// grid (blocks that a run of `tokens` slots can touch, batch * heads), 2 x width
+// threads.  VEC: the new values' rows begin at multiples of 16 bytes.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(512, 3) kv8_append_kernel(const __grid_constant__ Kv8Params p) {
+  __shared__ uint32_t red[2][16];
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y / p.heads, h = blockIdx.y - b * p.heads, which = blockIdx.z;
+  const int b = blockIdx.y / p.heads, h = blockIdx.y - b * p.heads;
+  const int per = p.width / 8, slot = threadIdx.x / per, e = (threadIdx.x % per) * 8;
   const int start = p.start[b];
   const bool bad = start < 0 || start > p.capacity;
   const int first = bad ? 0 : start / kKvBlock + static_cast<int>(blockIdx.x);
   const long long s0 = static_cast<long long>(first) * kKvBlock;  // the block's first slot
-  const int count = find_valid_tokens(p.valid ? p.valid + b * p.valid_stride : nullptr, p.tokens, s0 - start, src, red);
+  int count;
+  const int token = find_token(p.valid ? p.valid + b * p.valid_stride : nullptr, p.tokens, s0 - start,
+                               (threadIdx.x & ~31) / per, slot, p.width, count);
   const long long end = static_cast<long long>(start) + count;
-  if (blockIdx.x == 0 && h == 0 && which == 0 && threadIdx.x == 0) {
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) {
     p.lengths[b] = bad ? max(0, min(start, p.capacity)) : static_cast<int>(min(end, static_cast<long long>(p.capacity)));
     if (bad || end > p.capacity) atomicOr(&g_w4a4_device_error, kErrCacheFull);
   }
   if (bad || s0 >= end || s0 >= p.capacity) return;
-  const T* x = static_cast<const T*>(p.x[which]) + b * p.xb[which] + h * p.xh[which];
-  int8_t* codes = p.codes[which] + b * p.cb + s0 * p.ct + h * p.ch;
-  float* scale = p.scale[which] + (static_cast<long long>(b) * p.heads + h) * (p.capacity / kKvBlock) + first;
-  const int groups = p.width / W, total = kKvBlock * groups;
-  uint32_t key = 0;
-  for (int i = threadIdx.x; i < total; i += kKvThreads) {
-    const int t = i / groups, e = (i - t * groups) * W;
-    if (src[t] >= 0) {
-      float v[W];
-      load_w<W>(x + src[t] * p.xt[which] + e, v);
+  const int kept = start > s0 ? static_cast<int>(start - s0) : 0;  // earlier tokens that stay
+  const bool keeps = slot < kept;
+  const long long at = b * p.cb + (s0 + slot) * p.ct + h * p.ch + e;
+  const long long at_scale = (static_cast<long long>(b) * p.heads + h) * (p.capacity / kKvBlock) + first;
+  float v[2][8] = {}, was[2];
 #pragma unroll
-      for (int j = 0; j < W; ++j) key = max(key, abs_key(v[j]));
+  for (int i = 0; i < 2; ++i) {
+    was[i] = kept ? p.scale[i][at_scale] : 0.f;
+    if (token >= 0) {
+      const T* x = static_cast<const T*>(p.x[i]) + b * p.xb[i] + h * p.xh[i] + token * p.xt[i] + e;
+      if constexpr (VEC) {
+        load8(x, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = to_float(x[j]);
+      }
+    } else if (keeps) {
+      const uint2 raw = *reinterpret_cast<const uint2*>(p.codes[i] + at);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        v[i][j] = static_cast<float>(static_cast<int8_t>((j < 4 ? raw.x : raw.y) >> (8 * (j & 3))));
     }
   }
-  const float fresh = __uint_as_float(block_max(key, red_max)) * kInv127;
-  const int kept = start > s0 ? static_cast<int>(start - s0) : 0;  // earlier tokens that stay
-  const float was = kept ? *scale : 0.f;
-  // keeps a NaN of either side
-  const float now = __uint_as_float(max(abs_key(was), abs_key(fresh)));
-  __syncthreads();  // every thread has read the old scale
-  if (threadIdx.x == 0) *scale = now;
-  const float ratio = now > 0.f ? __fdiv_rn(was, now) : 0.f;
-  const bool usable = now > 0.f && now <= 3.4028234e38f;
-  for (int i = threadIdx.x; i < total; i += kKvThreads) {
-    const int t = i / groups, e = (i - t * groups) * W;
-    int8_t* dst = codes + t * p.ct + e;
-    int c[W];
-    if (t < kept) {
-      if (ratio == 1.f) continue;
 #pragma unroll
-      for (int j = 0; j < W; ++j) c[j] = usable ? __float2int_rn(static_cast<float>(dst[j]) * ratio) : 0;
-    } else if (src[t] >= 0) {
-      float v[W];
-      load_w<W>(x + src[t] * p.xt[which] + e, v);
+  for (int i = 0; i < 2; ++i) {
+    uint32_t key = 0;
+    if (token >= 0) {
 #pragma unroll
-      for (int j = 0; j < W; ++j)
-        c[j] = usable ? __float2int_rn(fminf(fmaxf(__fdiv_rn(v[j], now), -127.f), 127.f)) : 0;
-    } else {
-      continue;
+      for (int j = 0; j < 8; ++j) key = max(key, abs_key(v[i][j]));
     }
-    if constexpr (W == 8)
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-    else
-      dst[0] = static_cast<int8_t>(c[0]);
+    key = __reduce_max_sync(0xffffffffu, key);
+    if ((threadIdx.x & 31) == 0) red[i][threadIdx.x >> 5] = key;
+  }
+  __syncthreads();  // also: every thread has read the old scales
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t key = __reduce_max_sync(0xffffffffu, lane < static_cast<int>(blockDim.x >> 5) ? red[i][lane] : 0u);
+    // keeps a NaN of either side
+    const float now = __uint_as_float(max(abs_key(was[i]), abs_key(__uint_as_float(key) * kInv127)));
+    if (threadIdx.x == 0) p.scale[i][at_scale] = now;
+    if (token >= 0) {
+      Coder code(now);
+      // the product with the reciprocal is within 2^-16 of the quotient: a value that close to a tie is divided, so
+      // that the codes are those of the division, whatever was appended with it
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = v[i][j] * code.mul;
+        code.fast = code.fast && fabsf(t - rintf(t)) < 0.4999f;
+      }
+      store_codes(p.codes[i] + at, v[i], code);
+    } else if (keeps && was[i] != now) {
+      // in steps of the new scale, as if the scale were one
+      const float ratio = now > 0.f && now <= 3.4028234e38f ? __fdiv_rn(was[i], now) : 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[i][j] *= ratio;
+      store_codes(p.codes[i] + at, v[i], Coder(1.f));
+    }
   }
 }
 
@@ -158,28 +187,28 @@ struct Kv8ValuesParams {
   int batch, heads, width, capacity;
 };
 
-// The values the cache stands for, zero from lengths[b] on.  grid (groups of
-// 256 x 8 values of one token block of all heads..., batch, 2).
+// The values the cache stands for, zero from lengths[b] on.  grid (blocks of 16
+// tokens, batch * heads, 2), a thread to 16 codes: `width` threads.
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_values_kernel(const __grid_constant__ Kv8ValuesParams p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int b = blockIdx.y, which = blockIdx.z;
-  const int per_head = p.width / 8, per_token = p.heads * per_head;
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long token = i / per_token;
-  if (token >= p.capacity) return;
-  const int rem = static_cast<int>(i - token * per_token);
-  const int h = rem / per_head, e = (rem - h * per_head) * 8;
-  float v[8] = {};
-  if (token < p.lengths[b]) {
-    const float s = p.scale[which][(static_cast<long long>(b) * p.heads + h) * (p.capacity / kKvBlock) + token / kKvBlock];
-    const uint2 raw = *reinterpret_cast<const uint2*>(p.codes[which] + b * p.cb + token * p.ct + h * p.ch + e);
+  const int b = blockIdx.y / p.heads, h = blockIdx.y - b * p.heads, which = blockIdx.z;
+  const int token = blockIdx.x * kKvBlock + threadIdx.x / (p.width / 16), e = (threadIdx.x % (p.width / 16)) * 16;
+  const float s = p.scale[which][static_cast<long long>(blockIdx.y) * (p.capacity / kKvBlock) + blockIdx.x];
+  T* out = static_cast<T*>(p.out[which]) + ((static_cast<long long>(b) * p.capacity + token) * p.heads + h) * p.width + e;
+  uint4 raw = {};
+  const bool filled = token < p.lengths[b];
+  if (filled) raw = *reinterpret_cast<const uint4*>(p.codes[which] + b * p.cb + token * p.ct + h * p.ch + e);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      v[j] = static_cast<float>(static_cast<int8_t>((j < 4 ? raw.x : raw.y) >> (8 * (j & 3)))) * s;
+      v[j] = filled ? static_cast<float>(static_cast<int8_t>(w[2 * half + (j >> 2)] >> (8 * (j & 3)))) * s : 0.f;
+    store8(out + 8 * half, v);
   }
-  store8(static_cast<T*>(p.out[which]) + ((static_cast<long long>(b) * p.capacity + token) * p.heads + h) * p.width + e, v);
 }
 
 }  // namespace w4a4

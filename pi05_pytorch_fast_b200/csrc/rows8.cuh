@@ -107,18 +107,6 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ float from_float<float>(float v) { return v; }
 
-// W = 8 or 1 elements.
-template <int W, typename T>
-__device__ __forceinline__ void load_w(const T* p, float (&v)[W]) {
-  if constexpr (W == 8) load8(p, v);
-  else v[0] = to_float(*p);
-}
-template <int W, typename T>
-__device__ __forceinline__ void store_w(T* p, const float (&v)[W]) {
-  if constexpr (W == 8) store8(p, v);
-  else *p = from_float<T>(v[0]);
-}
-
 // gelu(x) = x / (1 + exp(-2 u)), u = sqrt(2/pi) (x + 0.044715 x^3): the tanh
 // form 0.5 x (1 + tanh u) with 1 + tanh u = 2 / (1 + exp(-2 u)), which does not
 // cancel for negative u.  exp(-2 u) = 2^(x (a + b x^2)).
@@ -168,18 +156,17 @@ struct Coder {
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-template <int W>
-__device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[W], const Coder& code) {
-  uint32_t c[W];
+// Eight codes.
+__device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[8], const Coder& code) {
+  uint32_t c[8];
   if (code.fast) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = code.quick(v[i]);
+    for (int i = 0; i < 8; ++i) c[i] = code.quick(v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) c[i] = code.slow(v[i]);
+    for (int i = 0; i < 8; ++i) c[i] = code.slow(v[i]);
   }
-  if constexpr (W == 8) *reinterpret_cast<uint2*>(p) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-  else *p = static_cast<int8_t>(c[0]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
 }
 
 // |v| as an unsigned key: ordered like the value, infinity above every finite
@@ -215,96 +202,73 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
   return __reduce_max_sync(0xffffffffu, v);
 }
 
-// W elements as they lie in memory, to be asked for early and unpacked later.
-template <typename T, int W>
+// Eight elements as they lie in memory, to be asked for early and unpacked later.
+template <typename T>
 struct RawVec {
-  static constexpr int kWords = W * sizeof(T) / 16;
-  uint4 q[kWords > 0 ? kWords : 1];
-  T one;
+  static constexpr int kWords = sizeof(T) / 2;
+  uint4 q[kWords];
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kWords > 0) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else {
-      one = *p;
-    }
+    for (int i = 0; i < kWords; ++i) q[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-  __device__ __forceinline__ void unpack(float (&v)[W]) const {
-    if constexpr (kWords > 0) load8(reinterpret_cast<const T*>(q), v);
-    else v[0] = to_float(one);
-  }
+  __device__ __forceinline__ void unpack(float (&v)[8]) const { load8(reinterpret_cast<const T*>(q), v); }
 };
 
-template <int W>
-__device__ __forceinline__ void mul_w(float (&v)[W], const float (&u)[W]) {
-  if constexpr (W == 8) {
+__device__ __forceinline__ void mul8(float (&v)[8], const float (&u)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(u[i], u[i + 1]));
-      v[i] = r.x, v[i + 1] = r.y;
-    }
-  } else {
-    v[0] *= u[0];
+  for (int i = 0; i < 8; i += 2) {
+    const float2 r = __fmul2_rn(make_float2(v[i], v[i + 1]), make_float2(u[i], u[i + 1]));
+    v[i] = r.x, v[i + 1] = r.y;
   }
 }
 // v = a v + b
-template <int W>
-__device__ __forceinline__ void fma_w(float (&v)[W], const float (&a)[W], const float (&b)[W]) {
-  if constexpr (W == 8) {
+__device__ __forceinline__ void fma8(float (&v)[8], const float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(v[i], v[i + 1]), make_float2(b[i], b[i + 1]));
-      v[i] = r.x, v[i + 1] = r.y;
-    }
-  } else {
-    v[0] = fmaf(a[0], v[0], b[0]);
+  for (int i = 0; i < 8; i += 2) {
+    const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(v[i], v[i + 1]), make_float2(b[i], b[i + 1]));
+    v[i] = r.x, v[i + 1] = r.y;
   }
 }
-template <int W>
-__device__ __forceinline__ void gelu_w(float (&v)[W]) {
-  if constexpr (W == 8) {
+__device__ __forceinline__ void gelu8(float (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float2 r = gelu_tanh_f32x2(make_float2(v[i], v[i + 1]));
-      v[i] = r.x, v[i + 1] = r.y;
-    }
-  } else {
-    v[0] = gelu_tanh_f32x2(make_float2(v[0], 0.f)).x;
+  for (int i = 0; i < 8; i += 2) {
+    const float2 r = gelu_tanh_f32x2(make_float2(v[i], v[i + 1]));
+    v[i] = r.x, v[i + 1] = r.y;
   }
 }
 
-// x and delta / up of W elements -> the value before the norm (v + gate u).
-template <int OP, int W>
-__device__ __forceinline__ void row8_combine(float (&v)[W], float (&u)[W], bool has, bool gated, const float (&gate)[W]) {
+// x and delta / up of 8 elements -> the value before the norm (v + gate u).
+template <int OP>
+__device__ __forceinline__ void row8_combine(float (&v)[8], float (&u)[8], bool has, bool gated, const float (&gate)[8]) {
   if constexpr (OP == kRowGeglu) {
-    gelu_w<W>(v);
-    mul_w<W>(v, u);
+    gelu8(v);
+    mul8(v, u);
   } else if constexpr (OP == kRowNorm) {
     if (has) {
       if (gated) {
-        fma_w<W>(u, gate, v);
+        fma8(u, gate, v);
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] = u[i];
+        for (int i = 0; i < 8; ++i) v[i] = u[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < W; ++i) v[i] += u[i];
+        for (int i = 0; i < 8; ++i) v[i] += u[i];
       }
     }
   }
 }
 
-// One row of a CTA at a time, held in registers: thread t has the W-element
+// One row of a CTA at a time, held in registers: thread t has the 8-element
 // groups t, t + blockDim, ... (VPT of them).  A CTA takes consecutive rows, so
 // that an observation's gain, shift and gate come from L1 after its first row.
-template <typename T, int OP, int W, int VPT, int MAXT, int MINB>
+template <typename T, int OP, int VPT, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant__ Row8Params p) {
   __shared__ float red_sum[32];
   __shared__ uint32_t red_max[2][32];
   pdl_launch_dependents();
   pdl_wait();
-  const int groups = (p.h + W - 1) / W;  // W = 8: h is a multiple of 8
+  const int groups = p.h / 8;
   const bool has2 = p.x2 != nullptr;
-  RawVec<T, W> rx[VPT], ru[VPT];
+  RawVec<T> rx[VPT], ru[VPT];
   const auto fetch = [&](long long row) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
     const T* x2 = static_cast<const T*>(p.x2) + row * p.ld2;
@@ -312,8 +276,8 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
     for (int j = 0; j < VPT; ++j) {
       const int g = threadIdx.x + j * blockDim.x;
       if (g < groups) {
-        rx[j].load(x + g * W);
-        if (OP != kRowQuant && has2) ru[j].load(x2 + g * W);
+        rx[j].load(x + g * 8);
+        if (OP != kRowQuant && has2) ru[j].load(x2 + g * 8);
       }
     }
   };
@@ -323,27 +287,27 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
   for (int turn = 0; row < end; ++row, turn ^= 1) {
     const long long obs = OP == kRowNorm ? row / p.rows_per_batch : 0;
     const T* gate = static_cast<const T*>(p.gate) + obs * p.gate_stride;
-    float v[VPT][W];
+    float v[VPT][8];
     float ss[2] = {0.f, 0.f};
     {
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
         const int g = threadIdx.x + j * blockDim.x;
         if (g < groups) {
-          float u[W];
+          float u[8];
           rx[j].unpack(v[j]);
           if (OP != kRowQuant && has2) ru[j].unpack(u);
-          float gv[W];
-          if (OP == kRowNorm && p.gate) load_w<W>(gate + g * W, gv);
-          row8_combine<OP, W>(v[j], u, has2, p.gate != nullptr, gv);
+          float gv[8];
+          if (OP == kRowNorm && p.gate) load8(gate + g * 8, gv);
+          row8_combine<OP>(v[j], u, has2, p.gate != nullptr, gv);
           if constexpr (OP == kRowNorm) {
-            if (p.total) store_w<W>(static_cast<T*>(p.total) + row * p.h + g * W, v[j]);
+            if (p.total) store8(static_cast<T*>(p.total) + row * p.h + g * 8, v[j]);
 #pragma unroll
-            for (int i = 0; i < W; ++i) ss[i & 1] = fmaf(v[j][i], v[j][i], ss[i & 1]);
+            for (int i = 0; i < 8; ++i) ss[i & 1] = fmaf(v[j][i], v[j][i], ss[i & 1]);
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < W; ++i) v[j][i] = 0.f;
+          for (int i = 0; i < 8; ++i) v[j][i] = 0.f;
         }
       }
     }
@@ -356,13 +320,13 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
       for (int j = 0; j < VPT; ++j) {
         const int g = threadIdx.x + j * blockDim.x;
         if (g < groups) {
-          float gn[W], sh[W], r[W];
-          load_w<W>(gain + g * W, gn);
+          float gn[8], sh[8], r[8];
+          load8(gain + g * 8, gn);
 #pragma unroll
-          for (int i = 0; i < W; ++i) r[i] = rstd, sh[i] = 0.f;
-          if (p.shift) load_w<W>(shift + g * W, sh);
-          mul_w<W>(v[j], r);
-          fma_w<W>(v[j], gn, sh);
+          for (int i = 0; i < 8; ++i) r[i] = rstd, sh[i] = 0.f;
+          if (p.shift) load8(shift + g * 8, sh);
+          mul8(v[j], r);
+          fma8(v[j], gn, sh);
         }
       }
     }
@@ -370,13 +334,13 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
 #pragma unroll
     for (int j = 0; j < VPT; ++j)
 #pragma unroll
-      for (int i = 0; i < W; ++i) amax = max_abs(amax, v[j][i]);
+      for (int i = 0; i < 8; ++i) amax = max_abs(amax, v[j][i]);
     const float scale = __uint_as_float(block_max(abs_key(amax), red_max[turn])) * kInv127;
     const Coder code(scale);
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
       const int g = threadIdx.x + j * blockDim.x;
-      if (g < groups) store_codes<W>(p.codes + row * p.ldc + g * W, v[j], code);
+      if (g < groups) store_codes(p.codes + row * p.ldc + g * 8, v[j], code);
     }
     if (threadIdx.x == 0) p.scale[row] = scale;
   }

@@ -96,10 +96,10 @@ int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* wh
       const int groups = p.h / 8;
       // few rows: as many threads as a row has vectors, for the latency; many: four vectors a thread, so that the
       // reductions' instructions are shared by more elements
-      if (groups <= 256 && p.rows <= 8 * sms) return go(row8_kernel<T, OP, 8, 1, 256, 4>, groups, 1, 64);
-      if (groups <= 64) return go(row8_kernel<T, OP, 8, 2, 512, 1>, groups, 2, 128);
-      if (groups <= 2048) return go(row8_kernel<T, OP, 8, 4, 512, 1>, groups, 4, 128);
-      return go(row8_kernel<T, OP, 8, 4, 1024, 1>, groups, 4, 64);
+      if (groups <= 256 && p.rows <= 8 * sms) return go(row8_kernel<T, OP, 1, 256, 4>, groups, 1, 64);
+      if (groups <= 64) return go(row8_kernel<T, OP, 2, 512, 1>, groups, 2, 128);
+      if (groups <= 2048) return go(row8_kernel<T, OP, 4, 512, 1>, groups, 4, 128);
+      return go(row8_kernel<T, OP, 4, 1024, 1>, groups, 4, 64);
     }
     if (p.h > kRow8AnyMax)
       return fail(W4A4_ERR_UNSUPPORTED, "%s: rows of more than %d elements are not supported", what, kRow8AnyMax);
@@ -319,9 +319,9 @@ Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, const int (&fit)
   const int64_t room = fit[0] / std::max<int64_t>(work, 1);
   plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, room, 256})));
   if (plan.few && plan.splits <= 8) {
-    int i = 3;
-    while (i > 0 && ((1 << i) > plan.splits || units > fit[i])) --i;
-    plan.splits = 1 << i;
+    // a cluster of 3, 5, 6 or 7 takes no more room than one of the next power of two
+    const auto room_for = [&](int splits) { return fit[splits > 4 ? 3 : splits > 2 ? 2 : splits - 1]; };
+    while (plan.splits > 1 && units > room_for(plan.splits)) --plan.splits;
   }
   return plan;
 }
@@ -468,6 +468,7 @@ int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_s
                            "kv8_append"))
     return e;
   if (tokens < 0) return fail(W4A4_ERR_INVALID, "kv8_append: invalid token count %d", tokens);
+  if (tokens > 1 << 30) return fail(W4A4_ERR_UNSUPPORTED, "kv8_append: too many tokens: %d", tokens);
   if (batch == 0) return ok();
   if (!start || !lengths || !k_stride || !v_stride || (tokens > 0 && (!k || !v)))
     return fail(W4A4_ERR_INVALID, "kv8_append: null pointer argument");
@@ -486,9 +487,9 @@ int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_s
     using T = decltype(tag);
     // a run of `tokens` slots touches at most ceil((tokens - 1) / 16) + 1 blocks
     const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(tokens) + 14) / kKvBlock + 1),
-                    static_cast<unsigned>(batch * heads), 2);
-    const auto kernel = vec ? kv8_append_kernel<T, 8> : kv8_append_kernel<T, 1>;
-    return cuda_status(launch_kernel(kernel, grid, dim3(kKvThreads), 0, static_cast<cudaStream_t>(stream), 1, p))
+                    static_cast<unsigned>(batch * heads));
+    const auto kernel = vec ? kv8_append_kernel<T, true> : kv8_append_kernel<T, false>;
+    return cuda_status(launch_kernel(kernel, grid, dim3(2 * width), 0, static_cast<cudaStream_t>(stream), 1, p))
                ? W4A4_ERR_CUDA
                : ok();
   });
@@ -511,9 +512,8 @@ int w4a4_kv8_values(const int8_t* k_codes, const int8_t* v_codes, const float* k
   p.batch = batch, p.heads = heads, p.width = width, p.capacity = capacity;
   return by_dtype(dtype, true, "kv8_values", [&](auto tag) {
     using T = decltype(tag);
-    const int64_t groups = static_cast<int64_t>(capacity) * heads * (width / 8);
-    const dim3 grid(static_cast<unsigned>((groups + 255) / 256), static_cast<unsigned>(batch), 2);
-    return cuda_status(launch_kernel(kv8_values_kernel<T>, grid, dim3(256), 0, static_cast<cudaStream_t>(stream), 1, p))
+    const dim3 grid(static_cast<unsigned>(capacity / kKvBlock), static_cast<unsigned>(batch * heads), 2);
+    return cuda_status(launch_kernel(kv8_values_kernel<T>, grid, dim3(width), 0, static_cast<cudaStream_t>(stream), 1, p))
                ? W4A4_ERR_CUDA
                : ok();
   });
