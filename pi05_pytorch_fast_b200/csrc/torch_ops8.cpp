@@ -59,18 +59,26 @@ Tensor empty_on(const Tensor& x, at::IntArrayRef size, at::ScalarType type) {
   return at::detail::empty_cuda(size, type, x.device(), std::nullopt);
 }
 
-// x [..., h] as rows: [m, h] with unit inner stride (a view where x's strides allow one).
+// x [..., h] as rows [m, h] with unit inner stride: x itself where its strides allow it (no view is made of it), else
+// a copy.
 struct Rows {
   Tensor t;
   int64_t m, ld;
   const void* data() const { return t.const_data_ptr(); }
 };
 Rows rows_of(const Tensor& x) {
-  const int64_t h = x.size(-1), m = x.numel() / h;
-  Tensor t = x;
-  if (t.stride(-1) != 1 && h > 1) t = t.contiguous();
-  if (t.dim() != 2) t = t.reshape({m, h});
-  return {t, m, m > 1 ? t.stride(0) : h};
+  const auto size = x.sizes(), stride = x.strides();
+  const int64_t h = size.back(), m = x.numel() / h;
+  int64_t ld = h, next = -1;  // ld: the stride of the innermost dimension with more than one entry
+  bool fits = stride.back() == 1 || h == 1;
+  for (int64_t d = x.dim() - 2; d >= 0 && fits; --d) {
+    if (size[d] == 1) continue;
+    if (next < 0) ld = next = stride[d];
+    fits = stride[d] == next && ld >= h;
+    next *= size[d];
+  }
+  if (fits) return {x, m, ld};
+  return {x.contiguous(), m, h};
 }
 
 // int8 of x's shape whose rows begin at multiples of 128 bytes, the product's
@@ -192,7 +200,7 @@ Tensor dequantize(const Tensor& codes, const Tensor& scale, at::ScalarType dtype
 
 // Rows that the product can read with TMA: 16-byte steps and base.
 Rows tma_rows(Rows r, const char* what) {
-  const int64_t k = r.t.size(1);
+  const int64_t k = r.t.size(-1);
   if (r.ld % 16 == 0 && reinterpret_cast<uintptr_t>(r.data()) % 16 == 0) return r;
   if (r.m == 1 && reinterpret_cast<uintptr_t>(r.data()) % 16 == 0) {
     r.ld = (k + 15) / 16 * 16;  // one row: the stride is never used
@@ -203,7 +211,7 @@ Rows tma_rows(Rows r, const char* what) {
                   "pack_weight lay them out.");
   const int64_t ld = (k + 127) / 128 * 128;
   Tensor t = empty_on(r.t, {r.m, ld}, at::kChar).narrow(1, 0, k);
-  t.copy_(r.t);
+  t.copy_(r.t.reshape({r.m, k}));
   return {t, r.m, ld};
 }
 
@@ -378,3 +386,13 @@ TORCH_LIBRARY_IMPL(pi05_w8a8, CompositeExplicitAutograd, m) {
   m.impl("kv_values", &kv_values);
   m.impl("kv_attention", &kv_attention);
 }
+
+// No op has a gradient: calls go past the autograd keys to the bodies.
+namespace {
+void past_autograd(torch::Library& m) {
+  for (const char* op : {"rms_norm_quant", "quantize", "dequantize", "linear", "kv_append", "kv_values", "kv_attention"})
+    m.impl(op, torch::CppFunction::makeFallthrough());
+}
+}  // namespace
+TORCH_LIBRARY_IMPL(pi05_w8a8, AutogradCUDA, m) { past_autograd(m); }
+TORCH_LIBRARY_IMPL(pi05_w8a8, AutogradCPU, m) { past_autograd(m); }
