@@ -933,7 +933,10 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       }
       const float up = p.scale < 0.f ? -shift : shift;
       if (group == 0) {
-        row_info[row] = make_float2(fabsf(p.scale) / shift, __int_as_float(r < p.rows ? keys_seen(p, n, p.causal ? r / p.group : 0) : 0));
+        // rows past the last count as it does (their queries are zero, nothing of theirs is stored): a warp with rows
+        // that see less than a tile takes the longer way through it
+        row_info[row] = make_float2(fabsf(p.scale) / shift,
+                                    __int_as_float(keys_seen(p, n, p.causal ? min(r, p.rows - 1) / p.group : 0)));
         row_m[row] = -INFINITY;
         row_v[row] = 0.f;
       }
@@ -1200,49 +1203,56 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
   }
 }
 
-// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one CTA of 128
-// threads per row, a thread with one 16-byte chunk of every (512 / D)-th part
-// (chunk c of row r lies at c ^ (r & 7)).
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attn8_join_kernel(const __grid_constant__ Attn8Params p) {
-  constexpr int NC = D / 4, G = 128 / NC;
+// out[row] = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m): one CTA of THREADS
+// per row, a thread with one 16-byte chunk of every (4 THREADS / D)-th part
+// (chunk c of row r lies at c ^ (r & 7)).  m first, from all parts' m_s, so that
+// the parts' loads do not wait for one another.  128 threads for up to 32 parts;
+// 512 for more (8 rows of width 256, 64 parts: 21.1 us with the attention in one
+// pass of 128 threads, 10.4 so).
+template <typename T, int D, int THREADS>
+__global__ void __launch_bounds__(THREADS) attn8_join_kernel(const __grid_constant__ Attn8Params p) {
+  constexpr int NC = D / 4, G = THREADS / NC;
   __shared__ float4 red[G][NC];
-  __shared__ float2 red_ml[G];
+  __shared__ float red_l[G];
   pdl_launch_dependents();
   pdl_wait();
   const int c = threadIdx.x % NC, g = threadIdx.x / NC;
   const int r = blockIdx.x, unit = blockIdx.y;
   const long long first = static_cast<long long>(unit) * p.splits * p.rows + r;
+  const float2* part_ml = p.part_ml + first;
+  float m = -INFINITY;
+  for (int s = threadIdx.x & 31; s < p.splits; s += 32) {
+    const float2 ml = part_ml[static_cast<long long>(s) * p.rows];
+    if (ml.y != 0.f) m = fmaxf(m, ml.x);  // l = 0: saw nothing (a NaN stays)
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  float m = -INFINITY, sum = 0.f;
+  float sum = 0.f;
 #pragma unroll 4
   for (int s = g; s < p.splits; s += G) {
-    const long long at = first + static_cast<long long>(s) * p.rows;
-    const float2 ml = p.part_ml[at];
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + (c ^ (r & 7)) * 4);
-    if (ml.y == 0.f) continue;  // saw nothing (a NaN stays)
-    const float mn = fmaxf(m, ml.x);
-    const float fo = m == -INFINITY ? 0.f : ex2_approx(m - mn), fn = ex2_approx(ml.x - mn);
-    m = mn;
-    sum = sum * fo + ml.y * fn;
-    acc = make_float4(acc.x * fo + v.x * fn, acc.y * fo + v.y * fn, acc.z * fo + v.z * fn, acc.w * fo + v.w * fn);
+    const float2 ml = part_ml[static_cast<long long>(s) * p.rows];
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + (first + static_cast<long long>(s) * p.rows) * D +
+                                                      (c ^ (r & 7)) * 4);
+    const bool saw = ml.y != 0.f;
+    const float f = ex2_approx(ml.x - m);
+    sum = saw ? fmaf(ml.y, f, sum) : sum;
+    acc.x = saw ? fmaf(v.x, f, acc.x) : acc.x;
+    acc.y = saw ? fmaf(v.y, f, acc.y) : acc.y;
+    acc.z = saw ? fmaf(v.z, f, acc.z) : acc.z;
+    acc.w = saw ? fmaf(v.w, f, acc.w) : acc.w;
   }
   red[g][c] = acc;
-  if (c == 0) red_ml[g] = make_float2(m, sum);
+  if (c == 0) red_l[g] = sum;
   __syncthreads();
   if (g > 0) return;
-  float mm = -INFINITY, total = 0.f;
+  float4 x = red[0][c];
+  float total = red_l[0];
 #pragma unroll
-  for (int w = 0; w < G; ++w) mm = fmaxf(mm, red_ml[w].x);
-  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-  for (int w = 0; w < G; ++w) {
-    const float2 ml = red_ml[w];
-    if (ml.y == 0.f) continue;
-    const float f = ex2_approx(ml.x - mm);
+  for (int w = 1; w < G; ++w) {
     const float4 v = red[w][c];
-    x = make_float4(fmaf(v.x, f, x.x), fmaf(v.y, f, x.y), fmaf(v.z, f, x.z), fmaf(v.w, f, x.w));
-    total = fmaf(ml.y, f, total);
+    x = make_float4(x.x + v.x, x.y + v.y, x.z + v.z, x.w + v.w);
+    total += red_l[w];
   }
   const float inv = total == 0.f ? 0.f : 1.f / total;
   const int b = unit / p.heads, h = unit - b * p.heads;

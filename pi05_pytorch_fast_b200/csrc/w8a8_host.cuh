@@ -94,9 +94,10 @@ int launch_row8(Row8Params p, int32_t dtype, cudaStream_t stream, const char* wh
     };
     if (vec && p.h <= kRow8MaxVec) {
       const int groups = p.h / 8;
-      // few rows: as many threads as a row has vectors, for the latency; many: four vectors a thread, so that the
-      // reductions' instructions are shared by more elements
-      if (groups <= 256 && p.rows <= 8 * sms) return go(row8_kernel<T, OP, 1, 256, 4>, groups, 1, 64);
+      // few rows: as many threads as a row has vectors, for the latency (400 x 1,024: 2.9 us, with four vectors a thread
+      // 3.4); many: four vectors a thread, so that the reductions' instructions are shared by more elements (776 x 2,048:
+      // 4.5 us against 5.1; 49,664 x 2,048: 115 against 140)
+      if (groups <= 256 && p.rows <= 4 * sms) return go(row8_kernel<T, OP, 1, 256, 4>, groups, 1, 64);
       if (groups <= 64) return go(row8_kernel<T, OP, 2, 512, 1>, groups, 2, 128);
       if (groups <= 2048) return go(row8_kernel<T, OP, 4, 512, 1>, groups, 4, 128);
       return go(row8_kernel<T, OP, 4, 1024, 1>, groups, 4, 64);
@@ -301,23 +302,32 @@ int check_cache8(const void* k, const void* v, const void* ks, const void* vs, c
 // How many CTAs the keys of one key/value head are split over, from the
 // cache's capacity (the lengths are on the device; a split without keys writes
 // an empty part).  Up to 8 CTAs of the few-rows form are a cluster, as long as
-// all clusters run at once: `fit[i]` of 1 << i CTAs.
+// all clusters run at once: `fit[i]` of 1 << i CTAs; they join their parts
+// themselves (8 heads of width 256 over 776 tokens: 7.5 us, 10.2 with the parts
+// in memory and a kernel that joins them).
+//
+// The few-rows form is for up to 16 rows, its MMA's; the other one pads them to
+// 128 (8 rows, 776 tokens of width 256: 7.5 and 14.8 us; 16 rows, 65,536 tokens
+// of 4 x 2 heads of width 128: 41 and 102 us).
 constexpr int kAttn8FewRows = 16;
 struct Attn8Plan {
   bool few;
   int tiles;   // row tiles of the many-rows form
   int splits;
 };
-Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, const int (&fit)[4]) {
+Attn8Plan attn8_plan(int64_t units, int64_t rows, int capacity, int width, const int (&fit)[4]) {
   Attn8Plan plan{};
   plan.few = rows <= kAttn8FewRows;
   plan.tiles = static_cast<int>((rows + 127) / 128);
   const int64_t work = units * (plan.few ? 1 : plan.tiles);
-  // splits that the keys are worth (a CTA's warps and three tiles of 64 keys take that many at a time), and that the
-  // SMs have room for
-  const int64_t most = plan.few ? (capacity + 127) / 128 : (capacity + 191) / 192;
-  const int64_t room = fit[0] / std::max<int64_t>(work, 1);
-  plan.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, room, 256})));
+  // splits that the keys are worth (one step of all 8 warps, or three tiles of 64 keys, each) and that the SMs have
+  // room for, at most 128 of them and the steps in equal shares, as each part costs the join (1 head of 256, 32,768
+  // tokens: 128 parts 14.7 us, 148 parts 20.9, 64 parts 15.7; 131,072 tokens: 26.5, 31.8 and 35.4)
+  const int step = plan.few ? 32768 / width : 192;
+  const int64_t steps = (capacity + step - 1) / step;
+  const int64_t room = std::max<int64_t>(1, std::min<int64_t>(128, fit[0] / std::max<int64_t>(work, 1)));
+  const int64_t each = (steps + room - 1) / room;
+  plan.splits = static_cast<int>(plan.few ? (steps + each - 1) / each : std::min(steps, room));
   if (plan.few && plan.splits <= 8) {
     // a cluster of 3, 5, 6 or 7 takes no more room than one of the next power of two
     const auto room_for = [&](int splits) { return fit[splits > 4 ? 3 : splits > 2 ? 2 : splits - 1]; };
@@ -364,9 +374,12 @@ int launch_attention8_d(const Attn8Params& p, const Attn8Plan& plan, int64_t uni
     W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.tiles, p.splits, static_cast<unsigned>(units)), dim3(C::kThreads), C::kSmem,
                                 stream, 1, mp));
   }
-  if (p.splits > (plan.few ? 8 : 1))
-    W4A4_CUDA_TRY(launch_kernel(attn8_join_kernel<T, D>, dim3(static_cast<unsigned>(p.rows), static_cast<unsigned>(units)),
-                                dim3(128), 0, stream, 1, p));
+  if (p.splits > (plan.few ? 8 : 1)) {
+    const bool wide = p.splits > 32;
+    W4A4_CUDA_TRY(launch_kernel(wide ? attn8_join_kernel<T, D, 512> : attn8_join_kernel<T, D, 128>,
+                                dim3(static_cast<unsigned>(p.rows), static_cast<unsigned>(units)), dim3(wide ? 512 : 128), 0,
+                                stream, 1, p));
+  }
   return ok();
 }
 
@@ -530,7 +543,7 @@ int w4a4_attention8_workspace(int32_t batch, int32_t tokens, int32_t q_heads, in
   if (int e = current_device(&dev)) return e;
   if (int e = cluster_fit(dev, fit)) return e;
   const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
-  const Attn8Plan plan = attn8_plan(units, rows, capacity, fit);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, width, fit);
   if (plan.splits > 1) *bytes = units * plan.splits * rows * (static_cast<int64_t>(width) * 4 + 8);
   return ok();
 }
@@ -556,7 +569,7 @@ int w4a4_attention8(const void* q, const int64_t* q_stride, const int8_t* k_code
   if (int e = current_device(&dev)) return e;
   if (int e = cluster_fit(dev, fit)) return e;
   const int64_t units = static_cast<int64_t>(batch) * heads, rows = static_cast<int64_t>(tokens) * (q_heads / heads);
-  const Attn8Plan plan = attn8_plan(units, rows, capacity, fit);
+  const Attn8Plan plan = attn8_plan(units, rows, capacity, width, fit);
   Attn8Params p{};
   p.q = q, p.out = out, p.k = k_codes, p.v = v_codes, p.ks = k_scale, p.vs = v_scale, p.lengths = lengths;
   p.qb = q_stride[0], p.qt = q_stride[1], p.qh = q_stride[2];
