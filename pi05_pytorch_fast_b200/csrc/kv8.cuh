@@ -18,7 +18,9 @@
 // and values together, a thread to 8 elements of one slot of each, which stay in
 // registers between the maximum and the rounding.  Every warp counts the valid
 // tokens for itself, 1,024 flags at a time, and finds those of its own slots: no
-// earlier kernel, no barrier, no list in memory.
+// earlier kernel, no barrier, no list in memory.  Measured: 8 x 776 tokens of
+// width 256 5.8 us, with flags 8.5 (with a scan by the CTA and a list in shared
+// memory 11.3); 8 x 1 token 3.2 us.
 #pragma once
 
 #include "rows8.cuh"
@@ -188,7 +190,8 @@ struct Kv8ValuesParams {
 };
 
 // The values the cache stands for, zero from lengths[b] on.  grid (blocks of 16
-// tokens, batch * heads, 2), a thread to 16 codes: `width` threads.
+// tokens, batch * heads, 2), a thread to 16 codes: `width` threads.  Bound: HBM;
+// 8 x 832 slots of width 256 3.7 us (10 MB).
 template <typename T>
 __global__ void __launch_bounds__(256) kv8_values_kernel(const __grid_constant__ Kv8ValuesParams p) {
   pdl_launch_dependents();

@@ -18,7 +18,10 @@
 // in turn, and asks for the next one's vectors before it reduces this one, so
 // that loads are under way all the time.  The arithmetic is two lanes wide
 // (f32x2) and codes come from one multiply-add, as at the memory's rate there
-// are about 25 issue slots for an element of the GeGLU.
+// are about 25 issue slots for an element of the GeGLU.  Measured: norm of 49,664
+// x 2,048 with residual 116 us (6.16 TB/s of 6.53; 153 us with fp32 one at a time
+// and no look ahead), GeGLU of 6,208 x 16,384 88 us (5.8 TB/s), codes of 6,208 x
+// 2,048 7.7 us, of one row 1.4 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -348,7 +351,10 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
 
 // Any row: one, two or four elements at a time, the row's fp32 values in shared
 // memory between the passes.  For rows that do not begin at multiples of 16
-// bytes (a length that is not a multiple of 8), and for long ones.
+// bytes (a length that is not a multiple of 8), and for long ones.  Bound by the
+// instructions of the narrow loads: 1,944 x 7,620 (by 4) 64 us, 6,208 x 2,047 (by
+// 1) 28 us; held in registers by one element 197 us and, as far as they fit, no
+// faster.
 constexpr int kRow8AnyThreads = 256;
 constexpr int kRow8AnyMax = 49152;  // elements: 192 KB of shared memory
 

@@ -231,8 +231,10 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     const Gemm8FewParams f{a, w, sa, sw, bias, y, lda, ldw, static_cast<int>(m), n, k};
     return by_dtype(dtype, true, "gemm8", [&](auto tag) {
       using T = decltype(tag);
-      // 16 channels a CTA where that leaves enough CTAs (the tokens are read half as often), and twice the
-      // warps, to have enough loads under way, where there are few CTAs and a long K
+      // 16 channels a CTA where that leaves enough CTAs (the tokens are read half as often; 1 x 2,048 x 32,768: 17.1 us,
+      // with 8 channels 19.0), and twice the warps, to have enough loads under way, where there are few CTAs and a long
+      // K (16 x 16,384 x 2,048: 9.6 us, with 8 warps 16.1); half the MMA's rows for up to 8 tokens (1 x 16,384 x 2,048:
+      // 11.6 us, with all of them and 8 warps 14.8)
       const bool wide = n >= 32 * sms, deep = !wide && k >= 4096;
       const auto by_shape = [&](auto half_tag) {
         constexpr bool H = decltype(half_tag)::value;
