@@ -352,9 +352,11 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
 // Any row: one, two or four elements at a time, the row's fp32 values in shared
 // memory between the passes.  For rows that do not begin at multiples of 16
 // bytes (a length that is not a multiple of 8), and for long ones.  Bound by the
-// instructions of the narrow loads: 1,944 x 7,620 (by 4) 64 us, 6,208 x 2,047 (by
-// 1) 28 us; held in registers by one element 197 us and, as far as they fit, no
-// faster.
+// instructions and latency of the narrow loads: 1,944 x 7,620 (by 4) 44 us, 4,464 x
+// 2,394 (by 2) 33 us, 6,208 x 2,047 codes (by 1) 28 us.  Vectors of 16 bytes from
+// the last multiple of 16 before each row on took 17 us for these codes, but 40
+// and 63 us for the two norms, whose operands lie differently; several steps'
+// loads at once took 42 us for 4,464 x 2,394.
 constexpr int kRow8AnyThreads = 256;
 constexpr int kRow8AnyMax = 49152;  // elements: 192 KB of shared memory
 
@@ -441,22 +443,33 @@ __global__ void __launch_bounds__(kRow8AnyThreads) row8_any_kernel(const __grid_
   if (threadIdx.x == 0) p.scale[row] = scale;
 }
 
-// out[r, :] = codes[r, :] * scale[r], rounded once.  W = 16, 4 or 1 codes a
-// thread; grid (column groups, rows).
-template <typename T, int W>
+// Elements from the last multiple of 16 bytes before p to p.
+template <typename T>
+__device__ __forceinline__ int row_lead(const T* p) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+}
+
+// out[r, :] = codes[r, :] * scale[r], rounded once; grid (column groups, rows).
+// VEC: 16 codes a thread, of rows of codes and results that begin at multiples
+// of 16 bytes.  Otherwise a thread writes one 16-byte vector of the results,
+// whose codes it cuts out of the words around them (rows of codes at multiples
+// of 4 bytes; else, and at the row's ends, by elements): 4,464 x 2,394 in 11 us,
+// by elements in 47.  Bound: HBM; 6,208 x 2,048 7.9 us (4.8 TB/s).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequant8_kernel(const int8_t* __restrict__ codes, long long ldc,
                                                        const float* __restrict__ scale, T* __restrict__ out,
                                                        long long rows, int h) {
   pdl_launch_dependents();
   pdl_wait();
-  const int e = (blockIdx.x * blockDim.x + threadIdx.x) * W;
-  if (e >= h) return;
+  const int at = blockIdx.x * blockDim.x + threadIdx.x;
   for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
-    const float s = __ldg(scale + row);
-    const int8_t* src = codes + row * ldc + e;
-    T* dst = out + row * h + e;
-    if constexpr (W == 16) {
-      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src));
+    const int8_t* src = codes + row * ldc;
+    T* dst = out + row * h;
+    if constexpr (VEC) {
+      const int e = 16 * at;
+      if (e >= h) return;
+      const float s = __ldg(scale + row);
+      const uint4 raw = __ldg(reinterpret_cast<const uint4*>(src + e));
       const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -464,15 +477,41 @@ __global__ void __launch_bounds__(256) dequant8_kernel(const int8_t* __restrict_
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           v[j] = static_cast<float>(static_cast<int8_t>(w[2 * half + (j >> 2)] >> (8 * (j & 3)))) * s;
-        store8(dst + 8 * half, v);
+        store8(dst + e + 8 * half, v);
       }
     } else {
-      struct alignas(W) Bytes { int8_t x[W]; };
-      const Bytes c = *reinterpret_cast<const Bytes*>(src);
-      float v[W];
+      constexpr int E = 16 / sizeof(T);
+      const int e = E * at - row_lead(dst);
+      if (e >= h) continue;
+      const float s = __ldg(scale + row);
+      float v[E];
+      if (e >= 0 && e + E <= h && (reinterpret_cast<uintptr_t>(src) & 3) == 0) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(src + (e & ~3));
+        const int cut = e & 3;
+        uint32_t w[E / 4 + 1];
 #pragma unroll
-      for (int i = 0; i < W; ++i) v[i] = static_cast<float>(c.x[i]) * s;
-      store_few<W>(dst, v);
+        for (int i = 0; i < E / 4; ++i) w[i] = __ldg(words + i);
+        w[E / 4] = cut ? __ldg(words + E / 4) : 0u;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const uint32_t four = __funnelshift_r(w[j / 4], w[j / 4 + 1], 8 * cut);
+          v[j] = static_cast<float>(static_cast<int8_t>(four >> (8 * (j & 3)))) * s;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = e + j >= 0 && e + j < h ? static_cast<float>(src[e + j]) * s : 0.f;
+      }
+      if (e >= 0 && e + E <= h) {
+        uint4 whole;
+        T* y = reinterpret_cast<T*>(&whole);
+#pragma unroll
+        for (int j = 0; j < E; ++j) y[j] = from_float<T>(v[j]);
+        *reinterpret_cast<uint4*>(dst + e) = whole;
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (e + j >= 0 && e + j < h) dst[e + j] = from_float<T>(v[j]);
+      }
     }
   }
 }

@@ -442,17 +442,15 @@ int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t 
                   void* out, void* stream) {
   if (int e = check_rows8(rows, h, out, h, codes, ldc, scale, "dequant8")) return e;
   if (rows == 0) return ok();
-  const int size = elem_size(dtype);
-  const int w = h % 16 == 0 && rows_aligned(codes, ldc, 1, 16) && aligned(out, 16)        ? 16
-                : h % 4 == 0 && rows_aligned(codes, ldc, 1, 4) && aligned(out, 4 * size) ? 4
-                                                                                         : 1;
+  const bool vec = h % 16 == 0 && rows_aligned(codes, ldc, 1, 16) && aligned(out, 16);
   return by_dtype(dtype, true, "dequant8", [&](auto tag) {
     using T = decltype(tag);
-    const int groups = (h + w - 1) / w, threads = std::min(256, (groups + 31) / 32 * 32);
+    const int each = vec ? 16 : 16 / static_cast<int>(sizeof(T));
+    const int groups = (h + each - 1) / each + !vec;  // one more where a row may begin inside its first vector
+    const int threads = std::min(256, (groups + 31) / 32 * 32);
     const dim3 grid((groups + threads - 1) / threads, static_cast<unsigned>(std::min<int64_t>(rows, 65535)));
-    const auto kernel = w == 16 ? dequant8_kernel<T, 16> : w == 4 ? dequant8_kernel<T, 4> : dequant8_kernel<T, 1>;
-    return cuda_status(launch_kernel(kernel, grid, dim3(threads), 0, static_cast<cudaStream_t>(stream), 1, codes, ldc, scale,
-                                     static_cast<T*>(out), rows, h))
+    return cuda_status(launch_kernel(vec ? dequant8_kernel<T, true> : dequant8_kernel<T, false>, grid, dim3(threads), 0,
+                                     static_cast<cudaStream_t>(stream), 1, codes, ldc, scale, static_cast<T*>(out), rows, h))
                ? W4A4_ERR_CUDA
                : ok();
   });
