@@ -6,6 +6,7 @@
 #include <torch/library.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -45,6 +46,12 @@ void check_cuda(const Tensor& t, const char* what) {
 
 void check_device(const Tensor& t, const Tensor& x, const char* what) {
   TORCH_CHECK(t.device() == x.device(), what, " is on ", t.device(), " but the input is on ", x.device());
+}
+
+// The results have no gradient: an input that wants one would silently lose it.
+void check_no_gradient(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
+              "the pi05_w8a8 ops have no gradient, but ", what, " requires one: call them under torch.no_grad()");
 }
 
 int32_t as_i32(int64_t v, const char* what) {
@@ -127,6 +134,8 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_quant(const Tensor& x, const Tensor&
                                                   const OptTensor& delta, const OptTensor& gate,
                                                   const OptTensor& shift) {
   check_rows(x, "x");
+  check_no_gradient(x, "x");
+  if (delta.has_value()) check_no_gradient(*delta, "delta");
   const int32_t dt = dtype_code(x.scalar_type(), true, "x");
   if (delta.has_value()) {
     check_device(*delta, x, "delta");
@@ -157,6 +166,8 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_quant(const Tensor& x, const Tensor&
 
 std::tuple<Tensor, Tensor> quantize(const Tensor& x, const OptTensor& up) {
   check_rows(x, "x");
+  check_no_gradient(x, "x");
+  if (up.has_value()) check_no_gradient(*up, "up");
   const int32_t dt = dtype_code(x.scalar_type(), true, "x");
   if (up.has_value()) {
     check_device(*up, x, "up");
@@ -303,6 +314,8 @@ Tensor kv_append(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_s
   TORCH_CHECK(v.sizes() == k.sizes() && v.scalar_type() == k.scalar_type(), "new values must have the keys' shape and dtype");
   check_device(k, k_cache, "new keys");
   check_device(v, k_cache, "new values");
+  check_no_gradient(k, "the new keys");
+  check_no_gradient(v, "the new values");
   const int32_t* start_ptr = check_lengths(start, k_cache, "start");
   const int64_t tokens = k.size(1);
   Tensor mask;
@@ -350,6 +363,7 @@ Tensor kv_attention(const Tensor& q, const Tensor& k_cache, const Tensor& v_cach
                     const Tensor& v_scale, const Tensor& lengths, bool causal, double scale) {
   const Cache c = check_cache(k_cache, v_cache, k_scale, v_scale);
   check_device(q, k_cache, "q");
+  check_no_gradient(q, "q");
   const int32_t dt = dtype_code(q.scalar_type(), false, "q");
   TORCH_CHECK(q.dim() == 4 && q.size(0) == c.batch && q.size(3) == c.width && q.size(2) > 0 && q.size(2) % c.heads == 0,
               "q must be [", c.batch, ", tokens, a multiple of ", c.heads, " heads, ", c.width, "], got ", q.sizes());
@@ -387,7 +401,7 @@ TORCH_LIBRARY_IMPL(pi05_w8a8, CompositeExplicitAutograd, m) {
   m.impl("kv_attention", &kv_attention);
 }
 
-// No op has a gradient: calls go past the autograd keys to the bodies.
+// No op has a gradient (check_no_gradient): calls go past the autograd keys to the bodies.
 namespace {
 void past_autograd(torch::Library& m) {
   for (const char* op : {"rms_norm_quant", "quantize", "dequantize", "linear", "kv_append", "kv_values", "kv_attention"})

@@ -743,6 +743,25 @@ def test_ops_refuse_bad_arguments():
     refuses("64, 128 or 256", lambda: w8a8.kv_values(wide, n))
 
 
+
+@pytest.mark.gpu
+def test_ops_refuse_inputs_that_want_a_gradient():
+    x = torch.ones(1, 1, 1, 64, dtype=torch.float16, device=DEV)
+    wants = x.clone().requires_grad_()
+    ones = torch.ones(64, device=DEV)
+    cache, n = w8a8.KVCache8.allocate(1, 16, 1, 64, DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    calls = (lambda t: w8a8.quantize(t), lambda t: w8a8.quantize(x, up=t), lambda t: w8a8.rms_norm_quant(t, ones),
+             lambda t: w8a8.rms_norm_quant(x, ones, delta=t), lambda t: w8a8.kv_append(cache, t, x, n),
+             lambda t: w8a8.kv_append(cache, x, t, n), lambda t: w8a8.kv_attention(t, cache, n))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(wants)
+        with torch.no_grad():
+            call(wants)
+        call(wants.detach())
+    assert w8a8.pack_weight(torch.nn.Parameter(torch.ones(8, 64, device=DEV))).codes.shape == (8, 64)
+
+
 # --- the operators together: the SnapFlow action expert in 8 bits -----------
 
 
