@@ -754,12 +754,14 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       const uint32_t idesc_s = idesc_f16(C::kRows, C::kKeys);
       const uint32_t idesc_o = idesc_f16(C::kRows, D);
       bool alive = nt == 0 || warp_all(mbar_wait_spin(bar_q, 0, abort_flag, err, kErrWaitUnpack, limit));
-      // whichever product is ready next: S(si) (its keys are there and S(si - 1) has been read) or P(pi) V
+      // whichever product is ready next: S(si) (its keys are there and S(si - 1) has been read) or P(pi) V.  S(si) comes
+      // after P(si - 3) V, so that bar_sfull(si) covers it too: the group of tile si may wait for P(si - 1) V, by parity
+      // on the other group's barrier, and must know the phase before that one to be over
       int si = 0, pi = 0, idle = 0;
       uint64_t since = 0;
       while (alive && pi < nt) {
         const int ss = si & 1, ps = pi & 1;
-        const bool s_ready = si < nt && mbar_test_wait(bar_kfull(ss), (si >> 1) & 1) &&
+        const bool s_ready = si < nt && si <= pi + 2 && mbar_test_wait(bar_kfull(ss), (si >> 1) & 1) &&
                              (si == 0 || mbar_test_wait(bar_sread, (si - 1) & 1));
         if (__any_sync(0xffffffffu, s_ready)) {
           tc_fence_after();

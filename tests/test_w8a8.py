@@ -514,6 +514,32 @@ def test_kv_attention_over_wide_ranges(tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_kv_attention_rescales_at_every_tile(width):
+    """Many rows over up to 20 tiles of 64 keys whose scores grow by about 18
+    bits a tile, so that each tile rescales what the one before it has just
+    accumulated, sequences of every number of tiles among them.  Enough CTAs
+    that none shares its keys with another; the same bits every time."""
+    b, tokens, group, cap = 80, 66, 2, 1280
+    g = gen(width)
+    codes, scale = cache_state(g, b, cap, 1, width)
+    codes[0, ..., 0] = 127
+    scale[0] = (0.01 + 0.4 * (torch.arange(cap // 16) // 4)).float()
+    q = 0.02 * randn(g, b, tokens, group, width)
+    q[..., 0] = 4
+    q = q.bfloat16()
+    n = torch.tensor([16 * (i + 1) - i % 16 for i in range(b)], dtype=torch.int32)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    qg, ng = on_gpu(q), on_gpu(n)
+    out = w8a8.kv_attention(qg, cache, ng, softmax_scale=1 / 16)
+    for _ in range(20):
+        assert torch.equal(w8a8.kv_attention(qg, cache, ng, softmax_scale=1 / 16), out)
+    want = attention64(q, codes, scale, n, False, 1 / 16)
+    within(out, want[0], attention_tol(torch.bfloat16, *want))
+    assert nat.device_error() == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 70])
 def test_kv_attention_strides_and_sentinel_lengths(tokens):
     q, codes, scale, n = attention_inputs(4, 2, 64, 96, (96, 50), tokens, torch.float16, 21)
