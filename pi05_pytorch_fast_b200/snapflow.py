@@ -364,15 +364,6 @@ class ActionExpert8(ActionExpert):
                 setattr(self, name, module)
         with torch.no_grad():
             self.layers = [ExpertLayer8(layer) for layer in expert.layers]
-        self._caches: dict = {}
-
-    def _cache(self, b: int, tokens: int, device) -> tuple[w8a8.KVCache8, torch.Tensor]:
-        # one cache for all layers: each fills it from its first slot again
-        key = (b, tokens)
-        if key not in self._caches:
-            self._caches[key] = (w8a8.KVCache8.allocate(b, tokens, self.cfg.expert_kv_heads, self.cfg.head_dim, device),
-                                 torch.zeros(b, dtype=torch.int32, device=device))
-        return self._caches[key]
 
     def launches_per_forward(self) -> int:
         """Kernels of the layers (the attention counted as one)."""
@@ -383,7 +374,11 @@ class ActionExpert8(ActionExpert):
         cfg = self.cfg
         b = x_t.shape[0]
         x, mod, rope = self.prepare(x_t, t, target_t, prefix_pad)
-        cache, empty = self._cache(b, prefix_pad.shape[1] + cfg.chunk, x.device)
+        # of this call alone, so that calls on other streams and captured graphs have their own; one for all layers, each
+        # of which fills it from its first slot again
+        cache = w8a8.KVCache8.allocate(b, prefix_pad.shape[1] + cfg.chunk, cfg.expert_kv_heads, cfg.head_dim, x.device,
+                                       clear=False)
+        empty = torch.zeros(b, dtype=torch.int32, device=x.device)
         delta = gate = None
         for i, (layer, k, v) in enumerate(zip(self.layers, keys, values)):
             pk, pv = (a.view(b, -1, cfg.expert_kv_heads, cfg.head_dim) for a in (k, v))

@@ -109,11 +109,15 @@ class KVCache8(NamedTuple):
     value_scale: torch.Tensor
 
     @classmethod
-    def allocate(cls, batch: int, capacity: int, heads: int, width: int, device) -> "KVCache8":
-        """An empty cache; the capacity is rounded up to a multiple of 16."""
+    def allocate(cls, batch: int, capacity: int, heads: int, width: int, device, *, clear: bool = True) -> "KVCache8":
+        """An empty cache; the capacity is rounded up to a multiple of 16.
+        ``clear=False`` leaves its memory as it is, which no result of the
+        operators depends on: they use no slot from the length on, and no scale
+        of a block that has none below it."""
         capacity = (capacity + CACHE_BLOCK - 1) // CACHE_BLOCK * CACHE_BLOCK
-        codes = torch.zeros((2, batch, capacity, heads, width), dtype=torch.int8, device=device)
-        scale = torch.zeros((2, batch, heads, capacity // CACHE_BLOCK), dtype=torch.float32, device=device)
+        make = torch.zeros if clear else torch.empty
+        codes = make((2, batch, capacity, heads, width), dtype=torch.int8, device=device)
+        scale = make((2, batch, heads, capacity // CACHE_BLOCK), dtype=torch.float32, device=device)
         return cls(codes[0], codes[1], scale[0], scale[1])
 
 

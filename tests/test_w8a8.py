@@ -14,6 +14,7 @@ import pytest
 import torch
 
 from pi05_pytorch_fast_b200 import _native as nat
+from pi05_pytorch_fast_b200 import prefix_lm as plm
 from pi05_pytorch_fast_b200 import snapflow as sf
 from pi05_pytorch_fast_b200 import w8a8
 
@@ -864,6 +865,87 @@ def test_snapflow_expert_in_8_bits_in_a_graph():
             out = expert8(*inputs)
         graph.replay()
     assert torch.equal(out, eager)
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_first_called_under_capture():
+    """A shape's first call recorded in a graph, an eager call before the graph
+    has run once, and the graph then: each as the call alone."""
+    expert, inputs = _expert(layers=1)
+    expert8 = sf.ActionExpert8(expert)
+    alone = sf.ActionExpert8(expert)
+    x_t, t, target, pad, keys, values = inputs
+    with torch.no_grad():
+        want = alone(*inputs)
+        expert8(x_t[:1], t[:1], target[:1], pad[:1], [k[:1] for k in keys], [v[:1] for v in values])  # libraries' set-up
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = expert8(*inputs)
+        eager = expert8(*inputs)
+        assert torch.equal(eager, want)
+        graph.replay()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_on_two_streams():
+    """Calls of one expert that run at the same time do not meet."""
+    expert, inputs = _expert()
+    expert8 = sf.ActionExpert8(expert)
+    x_t, t, target, pad, keys, values = inputs
+    other = (x_t.flip(0) * 3, t, target, ~pad, [k * 2 for k in keys], [v.flip(0) for v in values])
+    with torch.no_grad():
+        want = [expert8(*inputs), expert8(*other)]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        got = ([], [])
+        for _ in range(20):
+            for i, args in enumerate((inputs, other)):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(expert8(*args))
+        torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(v, w) for v in g)
+
+
+@pytest.mark.gpu
+def test_snapflow_expert_in_8_bits_keeps_nothing():
+    expert, inputs = _expert(layers=1)
+    expert8 = sf.ActionExpert8(expert)
+    x_t, t, target, pad, keys, values = inputs
+
+    def call(n, b):
+        with torch.no_grad():
+            expert8(x_t[:b], t[:b], target[:b], pad[:b, :n], [k[:b, :n] for k in keys], [v[:b, :n] for v in values])
+
+    call(40, 2), call(40, 1)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for n in (8, 24, 33):
+        call(n, 1)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.gpu
+def test_snapflow_policy_with_the_expert_in_8_bits():
+    """The whole step, eager and as a graph, and its velocity next to that of
+    the bf16 policy of the same weights: two layers, so at most 6 % for the 8
+    bits (see above) and 1 % for bf16 on either side."""
+    dev = torch.device("cuda:0")
+    lm_cfg = plm.PrefixLMConfig(layers=2)
+    cfg = sf.SnapFlowConfig(vision_layers=1, expert_layers=2, vocab=512, lm=lm_cfg)
+    lm = plm.W4A4PrefixLM.random(lm_cfg, dev, seed=5)
+    policy8 = sf.SnapFlowPolicy(cfg, lm, dev, seed=6, expert_bits=8)
+    obs = sf.synthetic_observation(cfg, 2, seed=7, device=dev)
+    eager = policy8.sample_actions(*obs)
+    graphed = sf.GraphedSnapFlow(policy8, 2)
+    assert torch.equal(graphed.run(*obs), eager)
+    x_t = obs[3].bfloat16().double()
+    v8 = x_t - eager.double()
+    v16 = x_t - sf.SnapFlowPolicy(cfg, lm, dev, seed=6).sample_actions(*obs).double()
+    rel = (v8 - v16).norm() / v16.norm()
+    assert rel < 0.08, float(rel)
 
 
 def test_snapflow_expert_in_8_bits_refusals():
