@@ -13,14 +13,17 @@
 //  * Q in fp16 times a power of two for each row (bf16 queries keep their 8
 //    bits wherever an element is within 2^28 of the row's largest);
 //  * scores, row maxima, row sums and O in fp32, softmax in base 2;
-//  * the reference m of a row is set 2^4 above the maximum so far and moves only
-//    when a block exceeds it by more than 2^11, so that O is rarely rescaled (a
-//    rescale of 128 x 256 takes as long as two tiles): p = 2^(s - m) <= 2^11;
-//  * p vs / vref is rounded to fp16 for the P V product (11 bits, as the
-//    scores' own error after exp2 is not much smaller).  vref, a running
-//    reference for the value scales, moves (and O is rescaled) when a scale
-//    exceeds it by more than 2^4: p vs / vref <= 2^15 fits fp16, and what
-//    falls below its range is below 2^-20 of the row's largest term.
+//  * a row has two running references.  m is for the sum l of p = 2^(s - m); r
+//    is for O, whose weights are w = 2^(s - r) vs, and follows s + e with e the
+//    exponent of vs (2^e <= vs < 2^(e+1)), so that it is the row's own largest
+//    terms that decide it, whatever the scales of blocks with little weight or
+//    of blocks that the row does not see.  Both are set 2^4 above the maximum so
+//    far and move only when a block exceeds them by more than 2^11, so that O is
+//    rarely rescaled (a rescale of 128 x 256 takes as long as two tiles);
+//  * w = p (vs 2^(m - r)) is one exponential a key and one factor a block.  It is
+//    rounded to fp16 for the P V product (11 bits, as the scores' own error after
+//    exp2 is not much smaller): w < 2^12 fits, the row's largest one is at least
+//    2^-4, so what falls below fp16's range is below 2^-20 of it.
 // When the keys of a head are split over CTAs, each writes its unnormalised O
 // with (m, l) and attn8_join_kernel adds them up.
 #pragma once
@@ -35,9 +38,8 @@ namespace w4a4 {
 // cluster's CTA holds could wait for good, each cluster's other half being
 // blocked by the other.
 constexpr int kOneCtaSmem = 117 * 1024;
-constexpr float kAttn8Margin = 4.f;    // log2 by which m is set above a row's maximum
-constexpr float kAttn8Grow = 11.f;     // log2 by which a block may exceed m
-constexpr float kAttn8VGrow = 16.f;    // factor by which a value scale may exceed vref
+constexpr float kAttn8Margin = 4.f;    // log2 by which m and r are set above a row's maxima
+constexpr float kAttn8Grow = 11.f;     // log2 by which a block may exceed them
 
 struct Attn8Params {
   const void* q;  // [batch, tokens, q_heads, width]
@@ -88,23 +90,25 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Ratio of a block's value scale to the reference, and the reference's move:
-// returns the factor for what was accumulated so far (1: no move).  A scale
-// that is not finite never becomes the reference (rows that do not see its
-// block stay clean); its ratio is NaN.
-__device__ __forceinline__ float move_vref(float vsc, float& vref) {
-  if (!(vsc > kAttn8VGrow * vref) || vsc > 3.4028234e38f) return 1.f;
-  const float f = vref / vsc;
-  vref = vsc;
-  return f;
+constexpr float kMaxFloat = 3.4028234e38f;
+
+// The exponent of a value scale; none (-infinity) for zero, and for one that is
+// not finite, whose rows are not finite whatever the reference.
+__device__ __forceinline__ float value_exponent(float vs) {
+  const float e = __uint_as_float(0x4b000000u | (__float_as_uint(vs) >> 23)) - (8388608.f + 127.f);
+  return vs > 0.f && vs <= kMaxFloat ? e : -INFINITY;
 }
-__device__ __forceinline__ float vscale_ratio(float vsc, float vref) {
-  if (vsc == 0.f) return 0.f;
-  if (!(vsc <= 3.4028234e38f)) return __uint_as_float(0x7fc00000u);
-  return vref >= 1e-30f ? __fdividef(vsc, vref) : vsc / vref;  // the quick division wants a normal divisor
+// 2^(d / 2): half of the way from one reference to another, as the whole of it
+// may leave fp32's range where its product with a scale does not.
+__device__ __forceinline__ float half_way(float d) { return fminf(ex2_approx(0.5f * d), 8.507059e37f); }  // 2^126
+// What turns p into w: vs 2^(m - r), `half` being half_way(m - r).  Past fp32's range
+// p is zero.
+__device__ __forceinline__ float value_factor(float vs, float half) { return fminf(vs * half * half, kMaxFloat); }
+__device__ __forceinline__ float any_value_factor(float vs, float half) {
+  return vs <= kMaxFloat ? value_factor(vs, half) : __uint_as_float(0x7fc00000u);
 }
-// p times the ratio; keys that are not seen (p = 0) add nothing whatever it is.
-__device__ __forceinline__ float weigh(float p, float rv) { return p == 0.f ? 0.f : p * rv; }
+// p times that; keys that are not seen (p = 0) add nothing whatever it is.
+__device__ __forceinline__ float weigh(float p, float factor) { return p == 0.f ? 0.f : p * factor; }
 
 // The power of two by which a row of queries is multiplied so that its largest
 // element lies in [2^14, 2^15) of fp16 (1 for a zero row).
@@ -132,9 +136,10 @@ __device__ __forceinline__ int keys_seen(const Attn8Params& p, int n, int t) {
 //  * V: lane (g, t) holds dims 16 g ... + 15 of the keys 2t, 2t+1, 2t+8, 2t+9;
 //    pairs of keys are zipped with byte permutes; column n of tile e is dim
 //    16 n + e, so a lane ends with runs of 16 consecutive dims of O.
-// P goes in as the sum of two fp16, its rounding and the rest: with at most 8
+// w goes in as the sum of two fp16, its rounding and the rest: with at most 8
 // rows (HALF) the rest takes the idle rows 8-15 of the same MMA, with more it
-// is a second one.  Bound: HBM (2 width bytes per key); legacy MMA is enough
+// is a second one.  The four lanes of a row agree on r (O's columns are theirs
+// in turns); m and l are each lane's own until the end.  Bound: HBM (2 width bytes per key); legacy MMA is enough
 // for it.  Which warp takes which keys does not depend on the lengths, so the
 // first loads are under way before the length has arrived.  Measured: 8 heads of
 // 256 over 776 tokens 7.5 us, over 131,072 (67 MB) 26.5 us; 4 x 16 heads on 2 of 128
@@ -287,17 +292,16 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
   }
   __syncthreads();
   constexpr int R = HALF ? 1 : 2;  // rows g, g + 8 of a lane
-  float factor[R], m[R], l[R];
+  float factor[R], m[R], l[R], ref[R];
   int seen[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const float2 info = row_info[g + 8 * i];
     factor[i] = info.x;
     seen[i] = __float_as_int(info.y);
-    m[i] = -INFINITY;
+    m[i] = ref[i] = -INFINITY;
     l[i] = 0.f;
   }
-  float vref = 0.f;
   float o[D / 8][4];
 #pragma unroll
   for (int e = 0; e < D / 8; ++e) o[e][0] = o[e][1] = o[e][2] = o[e][3] = 0.f;
@@ -351,64 +355,70 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
     // ---- softmax of the step
     const int j0 = step * NB * kKvBlock + 2 * t;
     float vsc[NB];
-    float bm[R];
+    float bm[R], br[R];  // maxima of s, and of s + e
 #pragma unroll
-    for (int i = 0; i < R; ++i) bm[i] = -INFINITY;
+    for (int i = 0; i < R; ++i) bm[i] = br[i] = -INFINITY;
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
       const bool has = step * NB + q < nblk;  // past the length: what the stage holds is not a scale
       const float2 x = sc[q];
       vsc[q] = has ? x.y : 0.f;
+      const float e = value_exponent(vsc[q]);
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const float fk = has ? factor[i] * x.x : 0.f;
         const int left = seen[i] - j0 - 16 * q;
+        float top = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float& v = s[2 * q + (j >> 1)][2 * i + (j & 1)];
           v = (j & 1) + 8 * (j >> 1) < left ? v * fk : -INFINITY;
-          bm[i] = fmaxf(bm[i], v);
+          top = fmaxf(top, v);
         }
+        bm[i] = fmaxf(bm[i], top);
+        br[i] = fmaxf(br[i], top + e);
       }
     }
-    float f[R];
+    float f[R], half[R];
     bool grow = false;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      bm[i] = fmaxf(bm[i], __shfl_xor_sync(0xffffffffu, bm[i], 1));
-      bm[i] = fmaxf(bm[i], __shfl_xor_sync(0xffffffffu, bm[i], 2));
-      f[i] = 1.f;
       if (bm[i] > m[i] + kAttn8Grow) {
         bm[i] += kAttn8Margin;
-        f[i] = m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm[i]);
+        l[i] *= m[i] == -INFINITY ? 0.f : ex2_approx(m[i] - bm[i]);
         m[i] = bm[i];
-        l[i] *= f[i];
+      }
+      br[i] = fmaxf(br[i], __shfl_xor_sync(0xffffffffu, br[i], 1));
+      br[i] = fmaxf(br[i], __shfl_xor_sync(0xffffffffu, br[i], 2));
+      f[i] = 1.f;
+      if (br[i] > ref[i] + kAttn8Grow) {
+        br[i] += kAttn8Margin;
+        f[i] = ref[i] == -INFINITY ? 0.f : ex2_approx(ref[i] - br[i]);
+        ref[i] = br[i];
         grow = true;
       }
+      half[i] = half_way(m[i] - ref[i]);
     }
-    float fv = 1.f;
-#pragma unroll
-    for (int q = 0; q < NB; ++q) fv *= move_vref(vsc[q], vref);
-    if (__any_sync(0xffffffffu, grow) || fv != 1.f) {
+    if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
       for (int e = 0; e < D / 8; ++e)
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-          o[e][2 * i] *= f[i] * fv;
-          o[e][2 * i + 1] *= f[i] * fv;
-          if constexpr (HALF) {  // rows 8-15 hold what the rest of P adds to rows 0-7
-            o[e][2] *= f[0] * fv;
-            o[e][3] *= f[0] * fv;
+          o[e][2 * i] *= f[i];
+          o[e][2 * i + 1] *= f[i];
+          if constexpr (HALF) {  // rows 8-15 hold what the rest of w adds to rows 0-7
+            o[e][2] *= f[0];
+            o[e][3] *= f[0];
           }
         }
     }
 #pragma unroll
     for (int q = 0; q < NB; ++q) {
-      const float rv = vscale_ratio(vsc[q], vref);
-      uint32_t ph[R][2], pl[R][2];  // P and the rest of its rounding: [rows][keys]
+      uint32_t ph[R][2], pl[R][2];  // w and the rest of its rounding: [rows][keys]
 #pragma unroll
       for (int i = 0; i < R; ++i) {
         const float nm = m[i] == -INFINITY ? 0.f : -m[i];
+        const float rv = any_value_factor(vsc[q], half[i]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const float p0 = ex2_approx(s[2 * q + j][2 * i] + nm), p1 = ex2_approx(s[2 * q + j][2 * i + 1] + nm);
@@ -465,9 +475,13 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
   // ---- the CTA's warps: O, m and l of each through shared memory
 #pragma unroll
   for (int i = 0; i < R; ++i) {
+    float top = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));  // the row's m, from its lanes'
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    l[i] *= m[i] == -INFINITY ? 1.f : ex2_approx(m[i] - top);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-    if (t == 0) warp_ml[warp * C::kRowsMax + g + 8 * i] = make_float2(m[i], l[i]);
+    if (t == 0) warp_ml[warp * C::kRowsMax + g + 8 * i] = make_float2(top, l[i]);
+    const float back = top == -INFINITY ? 0.f : half_way(ref[i] - top);  // O as the others' will be: with 2^-m
     float* row = xo + (warp * C::kRowsMax + g + 8 * i) * C::kPad;
 #pragma unroll
     for (int half = 0; half < 2; ++half)
@@ -479,7 +493,7 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
         float* xs = &x.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          xs[j] = (HALF ? o[e + j][half] + o[e + j][2 + half] : o[e + j][2 * i + half]) * vref;
+          xs[j] = (HALF ? o[e + j][half] + o[e + j][2 + half] : o[e + j][2 * i + half]) * back * back;
         *reinterpret_cast<float4*>(row + dim) = x;
       }
   }
@@ -562,8 +576,8 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
 // eight warps of their own:
 //   warps 0-7    softmax and epilogue (thread = row = TMEM lane): warps 0-3 take
 //                the even tiles, 4-7 the odd ones, so that one group's
-//                exponentials run beside the other's maxima; the running maximum
-//                passes from tile to tile through shared memory
+//                exponentials run beside the other's maxima; each has its own m
+//                and l, and r passes from tile to tile through shared memory
 //   warps 8-11   keys: 16 codes a load -> K-major rows, 128-byte swizzle
 //   warps 12-15  values: 8 keys of up to 16 dims -> V^T rows of 64 keys (byte
 //                permutes), as the second product wants its B operand K-major
@@ -591,9 +605,9 @@ struct Attn8Many {
   static constexpr int kPoolRegs = 256 * kSoftRegs + 256 * kConvRegs + 128 * kRestRegs;
   static constexpr int kNumBars = 33;
   // K and V^T rings (the raw Q before, and O after the tiles, use them), rings of codes, row data: score factor, keys
-  // seen; sums of both groups; running maxima; the last vref
+  // seen; l of both groups; r; m of both groups
   static constexpr int kRing = 2 * (kKBytes + kVBytes);
-  static constexpr int kNeed = kRing + 4 * kRaw + kRows * 8 + 4 * kRows * 4 + kNumBars * 8 + 32 + 1024;
+  static constexpr int kNeed = kRing + 4 * kRaw + kRows * 8 + 5 * kRows * 4 + kNumBars * 8 + 32 + 1024;
   static constexpr uint32_t kTmemCols = D == 64 ? 256 : 512;
   static constexpr int kSmem = kNeed > kOneCtaSmem ? kNeed : kOneCtaSmem;
   static constexpr uint32_t kOCol = 0, kQCol = D, kSCol = D == 64 ? 128 : D + D / 2, kPCol = kSCol + kKeys;
@@ -624,9 +638,9 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
   uint8_t* v_raw = k_raw + 2 * C::kRaw;
   float2* row_info = reinterpret_cast<float2*>(v_raw + 2 * C::kRaw);      // score factor, keys seen
   float* row_x = reinterpret_cast<float*>(row_info + C::kRows);           // [2 groups][128 rows]: amax of half of Q, later l
-  float* row_m = row_x + 2 * C::kRows;                                    // running maxima
-  float* row_v = row_m + C::kRows;                                        // the last tile's vref
-  uint64_t* bars = reinterpret_cast<uint64_t*>(row_v + C::kRows);
+  float* row_r = row_x + 2 * C::kRows;                                    // running references of O
+  float* row_m = row_r + C::kRows;                                        // [2 groups][128 rows]: m, after the tiles
+  uint64_t* bars = reinterpret_cast<uint64_t*>(row_m + 2 * C::kRows);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* plan = reinterpret_cast<int*>(tmem_slot + 2);  // length, first tile, tiles
@@ -640,7 +654,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
   const auto bar_vempty = [&](int s) { return smem_addr(bars + 14 + s); };
   const auto bar_pfull = [&](int s) { return smem_addr(bars + 16 + s); };
   const auto bar_pfree = [&](int s) { return smem_addr(bars + 18 + s); };  // P V of that parity's last tile is done
-  const auto bar_m = [&](int q) { return smem_addr(bars + 20 + q); };      // a quarter's maxima of a tile are decided
+  const auto bar_r = [&](int q) { return smem_addr(bars + 20 + q); };      // a quarter's references of a tile are decided
   const auto bar_l = [&](int q) { return smem_addr(bars + 24 + q); };      // both groups' sums of a quarter are there
   // one for each group, as a wait for a phase must not begin before the phase before it has passed
   const auto bar_sfull = [&](int s) { return smem_addr(bars + 28 + s); };
@@ -669,7 +683,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       mbar_init(bar_sfull(s), 1);
     }
     for (int q = 0; q < 4; ++q) {
-      mbar_init(bar_m(q), 1);
+      mbar_init(bar_r(q), 1);
       mbar_init(bar_l(q), 2);
     }
     mbar_init(bar_sread, 4);
@@ -943,8 +957,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
         // that see less than a tile takes the longer way through it
         row_info[row] = make_float2(fabsf(p.scale) / shift,
                                     __int_as_float(keys_seen(p, n, p.causal ? min(r, p.rows - 1) / p.group : 0)));
-        row_m[row] = -INFINITY;
-        row_v[row] = 0.f;
+        row_r[row] = -INFINITY;
       }
 #pragma unroll 1
       for (int c = group * (QC / 2); c < (group + 1) * (QC / 2); c += 4) {
@@ -970,7 +983,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       }
       tmem_st_wait();
       tc_fence_before();
-      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_info, row_m; row_x may be written again
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_info, row_r; row_x may be written again
       if (lane == 0) mbar_arrive(bar_q);
     }
     const float2 info = row_info[row];
@@ -978,25 +991,25 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
     const int seen = __float_as_int(info.y);
     const float* ks = p.ks + static_cast<long long>(unit) * (p.capacity / kKvBlock);
     const float* vs = p.vs + static_cast<long long>(unit) * (p.capacity / kKvBlock);
-    float m = -INFINITY, l = 0.f, vref = 0.f, vinv = 0.f;
+    float m = -INFINITY, l = 0.f;
     bool alive = true;
-    // a tile's scales, one to a lane, a turn ahead: keys' (lanes 0-3), values' (4-7), the tile before's values' (8-11);
-    // zero past the length
+    // a tile's scales, one to a lane, a turn ahead: keys' (lanes 0-3), values' (4-7), the exponents of these (8-11); zero
+    // past the length
     const float* scale_src = (lane < 4 ? ks : vs) + (lane & 3);
     const auto fetch_scale = [&](int i) {
-      const int blk = (tile0 + i - (lane >= 8)) * (C::kKeys / kKvBlock);
-      return lane < 12 && i < nt && blk >= 0 && blk + (lane & 3) < nblocks ? __ldg(scale_src + blk) : 0.f;
+      const int blk = (tile0 + i) * (C::kKeys / kKvBlock);
+      const float v = lane < 12 && i < nt && blk + (lane & 3) < nblocks ? __ldg(scale_src + blk) : 0.f;
+      return lane < 8 ? v : value_exponent(v);
     };
     float scales = fetch_scale(group);
-    const auto largest = [](const float (&v)[4]) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); };  // passes NaN by
     for (int i = group; i < nt; i += 2) {
       const int j0 = (tile0 + i) * C::kKeys;
-      float ksc[4], vsc[4], vbefore[4];
+      float ksc[4], vsc[4], ve[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         ksc[q] = __shfl_sync(0xffffffffu, scales, q) * factor;
         vsc[q] = __shfl_sync(0xffffffffu, scales, 4 + q);
-        vbefore[q] = __shfl_sync(0xffffffffu, scales, 8 + q);
+        ve[q] = __shfl_sync(0xffffffffu, scales, 8 + q);
       }
       scales = fetch_scale(i + 2);
       if (!warp_all(mbar_wait_spin(bar_sfull(group), (i >> 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
@@ -1012,9 +1025,9 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_sread);
-      // ---- the tile's maximum of the row; column c is key 8 (c % 8) + c / 8, whose scale is number (c % 8) / 2.  Keys
-      // that the row does not see are left out, whatever their block's scale
-      float bmax = -INFINITY;
+      // ---- the row's maxima of the tile, of s and of s + e; column c is key 8 (c % 8) + c / 8, whose scale is number
+      // (c % 8) / 2.  Keys that the row does not see are left out, whatever their block's scales
+      float bmax = -INFINITY, rmax = -INFINITY;
       const int left = seen - j0;
       const bool whole = __all_sync(0xffffffffu, left >= C::kKeys);
 #pragma unroll
@@ -1034,36 +1047,28 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
           }
         }
         x0 = fmaxf(x0, x1);
-        if (x0 > -INFINITY) bmax = fmaxf(bmax, x0 * ksc[q]);  // the factor is not negative
-      }
-      // ---- m as the tile before left it, then this tile's
-      if (i > 0) {
-        if (!warp_all(mbar_wait_spin(bar_m(quarter), (i - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
-          alive = false;
-          break;
-        }
-        const float mb = row_m[row];
-        if (mb != m) {
-          l *= m == -INFINITY ? 0.f : ex2_approx(m - mb);
-          m = mb;
-        }
-        if (largest(vbefore) > kAttn8VGrow * vref) {  // O has been rescaled for it
-#pragma unroll
-          for (int q = 0; q < 4; ++q) move_vref(vbefore[q], vref);
-          vinv = vref >= 1e-30f ? __fdividef(1.f, vref) : 0.f;
+        if (x0 > -INFINITY) {
+          x0 *= ksc[q];  // the factor is not negative
+          bmax = fmaxf(bmax, x0);
+          rmax = fmaxf(rmax, x0 + ve[q]);
         }
       }
-      float f = 1.f;
       if (bmax > m + kAttn8Grow) {
         bmax += kAttn8Margin;
-        f = m == -INFINITY ? 0.f : ex2_approx(m - bmax);
+        l *= m == -INFINITY ? 0.f : ex2_approx(m - bmax);
         m = bmax;
-        l *= f;
       }
-      if (largest(vsc) > kAttn8VGrow * vref) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) f *= move_vref(vsc[q], vref);
-        vinv = vref >= 1e-30f ? __fdividef(1.f, vref) : 0.f;
+      // ---- r as the tile before left it, then this tile's
+      if (i > 0 && !warp_all(mbar_wait_spin(bar_r(quarter), (i - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
+        alive = false;
+        break;
+      }
+      float ref = row_r[row];
+      float f = 1.f;
+      if (rmax > ref + kAttn8Grow) {
+        rmax += kAttn8Margin;
+        f = ref == -INFINITY ? 0.f : ex2_approx(ref - rmax);
+        ref = rmax;
       }
       if (i >= 1 && __any_sync(0xffffffffu, f != 1.f)) {
         // O holds the earlier tiles: wait for the last of them, rescale this warp's rows
@@ -1086,15 +1091,16 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
         tmem_st_wait();
         tc_fence_before();
       }
-      row_m[row] = m;
+      row_r[row] = ref;
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_m(quarter));
-      // ---- P = 2^(s - m), times vs / vref
+      if (lane == 0) mbar_arrive(bar_r(quarter));
+      // ---- w = p (vs 2^(m - r))
       const float nm = m == -INFINITY ? 0.f : -m;
-      const bool plain = whole && vsc[0] + vsc[1] + vsc[2] + vsc[3] <= 3.4028234e38f;  // false for NaN
+      const bool plain = whole && vsc[0] + vsc[1] + vsc[2] + vsc[3] <= kMaxFloat;  // false for NaN
+      const float half = half_way(m - ref);
       float rv[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) rv[q] = vinv > 0.f && plain ? vsc[q] * vinv : vscale_ratio(vsc[q], vref);
+      for (int q = 0; q < 4; ++q) rv[q] = plain ? value_factor(vsc[q], half) : any_value_factor(vsc[q], half);
       if (i >= 2 && !warp_all(mbar_wait_spin(bar_pfree(group), ((i >> 1) - 1) & 1, abort_flag, err, kErrWaitAccum, limit))) {
         alive = false;
         break;
@@ -1139,26 +1145,27 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar_pfull(group));
     }
-    // ---- epilogue: O vref / l as T, or the unnormalised O vref and (m, l) of this split, to shared memory (the
-    // idle rings)
+    // ---- epilogue: O 2^(r - m) / l as T, or without the division and with (m, l) for this split, to shared memory (the
+    // idle rings).  Where a wait gave up l is NaN
     alive = alive && warp_all(mbar_wait_bounded(bar_o, 0, abort_flag, err, kErrWaitAccum, limit));
     tc_fence_after();
+    row_x[group * C::kRows + row] = l;
+    row_m[group * C::kRows + row] = m;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar_l(quarter));
+    alive = warp_all(mbar_wait_spin(bar_l(quarter), 0, abort_flag, err, kErrWaitAccum, limit)) && alive;
     {
-      // the groups' sums, each at its own last maximum; the last tile's group has the final vref
-      const float mb = row_m[row];
-      row_x[group * C::kRows + row] = m == -INFINITY ? l : l * ex2_approx(m - mb);
-      if (nt > 0 && group == ((nt - 1) & 1)) row_v[row] = vref;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_l(quarter));
-      alive = warp_all(mbar_wait_spin(bar_l(quarter), 0, abort_flag, err, kErrWaitAccum, limit)) && alive;
-      m = mb;
-      l = row_x[row] + row_x[C::kRows + row];
-      vref = row_v[row];
+      const float m0 = row_m[row], m1 = row_m[C::kRows + row];
+      m = fmaxf(m0, m1);
+      l = (m0 == -INFINITY ? 0.f : row_x[row] * ex2_approx(m0 - m)) +
+          (m1 == -INFINITY ? 0.f : row_x[C::kRows + row] * ex2_approx(m1 - m));
     }
+    if (!alive) l = __uint_as_float(0x7fc00000u);
     const bool part = p.splits > 1;
-    const float f = part ? vref : l == 0.f ? 0.f : vref / l;
+    const float back = half_way(row_r[row] - m);  // half of the way from r to m
+    const float f = part ? back : back / l;
     if (part && group == 0 && r < p.rows)
-      p.part_ml[(static_cast<long long>(unit) * p.splits + split) * p.rows + r] = make_float2(m, alive ? l : __uint_as_float(0x7fc00000u));
+      p.part_ml[(static_cast<long long>(unit) * p.splits + split) * p.rows + r] = make_float2(m, l);
 #pragma unroll 1
     for (int c0 = group * (D / 2); c0 < (group + 1) * (D / 2); c0 += 16) {
       uint32_t o[16];
@@ -1171,7 +1178,7 @@ __global__ void __launch_bounds__(Attn8Many<D>::kThreads, 1)
       }
       float v[2][8];
 #pragma unroll
-      for (int c = 0; c < 16; ++c) v[c >> 3][c & 7] = f == 0.f ? 0.f : __uint_as_float(o[c]) * f;
+      for (int c = 0; c < 16; ++c) v[c >> 3][c & 7] = l == 0.f ? 0.f : __uint_as_float(o[c]) * back * f;
       if (part) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)

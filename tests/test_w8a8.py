@@ -540,6 +540,121 @@ def test_kv_attention_rescales_at_every_tile(width):
     assert nat.device_error() == 0
 
 
+def attention64_rows(q, codes, scale, lengths, causal, softmax_scale):
+    """(out, how far it may be off) in 64 bits, by each row's own terms alone:
+    the scores' error as in attention_tol, 11 bits of each weight P vs, and for
+    weights below fp16's normal numbers half a step of 2^-24 where the row's
+    largest weight counts at least 2^-4: n 2^-21 of it, times 127."""
+    b, t, qh, w = q.shape
+    cap, heads = codes.shape[2:4]
+    steps = scale.double().repeat_interleave(16, 3).transpose(2, 3)
+    k, v = ((codes.double() * steps[..., None])[i].repeat_interleave(qh // heads, 2) for i in range(2))
+    limit = lengths.long()[:, None].expand(b, t)
+    if causal:
+        limit = limit - t + 1 + torch.arange(t)
+    sees = (torch.arange(cap) < limit[..., None])[:, None]
+    v = torch.where((torch.arange(cap) < lengths.long()[:, None])[..., None, None], v, 0.0)
+    s = torch.einsum("bthw,bchw->bhtc", q.double(), torch.nan_to_num(k)) * softmax_scale
+    top = torch.where(sees, s.abs(), 0.0).amax(-1).permute(0, 2, 1)[..., None]
+    p = torch.nan_to_num(torch.softmax(s.masked_fill(~sees, -math.inf), -1))
+    own = torch.where(sees, p * torch.nan_to_num(steps[1].repeat_interleave(qh // heads, 2).transpose(1, 2))[:, :, None], 0.0)
+    v = torch.nan_to_num(v)
+    out, mag = (torch.einsum("bhtc,bchw->bthw", p, x) for x in (v, v.abs()))
+    largest = own.amax(-1).permute(0, 2, 1)[..., None]
+    u = U[q.dtype]
+    return out, u * out.abs() + (2.0 ** -10 + 2.0 ** -18 * (1 + top)) * mag + cap * 127 * 2.0 ** -21 * largest + TINY[q.dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [0, 10, 14, 20, 40])
+@pytest.mark.parametrize("tokens,width", [(1, 64), (1, 128), (1, 256), (4, 128), (140, 64), (140, 128), (140, 256)])
+def test_kv_attention_value_scales_far_apart(tokens, width, gap):
+    """Blocks whose value scale is 2^gap times the others' and whose keys get
+    next to no weight: what they add to a row is below 2^-20 of it."""
+    g = gen(gap + tokens)
+    b, heads, group, cap = 2, 2, 4, 640
+    codes, scale = cache_state(g, b, cap, heads, width)
+    loud = torch.zeros(cap // 16, dtype=torch.bool)
+    loud[[0, 3, 4, 17, 38]] = True
+    codes[0, ..., 0] = torch.where(loud.repeat_interleave(16), -127, 127).to(torch.int8)[None, :, None]
+    scale[0] = 0.02
+    scale[1] = torch.where(loud, scale[1] * 2.0 ** gap, scale[1])
+    q = 0.3 * randn(g, b, tokens, heads * group, width)
+    q[..., 0] = 8
+    n = torch.tensor([633, 320], dtype=torch.int32)
+    q = q.bfloat16()
+    shift = (gap + 24) * math.log(2) / (8 * 2 * 127 * 0.02)  # loud keys' scores lie gap + 24 bits below the others'
+    want, tol = attention64_rows(q, codes, scale, n, False, shift)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    out = w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), softmax_scale=shift)
+    within(out, want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [14, 20, 40, math.nan, math.inf])
+@pytest.mark.parametrize("tokens,width", [(4, 64), (4, 256), (5, 128), (140, 64), (140, 128), (140, 256)])
+def test_kv_attention_value_scales_that_a_row_does_not_see(tokens, width, gap):
+    """Causal: the blocks of the last tokens have value scales 2^gap times the
+    others', or ones that are not finite.  Rows before them are what they are
+    without, and rows that see them are right or not finite."""
+    g = gen(tokens)
+    b, heads, group, cap = 2, 1, 2, 320
+    codes, scale = cache_state(g, b, cap, heads, width)
+    q = randn(g, b, tokens, heads * group, width).bfloat16()
+    n = torch.tensor([305, 161], dtype=torch.int32)  # the last token begins a block
+    first = (n.long() - 1) // 16 * 16 if tokens < 100 else (n.long() - 70) // 16 * 16
+    factor = 2.0 ** gap if math.isfinite(gap) else gap
+    for i in range(b):
+        scale[1, i, :, first[i] // 16:] *= factor
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    out = w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), causal=True)
+    want, tol = attention64_rows(q, codes, scale, n, True, width ** -0.5)
+    sees = n.long()[:, None] - tokens + 1 + torch.arange(tokens) > first[:, None]
+    assert sees.any(1).all() and (~sees).any(1).all()
+    within(out.cpu()[~sees], want[~sees], tol[~sees])
+    if math.isfinite(factor):
+        within(out, want, tol)
+    else:
+        assert not torch.isfinite(out.cpu()[sees]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,width", [(1, 64), (1, 128), (1, 256), (140, 64), (140, 128), (140, 256)])
+def test_kv_attention_values_of_zero_that_get_nearly_all_weight(tokens, width):
+    """Blocks of zero values whose scores lie 60 bits above the others': the
+    result is the others' share, 2^-60 of their values."""
+    g = gen(width + tokens)
+    b, heads, group, cap = 1, 1, 8, 208
+    codes, scale = cache_state(g, b, cap, heads, width)
+    zero = torch.zeros(cap // 16, dtype=torch.bool)
+    zero[[1, 6]] = True
+    codes[0, ..., 0] = torch.where(zero.repeat_interleave(16), 127, -127).to(torch.int8)[None, :, None]
+    scale[0] = 0.02
+    scale[1, ..., zero] = 0
+    q = 0.3 * randn(g, b, tokens, heads * group, width)
+    q[..., 0] = 8
+    q = q.bfloat16()
+    n = torch.tensor([200], dtype=torch.int32)
+    s = 60 * math.log(2) / (8 * 2 * 127 * 0.02)
+    want, tol = attention64_rows(q, codes, scale, n, False, s)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    within(w8a8.kv_attention(on_gpu(q), cache, on_gpu(n), softmax_scale=s), want, tol)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 140])
+@pytest.mark.parametrize("size", [1e-30, 1e-36, 1e30])
+def test_kv_attention_value_scales_of_any_size(tokens, size):
+    g = gen(tokens)
+    codes, scale = cache_state(g, 1, 320, 1, 128)
+    scale[1] *= size * 100
+    q = randn(g, 1, tokens, 2, 128).bfloat16()
+    n = torch.tensor([311], dtype=torch.int32)
+    want, tol = attention64_rows(q, codes, scale, n, False, 128 ** -0.5)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    within(w8a8.kv_attention(on_gpu(q), cache, on_gpu(n)), want, tol)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [1, 70])
 def test_kv_attention_strides_and_sentinel_lengths(tokens):
