@@ -1,7 +1,8 @@
 // Rows in signed 8 bits with one fp32 scale each: the input side of the
 // int8 matrix product (gemm8.cuh).
 //
-// For a row v of h values: scale = fl(amax|v| / 127), codes = rint(v / scale).
+// For a row v of h values, in fp32: scale = amax|v| * fl(1 / 127), codes =
+// rint(v / scale), the quotient rounded as a division does and ties to even.
 // The row kernels differ in where v comes from:
 //   kRowQuant  v = x
 //   kRowGeglu  v = gelu_tanh(x) * up
@@ -17,11 +18,10 @@
 // reductions, one CTA of h / (8 VPT) threads to a row; a CTA takes several rows
 // in turn, and asks for the next one's vectors before it reduces this one, so
 // that loads are under way all the time.  The arithmetic is two lanes wide
-// (f32x2) and codes come from one multiply-add, as at the memory's rate there
-// are about 25 issue slots for an element of the GeGLU.  Measured: norm of 49,664
-// x 2,048 with residual 116 us (6.16 TB/s of 6.53; 153 us with fp32 one at a time
-// and no look ahead), GeGLU of 6,208 x 16,384 88 us (5.8 TB/s), codes of 6,208 x
-// 2,048 7.7 us, of one row 1.4 us.
+// (f32x2), as at the memory's rate there are about 25 issue slots for an element
+// of the GeGLU.  Measured: norm of 49,664 x 2,048 with residual 118 us (6.03 TB/s of
+// 6.53), GeGLU of 6,208 x 16,384 93 us (5.5 TB/s), codes of 6,208 x 2,048 8.4 us, of
+// one row 1.5 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -132,26 +132,48 @@ __device__ __forceinline__ float2 gelu_tanh_f32x2(float2 x) {
   return __fmul2_rn(x, make_float2(fast_rcp(d.x), fast_rcp(d.y)));
 }
 
-// How codes of a value are formed from a row's scale.  fast: v / scale rounded
-// by the addition of 1.5 x 2^23, whose sum holds the code in its low byte (a
-// value within an ulp of a tie may go to the other side; |v| <= 127.0001 scale,
-// so nothing needs a clamp).  Scales that are zero, not finite, or so small
-// that the reciprocal overflows take the slow way.
+// How codes of a value are formed from a row's scale.  fast: the quotient from
+// the reciprocal y, q0 = v y, corrected by its residual, q = q0 + (v - q0 scale) y
+// (Markstein, IBM J. Res. Dev. 34, 1990), and rounded by the addition of 1.5 x
+// 2^23, whose sum holds the code in its low byte (|v| <= 127.0001 scale, so
+// nothing needs a clamp).  Checked for every mantissa of the scale and every v
+// within 6 ulp of a tie: q is the quotient that a division rounds to.  q0 alone
+// is on the wrong side of ties, of which 16-bit values have many (an element
+// that is half of the row's largest).  Measured: 6,208 x 2,048 8.4 us, with q0
+// alone 7.7, with a division where one of a thread's values is near a tie 16.0.  Scales
+// that are zero, not finite, or whose reciprocal or residual leaves the normal
+// numbers are divided by.
 struct Coder {
   float mul, div;
   bool fast;
   __device__ __forceinline__ explicit Coder(float scale) {
     const bool finite = scale <= 3.4028234e38f;  // false for NaN
-    const bool tiny = scale < 7.8886091e-31f;    // 2^-100
-    fast = finite && !tiny;
+    fast = scale >= 7.8886091e-31f && scale <= 4.2535296e37f;  // 2^-100, 2^125
     mul = fast ? __frcp_rn(scale) : 0.f;
     div = finite && scale > 0.f ? scale : 0.f;
   }
-  // the code in the low byte
-  __device__ __forceinline__ uint32_t quick(float v) const { return __float_as_uint(fmaf(v, mul, 12582912.f)); }
   __device__ __forceinline__ uint32_t slow(float v) const {
     const float t = div > 0.f ? __fdiv_rn(v, div) : 0.f;
     return t == t ? static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(t, -127.f), 127.f))) : 0u;
+  }
+  // the codes of N values in the low bytes of c
+  template <int N>
+  __device__ __forceinline__ void codes(const float (&v)[N], uint32_t (&c)[N]) const {
+    if (!fast) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) c[i] = slow(v[i]);
+      return;
+    }
+    constexpr float kMagic = 12582912.f;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float2 y = make_float2(mul, mul), x = make_float2(v[i], i + 1 < N ? v[i + 1] : 0.f);
+      const float2 q0 = __fmul2_rn(x, y);
+      const float2 q = __ffma2_rn(__ffma2_rn(q0, make_float2(-div, -div), x), y, q0);
+      const float2 u = __fadd2_rn(q, make_float2(kMagic, kMagic));
+      c[i] = __float_as_uint(u.x);
+      if (i + 1 < N) c[i + 1] = __float_as_uint(u.y);
+    }
   }
 };
 
@@ -162,13 +184,7 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
 // Eight codes.
 __device__ __forceinline__ void store_codes(int8_t* p, const float (&v)[8], const Coder& code) {
   uint32_t c[8];
-  if (code.fast) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code.quick(v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code.slow(v[i]);
-  }
+  code.codes(v, c);
   *reinterpret_cast<uint2*>(p) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
 }
 
@@ -433,12 +449,14 @@ __global__ void __launch_bounds__(kRow8AnyThreads) row8_any_kernel(const __grid_
   const Coder code(scale);
 #pragma unroll 4
   for (int e = W * threadIdx.x; e < p.h; e += W * blockDim.x) {
-    struct alignas(W) Bytes { int8_t x[W]; } c;
+    struct alignas(W) Bytes { int8_t x[W]; } bytes;
     float v[W];
+    uint32_t c[W];
     load_few<W>(row8_smem + e, v);
+    code.codes(v, c);
 #pragma unroll
-    for (int i = 0; i < W; ++i) c.x[i] = static_cast<int8_t>(code.fast ? code.quick(v[i]) : code.slow(v[i]));
-    *reinterpret_cast<Bytes*>(p.codes + row * p.ldc + e) = c;
+    for (int i = 0; i < W; ++i) bytes.x[i] = static_cast<int8_t>(c[i]);
+    *reinterpret_cast<Bytes*>(p.codes + row * p.ldc + e) = bytes;
   }
   if (threadIdx.x == 0) p.scale[row] = scale;
 }

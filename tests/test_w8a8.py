@@ -178,6 +178,39 @@ def test_quantize(m, h, dtype, geglu):
     within(back, exact, (U[dtype] + 2.0 ** -23) * exact.abs() + TINY[dtype])
 
 
+def codes_plain(x):
+    """(codes, scale) in the fp32 steps that the operator defines."""
+    x = x.float()
+    scale = x.abs().amax(-1) * (torch.tensor(1.0) / 127)
+    return (x / scale[:, None]).round().clamp(-127, 127).to(torch.int8), scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("h", [17, 18, 20, 64, 2048, 2050])
+def test_quantize_codes_at_ties(h, dtype):
+    """Rows of every mantissa of the largest element (of 1,024 in fp32), with
+    elements at its half, quarter and other multiples, and (fp32) at and next
+    to every tie: the codes of the division, bit for bit."""
+    g = gen(h)
+    rows = 128 if dtype == torch.bfloat16 else 1024
+    top = (1 + torch.arange(rows) / rows) * 2.0 ** torch.randint(-8, 9, (rows,), generator=g)
+    x = (2 * torch.rand(rows, h, generator=g) - 1) * top[:, None]
+    share = torch.tensor([1, -0.5, 0.5, 0.25, -0.75, 0.125, 0.375])
+    x[:, :7] = top[:, None] * share
+    if dtype == torch.float32:
+        tie = (torch.randint(0, 127, (rows, h - 7), generator=g) + 0.5) * codes_plain(x)[1][:, None]
+        beside = torch.randint(-1, 2, tie.shape, generator=g, dtype=torch.int32)
+        tie = (tie.view(torch.int32) + beside).view(torch.float32) * (2 * torch.randint(0, 2, tie.shape, generator=g) - 1)
+        x[:, 7:] = torch.where(tie.abs() <= top[:, None], tie, x[:, 7:])
+    x = x.to(dtype)
+    want_codes, want_scale = codes_plain(x)
+    for n in (rows, 5):  # many rows and few take different kernels
+        codes, scale = w8a8.quantize(on_gpu(x[:n].contiguous()))
+        assert torch.equal(scale.cpu(), want_scale[:n])
+        assert torch.equal(codes.cpu(), want_codes[:n])
+
+
 # --------------------------------------------------------------- linear
 LINEAR_CASES = [
     # m, n, k, dtype, bias
