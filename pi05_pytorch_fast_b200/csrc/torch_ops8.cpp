@@ -10,6 +10,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/AutogradState.h>
 #include <c10/util/Exception.h>
 
 #include <cstdint>
@@ -48,10 +49,13 @@ void check_device(const Tensor& t, const Tensor& x, const char* what) {
   TORCH_CHECK(t.device() == x.device(), what, " is on ", t.device(), " but the input is on ", x.device());
 }
 
-// The results have no gradient: an input that wants one would silently lose it.
+// The results have no gradient: an input that wants one, or that carries a
+// forward-mode tangent, would silently lose it.
 void check_no_gradient(const Tensor& t, const char* what) {
   TORCH_CHECK(!t.requires_grad() || !at::GradMode::is_enabled(),
               "the pi05_w8a8 ops have no gradient, but ", what, " requires one: call them under torch.no_grad()");
+  TORCH_CHECK(!t._fw_grad(/*level=*/0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(),
+              "the pi05_w8a8 ops have no gradient, but ", what, " carries a forward-mode tangent: give them its primal");
 }
 
 int32_t as_i32(int64_t v, const char* what) {
@@ -120,6 +124,7 @@ Param param(const OptTensor& p, const Tensor& x, at::ScalarType type, const char
   if (!p.has_value()) return r;
   const int64_t h = x.size(-1);
   check_device(*p, x, what);
+  check_no_gradient(*p, what);
   TORCH_CHECK(p->scalar_type() == type, what, " must be ", type, ", got ", p->scalar_type());
   const bool per_obs = p->dim() == 2;
   TORCH_CHECK((p->dim() == 1 || (per_obs && x.dim() >= 2 && p->size(0) == x.size(0))) && p->size(-1) == h, what,
@@ -196,6 +201,7 @@ Rows check_codes(const Tensor& codes, const Tensor& scale, const char* what, con
   TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.numel() == m && scale.is_contiguous(), scale_what,
               " must be contiguous float32 with one value per row (", m, "), got ", scale.sizes(), " ",
               scale.scalar_type());
+  check_no_gradient(scale, scale_what);
   return rows_of(codes);
 }
 
@@ -246,6 +252,7 @@ Tensor linear(const Tensor& codes, const Tensor& scale, const Tensor& weight, co
     check_device(*bias, codes, "bias");
     TORCH_CHECK(bias->scalar_type() == dtype && bias->dim() == 1 && bias->size(0) == n && bias->is_contiguous(),
                 "bias must be contiguous ", dtype, " [", n, "], got ", bias->sizes(), " ", bias->scalar_type());
+    check_no_gradient(*bias, "bias");
   }
   std::vector<int64_t> shape(codes.sizes().begin(), codes.sizes().end());
   shape.back() = n;
@@ -284,6 +291,7 @@ Cache check_cache(const Tensor& k, const Tensor& v, const Tensor& ks, const Tens
                     s->size(1) == c.heads && s->size(2) == c.capacity / kBlock,
                 "cache scales must be contiguous float32 [batch, heads, capacity / ", kBlock, "], got ", s->sizes(), " ",
                 s->scalar_type());
+    check_no_gradient(*s, "a cache scale");
   }
   return c;
 }

@@ -10,8 +10,9 @@ cache as int8 codes with fp32 scales.
   bits with a scale for each block of 16 tokens and head, and attention over it
 
 Importing registers the ``pi05_w8a8::*`` custom ops (bodies in C++,
-``csrc/torch_ops8.cpp``).  Inference only: no op has a gradient, and an input that
-requires one is refused outside ``torch.no_grad()``.
+``csrc/torch_ops8.cpp``).  Inference only: no op has a gradient.  An input (scales,
+gain, shift, gate and bias as well) that requires one is refused outside
+``torch.no_grad()``, one with a forward-mode tangent everywhere.
 """
 
 from .extension import (

@@ -937,6 +937,57 @@ def test_ops_refuse_inputs_that_want_a_gradient():
     assert w8a8.pack_weight(torch.nn.Parameter(torch.ones(8, 64, device=DEV))).codes.shape == (8, 64)
 
 
+def _float_inputs():
+    """Every floating-point input of every op: (name, a value, the call with it in that place)."""
+    g = gen(60)
+    x = on_gpu(randn(g, 2, 1, 64).half())
+    gain, shift, gate = torch.ones(64, device=DEV), torch.zeros(2, 64, device=DEV), torch.ones(2, 64, device=DEV).half()
+    codes, scale = w8a8.quantize(x)
+    weight = w8a8.pack_weight(on_gpu(randn(g, 8, 64).half()))
+    bias = torch.zeros(8, dtype=torch.float16, device=DEV)
+    cache, n = w8a8.KVCache8.allocate(1, 16, 1, 64, DEV), torch.ones(1, dtype=torch.int32, device=DEV)
+    kv = on_gpu(randn(g, 1, 1, 1, 64).half())
+    f16 = dict(dtype=torch.float16)
+    norm = lambda **k: w8a8.rms_norm_quant(**{**dict(x=x, gain=gain, delta=x, gate=gate, shift=shift), **k})  # noqa: E731
+    put = lambda t, i: cache._replace(**{("key_scale", "value_scale")[i]: t})  # noqa: E731
+    return [
+        ("x", x, lambda t: norm(x=t)), ("gain", gain, lambda t: norm(gain=t)), ("delta", x, lambda t: norm(delta=t)),
+        ("gate", gate, lambda t: norm(gate=t)), ("shift", shift, lambda t: norm(shift=t)),
+        ("x", x, lambda t: w8a8.quantize(t)), ("up", x, lambda t: w8a8.quantize(x, up=t)),
+        ("scale", scale, lambda t: w8a8.dequantize(codes, t)),
+        ("scale", scale, lambda t: w8a8.linear(codes, t, weight, **f16)),
+        ("weight_scale", weight.scale, lambda t: w8a8.linear(codes, scale, weight._replace(scale=t), **f16)),
+        ("bias", bias, lambda t: w8a8.linear(codes, scale, weight, bias=t, **f16)),
+        ("new keys", kv, lambda t: w8a8.kv_append(cache, t, kv, n)), ("new values", kv, lambda t: w8a8.kv_append(cache, kv, t, n)),
+        ("q", kv, lambda t: w8a8.kv_attention(t, cache, n)),
+        *[("cache scale", cache.key_scale, lambda t, i=i, op=op: op(put(t, i))) for i in (0, 1) for op in (
+            lambda c: w8a8.kv_append(c, kv, kv, n), lambda c: w8a8.kv_values(c, n), lambda c: w8a8.kv_attention(kv, c, n))],
+    ]
+
+
+@pytest.mark.gpu
+def test_ops_refuse_a_gradient_of_any_input():
+    for name, value, call in _float_inputs():
+        wants = value.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match=name + " requires one"):
+            call(wants)
+        with torch.no_grad():
+            call(wants)
+        call(wants.detach())
+
+
+@pytest.mark.gpu
+def test_ops_refuse_forward_mode_tangents():
+    import torch.autograd.forward_ad as fwd
+
+    for name, value, call in _float_inputs():
+        with fwd.dual_level():
+            dual = fwd.make_dual(value.clone(), torch.ones_like(value))
+            with pytest.raises(RuntimeError, match=name + " carries a forward-mode tangent"):
+                call(dual)
+            call(fwd.unpack_dual(dual).primal)
+
+
 # --- the operators together: the SnapFlow action expert in 8 bits -----------
 
 
