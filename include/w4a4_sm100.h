@@ -369,6 +369,17 @@ int w4a4_dequant8(const int8_t* codes, int64_t ldc, const float* scale, int32_t 
 int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, int64_t ldw, const float* sw,
                const void* bias, int32_t dtype, int64_t m, int32_t n, int32_t k, void* y, void* stream);
 
+/* Test hook (host only, no GPU needed): how w4a4_gemm8 would run m tokens on a
+ * device that runs clusters[i] clusters of 1 << i CTAs at once (i = 0 .. 3, one
+ * CTA to an SM).  out[4] receives the kernel (W4A4_GEMM8_*), its token tile, the
+ * CTAs that share K, and the grid size. */
+#define W4A4_GEMM8_FEW 0      /* up to 16 tokens                               */
+#define W4A4_GEMM8_FEW_WIDE 1 /* of them, many channels: 16 to a CTA           */
+#define W4A4_GEMM8_FEW_DEEP 2 /* of them, a long K: 16 warps to a CTA          */
+#define W4A4_GEMM8_TILE 3     /* a tile a cluster, K split over its CTAs       */
+#define W4A4_GEMM8_PAIR 4     /* persistent CTA pairs                          */
+int w4a4_gemm8_plan(int64_t m, int32_t n, int32_t k, const int32_t* clusters, int32_t* out);
+
 /* The 8-bit cache: codes int8 [batch, capacity, heads, width] for keys and
  * values (cache_stride: elements of batch, token, head; multiples of 16),
  * scales fp32 [batch, heads, capacity / 16] contiguous; width 64, 128 or 256,

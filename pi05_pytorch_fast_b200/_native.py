@@ -62,6 +62,7 @@ EXPORTED_SYMBOLS = (
     "w4a4_quant8",
     "w4a4_dequant8",
     "w4a4_gemm8",
+    "w4a4_gemm8_plan",
     "w4a4_kv8_append",
     "w4a4_kv8_values",
     "w4a4_attention8",
@@ -131,6 +132,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.w4a4_quant8.argtypes = [vp, c_i64, vp, c_i64, c_i32, c_i64, c_i32, vp, c_i64, vp, vp]
     lib.w4a4_dequant8.argtypes = [vp, c_i64, vp, c_i32, c_i64, c_i32, vp, vp]
     lib.w4a4_gemm8.argtypes = [vp, c_i64, vp, vp, c_i64, vp, vp, c_i32, c_i64, c_i32, c_i32, vp, vp]
+    lib.w4a4_gemm8_plan.argtypes = [c_i64, c_i32, c_i32, ctypes.POINTER(c_i32), ctypes.POINTER(c_i32)]
     lib.w4a4_kv8_append.argtypes = [vp, vp, vp, vp, strides, c_i32, vp, strides, vp, strides, c_i32, vp, c_i64, vp, vp,
                                     c_i32, c_i32, c_i32, c_i32, vp]
     lib.w4a4_kv8_values.argtypes = [vp, vp, vp, vp, strides, c_i32, vp, c_i32, c_i32, c_i32, c_i32, vp, vp, vp]
@@ -204,6 +206,15 @@ def gemm_plan(m: int, k: int, ns, sms: int = 148, variant: int = GEMM_SINGLE_CTA
     check(lib().w4a4_gemm_plan(m, k, len(ns), n_arr, sms, variant, layout, out))
     return {"tok_tile": out[0], "split": bool(out[1]), "grid": out[2], "tok_tiles": out[3],
             "tok_group": out[4], "w_tiles": out[5]}
+
+
+def gemm8_plan(m: int, n: int, k: int, clusters=(148, 74, 33, 15)) -> dict:
+    """How w4a4_gemm8 would run (host computation, no GPU); clusters: how many
+    of 1, 2, 4 and 8 CTAs the device runs at once (a B200's)."""
+    fit, out = (ctypes.c_int32 * 4)(*clusters), (ctypes.c_int32 * 4)()
+    check(lib().w4a4_gemm8_plan(m, n, k, fit, out))
+    return {"kernel": ("few", "few_wide", "few_deep", "tile", "pair")[out[0]], "tok_tile": out[1], "split": out[2],
+            "grid": out[3]}
 
 
 def attn_vt_stride(seq: int) -> int:

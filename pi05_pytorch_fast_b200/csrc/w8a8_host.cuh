@@ -188,6 +188,20 @@ Gemm8Plan gemm8_plan(int64_t m, int n, int k, const int (&fit)[4]) {
   return best;
 }
 
+// The launch shape for up to 16 tokens.  16 channels a CTA where that leaves enough CTAs (the tokens are read half as
+// often; 1 x 2,048 x 32,768: 17.1 us, with 8 channels 19.0), and twice the warps, to have enough loads under way, where
+// there are few CTAs and a long K (16 x 16,384 x 2,048: 9.6 us, with 8 warps 16.1); half the MMA's rows for up to 8 tokens
+// (1 x 16,384 x 2,048: 11.6 us, with all of them and 8 warps 14.8).
+struct Gemm8FewPlan {
+  bool half, wide, deep;
+  int ctas, threads;
+};
+Gemm8FewPlan gemm8_few_plan(int64_t m, int n, int k, int sms) {
+  const bool wide = n >= 32 * sms, deep = !wide && k >= 4096;
+  const int per = wide ? 16 : 8;
+  return {m <= 8, wide, deep, (n + per - 1) / per, deep ? 512 : 256};
+}
+
 // Clusters of 1, 2, 4 and 8 CTAs that the device runs at once with one CTA to an SM.
 int g_cluster_fit[kMaxDevices][4];
 int cluster_fit(int dev, int (&fit)[4]) {
@@ -231,18 +245,15 @@ int launch_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w,
     const Gemm8FewParams f{a, w, sa, sw, bias, y, lda, ldw, static_cast<int>(m), n, k};
     return by_dtype(dtype, true, "gemm8", [&](auto tag) {
       using T = decltype(tag);
-      // 16 channels a CTA where that leaves enough CTAs (the tokens are read half as often; 1 x 2,048 x 32,768: 17.1 us,
-      // with 8 channels 19.0), and twice the warps, to have enough loads under way, where there are few CTAs and a long
-      // K (16 x 16,384 x 2,048: 9.6 us, with 8 warps 16.1); half the MMA's rows for up to 8 tokens (1 x 16,384 x 2,048:
-      // 11.6 us, with all of them and 8 warps 14.8)
-      const bool wide = n >= 32 * sms, deep = !wide && k >= 4096;
+      const Gemm8FewPlan plan = gemm8_few_plan(m, n, k, sms);
       const auto by_shape = [&](auto half_tag) {
         constexpr bool H = decltype(half_tag)::value;
-        return deep ? gemm8_few_kernel<T, H, 1, 16> : wide ? gemm8_few_kernel<T, H, 2, 8> : gemm8_few_kernel<T, H, 1, 8>;
+        return plan.deep   ? gemm8_few_kernel<T, H, 1, 16>
+               : plan.wide ? gemm8_few_kernel<T, H, 2, 8>
+                           : gemm8_few_kernel<T, H, 1, 8>;
       };
-      const auto kernel = m <= 8 ? by_shape(std::true_type{}) : by_shape(std::false_type{});
-      const int per = wide ? 16 : 8;
-      W4A4_CUDA_TRY(launch_kernel(kernel, dim3((n + per - 1) / per), dim3(deep ? 512 : 256), 0, stream, 1, f));
+      const auto kernel = plan.half ? by_shape(std::true_type{}) : by_shape(std::false_type{});
+      W4A4_CUDA_TRY(launch_kernel(kernel, dim3(plan.ctas), dim3(plan.threads), 0, stream, 1, f));
       return ok();
     });
   }
@@ -471,6 +482,25 @@ int w4a4_gemm8(const int8_t* a, int64_t lda, const float* sa, const int8_t* w, i
   if (!aligned(y, 16) || (bias && !aligned(bias, 16)))
     return fail(W4A4_ERR_INVALID, "gemm8: y and bias must be 16-byte aligned");
   return launch_gemm8(a, lda, sa, w, ldw, sw, bias, dtype, m, n, k, y, static_cast<cudaStream_t>(stream));
+}
+
+int w4a4_gemm8_plan(int64_t m, int32_t n, int32_t k, const int32_t* clusters, int32_t* out) {
+  if (m <= 0 || m > 0x7fffff00LL || n <= 0 || k <= 0 || k >= 131072 || !clusters || !out)
+    return fail(W4A4_ERR_INVALID, "gemm8: invalid plan query");
+  const int fit[4] = {clusters[0], clusters[1], clusters[2], clusters[3]};
+  if (fit[0] < 2 || fit[1] < 1 || fit[2] < 0 || fit[3] < 0) return fail(W4A4_ERR_INVALID, "gemm8: invalid plan query");
+  if (m <= kG8FewTokens) {
+    const Gemm8FewPlan plan = gemm8_few_plan(m, n, k, fit[0]);
+    out[0] = plan.deep ? W4A4_GEMM8_FEW_DEEP : plan.wide ? W4A4_GEMM8_FEW_WIDE : W4A4_GEMM8_FEW;
+    out[1] = plan.half ? 8 : 16, out[2] = 1, out[3] = plan.ctas;
+    return ok();
+  }
+  const Gemm8Plan plan = gemm8_plan(m, n, k, fit);
+  out[0] = plan.pair ? W4A4_GEMM8_PAIR : W4A4_GEMM8_TILE;
+  out[1] = plan.pair ? 256 : plan.tok_tile, out[2] = plan.split;
+  out[3] = plan.pair ? 2 * std::min(fit[0] / 2, plan.n_tok_tiles * plan.n_w_tiles)
+                     : plan.split * plan.n_tok_tiles * plan.n_w_tiles;
+  return ok();
 }
 
 int w4a4_kv8_append(int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale, const int64_t* cache_stride,

@@ -113,6 +113,31 @@ def test_rms_norm_quant(case):
     check_rows(codes, scale, y, tol)
 
 
+MANY_ROW_CASES = [
+    # more rows than CTAs of the kernel for them: a CTA takes several, of more than one observation
+    (1001, 5, 64, torch.float16, True, True, True),
+    (2003, 3, 512, torch.bfloat16, True, True, True),
+    (31, 129, 2048, torch.float16, True, False, True),
+    (9, 555, 1152, torch.bfloat16, False, False, True),
+    (7, 100, 24576, torch.bfloat16, True, True, True),
+    (5, 601, 328, torch.float32, True, True, False),
+    (3, 701, 1026, torch.float16, True, True, True),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_ROW_CASES)
+def test_rms_norm_quant_many_rows(case):
+    x, d, ga, gain, shift = norm_inputs(*case, seed=1)
+    z, y, tol, mag = norm64(x, d, ga, gain, shift, 1e-6)
+    codes, scale, total = w8a8.rms_norm_quant(on_gpu(x), on_gpu(gain), 1e-6, delta=on_gpu(d), gate=on_gpu(ga), shift=on_gpu(shift))
+    if d is not None:
+        within(total, z, U[x.dtype] * z.abs() + 2.0 ** -22 * mag + TINY[x.dtype])
+    check_rows(codes, scale, y, tol)
+    again = w8a8.rms_norm_quant(on_gpu(x), on_gpu(gain), 1e-6, delta=on_gpu(d), gate=on_gpu(ga), shift=on_gpu(shift))
+    assert torch.equal(codes, again[0]) and torch.equal(scale, again[1])
+
+
 @pytest.mark.gpu
 def test_rms_norm_quant_takes_strided_and_misaligned_rows():
     g = gen(3)
@@ -176,6 +201,23 @@ def test_quantize(m, h, dtype, geglu):
     assert back.is_contiguous() and back.dtype == dtype
     exact = codes.cpu().double() * scale.cpu().double()[:, None]
     within(back, exact, (U[dtype] + 2.0 ** -23) * exact.abs() + TINY[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("m,h", [(5005, 64), (6007, 512), (4003, 2048), (601, 24576), (2003, 2394)])
+def test_quantize_many_rows(m, h, dtype):
+    """More rows than CTAs: each row as if it were alone, plain and of the GeGLU."""
+    g = gen(m)
+    both = (2 * randn(g, m, 2 * h)).to(dtype)
+    big = on_gpu(both)
+    codes, scale = w8a8.quantize(big[:, :h])
+    want_codes, want_scale = codes_plain(both[:, :h])
+    assert torch.equal(codes.cpu(), want_codes) and torch.equal(scale.cpu(), want_scale)
+    x, up = both[:, :h].double(), both[:, h:].double()
+    u = 1.6 * (x.abs() + 0.044715 * x.abs() ** 3).clamp(max=88)  # as in test_quantize
+    v = gelu64(x) * up
+    check_rows(*w8a8.quantize(big[:, :h], up=big[:, h:]), v, v.abs() * (2.0 ** -20 + 2.0 ** -20 * u) + 1e-37 * up.abs())
 
 
 def codes_plain(x):
@@ -260,6 +302,59 @@ def test_linear(m, n, k, dtype, bias):
     within(y, want, U[dtype] * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -22 * mag + TINY[dtype])
     # the same call gives the same bits
     assert torch.equal(y, w8a8.linear(ag, on_gpu(sa), w8a8.Int8Weight(wg, on_gpu(sw)), bias=on_gpu(bi), dtype=dtype))
+    assert nat.device_error() == 0
+
+
+# shapes of the kernels for many tokens and many channels: rows of y at multiples of 16 bytes (TMA stores), of 8, 4 and 2;
+# token counts that end inside a tile; several tiles a pair of CTAs and less than one
+LARGE_LINEAR_CASES = [
+    (4097, 4096, 400, torch.float16, True),
+    (3003, 3004, 144, torch.float16, True),
+    (3003, 3002, 272, torch.bfloat16, False),
+    (3003, 3001, 130, torch.float16, True),
+    (3003, 3000, 400, torch.float32, True),
+    (3003, 3002, 144, torch.float32, False),
+    (3003, 3001, 144, torch.float32, True),
+    (9000, 1029, 528, torch.bfloat16, True),
+    (1600, 2048, 2064, torch.float16, False),
+    (3, 5001, 160, torch.float16, True),
+    (16, 4999, 130, torch.bfloat16, False),
+    (8, 4737, 64, torch.float32, True),
+    (2, 130, 4100, torch.bfloat16, True),
+    (11, 257, 4097, torch.float16, True),
+    (20, 64, 1024, torch.float16, True),
+    (40, 257, 2064, torch.bfloat16, True),
+]
+
+
+def test_linear_cases_reach_every_kernel():
+    plans = [nat.gemm8_plan(m, n, k) for m, n, k, _, _ in LINEAR_CASES + LARGE_LINEAR_CASES]
+    assert {p["kernel"] for p in plans} == {"few", "few_wide", "few_deep", "tile", "pair"}
+    assert {p["split"] for p in plans if p["kernel"] == "tile"} == {1, 2, 4, 8}
+    assert {p["tok_tile"] for p in plans if p["kernel"].startswith("few")} == {8, 16}
+    pairs = [(n * torch.finfo(t).bits // 8 % 16, t) for (m, n, k, t, _), p in
+             zip(LARGE_LINEAR_CASES, plans[len(LINEAR_CASES):]) if p["kernel"] == "pair"]
+    assert {r for r, t in pairs if t != torch.float32} >= {0, 2, 4, 8} and {r for r, t in pairs if t == torch.float32} >= {0, 4, 8}
+    for args in ((0, 8, 8), (4, 0, 8), (4, 8, 131072)):
+        with pytest.raises(nat.W4A4Error, match="plan query"):
+            nat.gemm8_plan(*args)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,dtype,bias", LARGE_LINEAR_CASES)
+def test_linear_large(m, n, k, dtype, bias):
+    g = gen(m + n + k)
+    a, w = on_gpu(codes_rows(g, m, k)), on_gpu(codes_rows(g, n, k, low=-128))
+    sa, sw = (torch.rand(m, generator=g) * 0.02 + 0.001), (torch.rand(n, generator=g) * 0.002 + 0.0001)
+    sa[m // 2] = 0
+    bi = on_gpu(randn(g, n).to(dtype)) if bias else None
+    want, mag = linear64(a, on_gpu(sa), w, on_gpu(sw), bi)
+    weight = w8a8.Int8Weight(w, on_gpu(sw))
+    y = w8a8.linear(a, on_gpu(sa), weight, bias=bi, dtype=dtype)
+    err = (y.double() - want).abs()
+    tol = U[dtype] * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -22 * mag + TINY[dtype]
+    assert torch.isfinite(err).all() and (err <= tol).all(), f"{int((err > tol).sum())} of {err.numel()} too far"
+    assert torch.equal(y, w8a8.linear(a, on_gpu(sa), weight, bias=bi, dtype=dtype))
     assert nat.device_error() == 0
 
 
