@@ -33,11 +33,13 @@
 
 namespace w4a4 {
 
-// At least 117 KB of shared memory for a CTA with TMEM, so that no two of them
-// share an SM: a CTA of a cluster that waited for columns which another
-// cluster's CTA holds could wait for good, each cluster's other half being
-// blocked by the other.
-constexpr int kOneCtaSmem = 117 * 1024;
+// At least 160 KB of shared memory for a CTA with TMEM, so that no other one of
+// this library shares its SM, the 4-bit products with their narrowest tiles (71 KB)
+// among them.  A CTA that waits for columns waits without a limit, and could for
+// good: two clusters (of two streams), each with one half's columns taken by the
+// other; or a kernel that has let its dependents start and asks for its columns
+// only then, which a dependent holds until that kernel is over.
+constexpr int kOneCtaSmem = 160 * 1024;
 constexpr float kAttn8Margin = 4.f;    // log2 by which m and r are set above a row's maxima
 constexpr float kAttn8Grow = 11.f;     // log2 by which a block may exceed them
 

@@ -11,6 +11,16 @@
 namespace w4a4 {
 namespace {
 
+// No kernel with TMEM fits beside one of these on an SM (kOneCtaSmem).
+constexpr int kSmSharedMemory = 228 * 1024, kCtaReserved = 1024;
+constexpr bool fits_beside(int bytes) { return kOneCtaSmem + bytes + 2 * kCtaReserved <= kSmSharedMemory; }
+static_assert(!fits_beside(kOneCtaSmem) && !fits_beside(gemm_smem_bytes(16)) && !fits_beside(gemm_pair_smem_bytes(16)) &&
+                  !fits_beside(gemm_pair_i8_smem_bytes(16)) && !fits_beside(kAttnSmem),
+              "a kernel with TMEM could share an SM with an 8-bit one");
+static_assert(gemm8_tile_smem(16, 1, false) >= kOneCtaSmem && kG8PairSmem >= kOneCtaSmem &&
+                  Attn8Many<64>::kSmem >= kOneCtaSmem && Attn8Many<256>::kSmem >= kOneCtaSmem,
+              "every 8-bit kernel with TMEM has its SM to itself");
+
 // Calls f with a value of the element type that `dtype` names.
 template <class F>
 int by_dtype(int32_t dtype, bool fp32_too, const char* what, F f) {

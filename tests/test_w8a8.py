@@ -857,6 +857,49 @@ def test_operators_follow_the_current_stream():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("variant", [nat.GEMM_CTA_PAIR, nat.GEMM_SPLIT_K, nat.GEMM_NO_SPLIT])
+def test_operators_beside_four_bit_products(variant):
+    """Few-token 4-bit products (CTA pairs, split K) and 8-bit kernels with
+    tensor memory: one after the other in a stream, and on two streams."""
+    from pi05_pytorch_fast_b200 import w4a4
+
+    g = gen(70)
+    x = on_gpu(randn(g, 9, 2048).half())
+    packed = w4a4.pack_linear_weight(randn(g, 2048, 2048).float(), device=DEV)
+    x8 = on_gpu(randn(g, 40, 2048).half())
+    weight = w8a8.pack_weight(on_gpu(randn(g, 512, 2048).half()))
+    codes8, scale8 = w8a8.quantize(x8)
+    q, codes, scale, n = attention_inputs(8, 1, 64, 1024, (1024,) * 4, 20, torch.bfloat16, 71)
+    cache = w8a8.KVCache8(*(codes.to(DEV)), *(scale.to(DEV)))
+    qg, ng = on_gpu(q), on_gpu(n)
+
+    def four():
+        return w4a4.int4_gemm(x, packed)
+
+    def eight():
+        return w8a8.linear(codes8, scale8, weight), w8a8.kv_attention(qg, cache, ng)
+
+    try:
+        nat.set_gemm_variant(variant)
+        want4, want8 = four(), eight()
+        for _ in range(50):
+            got4, got8 = four(), eight()
+        assert torch.equal(got4, want4) and all(torch.equal(a, b) for a, b in zip(got8, want8))
+        torch.cuda.synchronize()
+        streams = torch.cuda.Stream(), torch.cuda.Stream()
+        for _ in range(50):
+            with torch.cuda.stream(streams[0]):
+                got4 = four()
+            with torch.cuda.stream(streams[1]):
+                got8 = eight()
+        torch.cuda.synchronize()
+        assert torch.equal(got4, want4) and all(torch.equal(a, b) for a, b in zip(got8, want8))
+        assert nat.device_error() == 0
+    finally:
+        nat.set_gemm_variant(nat.GEMM_SINGLE_CTA)
+
+
+@pytest.mark.gpu
 def test_operators_in_a_cuda_graph():
     g = gen(50)
     x = on_gpu(randn(g, 8, 1, 512).bfloat16())
