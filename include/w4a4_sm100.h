@@ -342,7 +342,7 @@ int w4a4_layer_norm_bf16(const void* x, void* y, int64_t rows, int32_t h, const 
 /* Residual addition + RMSNorm + 8-bit codes: per row
  *   s = x + gate * delta (delta NULL: s = x; gate NULL: 1), total = s rounded
  *   y = s rsqrt(mean(s^2) + eps) gain + shift (shift NULL: 0)
- *   scale = amax|y| / 127, codes = rint(y / scale)
+ *   scale = amax|y| * fl(1 / 127), codes = rint(y / scale)
  * x, delta and gate of type `dtype`, gain and shift fp32; gate, gain and shift
  * rows of h for each observation of rows_per_batch rows, `*_stride` elements
  * apart (0: one row for all).  total (NULL: not stored) is [rows, h]
@@ -354,7 +354,7 @@ int w4a4_rms_norm_quant8(const void* x, int64_t ldx, const void* delta, int64_t 
                          int32_t h, void* total, int8_t* codes, int64_t ldc, float* scale, void* stream);
 
 /* 8-bit codes of rows of x, or with `up` of gelu_tanh(x) * up: scale =
- * amax / 127, codes = rint(value / scale). */
+ * amax * fl(1 / 127), codes = rint(value / scale), both in fp32. */
 int w4a4_quant8(const void* x, int64_t ldx, const void* up, int64_t ldu, int32_t dtype, int64_t rows, int32_t h,
                 int8_t* codes, int64_t ldc, float* scale, void* stream);
 

@@ -144,8 +144,8 @@ __device__ __forceinline__ int keys_seen(const Attn8Params& p, int n, int t) {
 // in turns); m and l are each lane's own until the end.  Bound: HBM (2 width bytes per key); legacy MMA is enough
 // for it.  Which warp takes which keys does not depend on the lengths, so the
 // first loads are under way before the length has arrived.  Measured: 8 heads of
-// 256 over 776 tokens 7.5 us, over 131,072 (67 MB) 26.5 us; 4 x 16 heads on 2 of 128
-// over 65,536 (134 MB) 34.5 us: 5.4 to 6 TB/s once it streams.
+// 256 over 776 tokens 7.4 us, over 131,072 (67 MB) 26.3 us; 4 x 16 heads on 2 of 128
+// over 65,536 (134 MB) 33 to 34 us: 5.4 to 6 TB/s once it streams.
 template <int D, bool HALF>
 struct Attn8Few {
   static constexpr int kWarps = 8, kStages = 3;
@@ -594,8 +594,8 @@ __global__ void __launch_bounds__(Attn8Few<D, HALF>::kThreads, 1)
 // them, 256 x 80 for the converters, 128 x 56 for the rest).
 // At D = 256 a tile costs the tensor pipe 1024 cycles, shared memory 1280 (codes
 // read, fp16 written, operands read) and the exponentials (16 a cycle) 512;
-// measured are 2200 (512 tokens x 8 heads over 16,384: 120-126 us, tensor pipe
-// 34 %), and 1900 at D = 64: the chain of a tile is what bounds it.
+// measured are 3080 (512 tokens x 8 heads over 16,384: 114 to 118 us, tensor pipe
+// 38 %), 2120 at D = 128 and 1930 at D = 64: the chain of a tile is what bounds it.
 template <int D>
 struct Attn8Many {
   static constexpr int kRows = 128, kKeys = 64;

@@ -21,7 +21,7 @@
 // (f32x2), as at the memory's rate there are about 25 issue slots for an element
 // of the GeGLU.  Measured: norm of 49,664 x 2,048 with residual 118 us (6.03 TB/s of
 // 6.53), GeGLU of 6,208 x 16,384 93 us (5.5 TB/s), codes of 6,208 x 2,048 8.4 us, of
-// one row 1.5 us.
+// one row 1.4 us.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -368,8 +368,8 @@ __global__ void __launch_bounds__(MAXT, MINB) row8_kernel(const __grid_constant_
 // Any row: one, two or four elements at a time, the row's fp32 values in shared
 // memory between the passes.  For rows that do not begin at multiples of 16
 // bytes (a length that is not a multiple of 8), and for long ones.  Bound by the
-// instructions and latency of the narrow loads: 1,944 x 7,620 (by 4) 44 us, 4,464 x
-// 2,394 (by 2) 33 us, 6,208 x 2,047 codes (by 1) 28 us.  Vectors of 16 bytes from
+// instructions and latency of the narrow loads: 1,944 x 7,620 (by 4) 40 us, 4,464 x
+// 2,394 (by 2) 33 us, 6,208 x 2,047 codes (by 1) 29 us.  Vectors of 16 bytes from
 // the last multiple of 16 before each row on took 17 us for these codes, but 40
 // and 63 us for the two norms, whose operands lie differently; several steps'
 // loads at once took 42 us for 4,464 x 2,394.

@@ -125,7 +125,7 @@ def rms_norm_quant(x: torch.Tensor, gain: torch.Tensor, eps: float = 1e-6, *, de
                    gate: torch.Tensor | None = None, shift: torch.Tensor | None = None):
     """Residual addition, RMSNorm and 8-bit codes in one pass over x [..., h]:
     total = x + gate * delta; y = total * rsqrt(mean(total^2) + eps) * gain +
-    shift; scale = amax|y| / 127 per row; codes = rint(y / scale).
+    shift; scale = amax|y| * fl(1 / 127) per row; codes = rint(y / scale).
 
     x and delta (the sublayer's output) fp16, bf16 or fp32 of one shape; gain
     and shift fp32, gate of x's dtype, each [h], or [batch, h] for x [batch,
@@ -143,7 +143,7 @@ def quantize(x: torch.Tensor, up: torch.Tensor | None = None):
     """8-bit codes of the rows of x [..., h] (fp16, bf16, fp32), or with ``up``
     of gelu_tanh(x) * up (the input of a GeGLU's down projection; x and up may
     be the halves of one product).  Returns (codes int8 like x, scale fp32
-    [...]): scale = amax / 127, codes = rint(value / scale)."""
+    [...]): scale = amax * fl(1 / 127), codes = rint(value / scale) in fp32."""
     return _call("quantize", x, up)
 
 
